@@ -261,6 +261,108 @@ mg_status mg_gemm_bf16(const void *a_dev, int64_t lda, const void *b_dev, int64_
  * before any rank destroys its model, so no buffer is freed while mapped. */
 mg_status mg_tp_disconnect(mg_model *m);
 
+/* ---- paged key/value cache held in 8 bits (no counterpart in the reference,
+ * whose cache is one fp32 slab per layer, core.mojo:326-338) ----
+ * A cache of one layer is num_pages pages of page_size tokens (a power of two,
+ * 16..256).  Element (page, kv head, token, d) of K and of V is an e4m3 code at
+ * byte page * page_stride + head * head_stride + token * token_stride + d
+ * (strides in bytes, multiples of 16); every MG_KV8_BLOCK tokens of a page and
+ * head share one fp32 scale, [num_pages][num_kv_heads][page_size / 16] packed,
+ * for K and for V: value = code * scale.  head_dim is 64, 128 or 256.
+ *
+ * A batch names `batch` sequences.  Their new tokens are packed: sequence b has
+ * rows q_start[b] .. q_start[b + 1] - 1 (q_start_dev: [batch + 1], rising, the
+ * last at most total_q, the number of rows of the row tensors; rows behind it
+ * are not touched).  ctx_len[b] counts its positions with the new ones: its
+ * i-th new token is at position ctx_len[b] - q_len[b] + i.  Position p lives in
+ * page page_table[b * table_stride + p / page_size].  max_q and max_ctx bound
+ * every q_len and ctx_len (host values: the device arrays are not read on the
+ * host); max_ctx <= table_stride * page_size.
+ * All of it is read on the device when the kernels run, so a captured call may
+ * be replayed with new lengths, tables and rows within those bounds.
+ *
+ * err_dev is a device word that receives a nonzero code (the first one stays)
+ * when a length breaks the bounds or a page id is outside [0, num_pages): the
+ * tokens concerned are then neither stored nor seen; nothing outside the
+ * tensors is touched.
+ * Both calls run on `stream` (a cudaStream_t of the current device; NULL: the
+ * legacy default stream) without allocating or synchronising. */
+#define MG_KV8_BLOCK 16
+typedef struct mg_kv8_cache {
+    int32_t struct_size; /* sizeof(mg_kv8_cache) */
+    int32_t num_pages, page_size, num_kv_heads, head_dim;
+    int32_t reserved0;
+    void *k_dev, *v_dev;              /* 16-byte aligned */
+    float *k_scale_dev, *v_scale_dev; /* positive, finite */
+    int64_t page_stride, head_stride, token_stride;
+} mg_kv8_cache;
+typedef struct mg_kv8_batch {
+    int32_t struct_size; /* sizeof(mg_kv8_batch) */
+    int32_t batch, total_q, max_q, max_ctx;
+    int32_t reserved0;
+    const int32_t *q_start_dev, *ctx_len_dev, *page_table_dev;
+    int64_t table_stride; /* page ids per sequence */
+    uint32_t *err_dev;
+} mg_kv8_batch;
+
+/* Appends the batch's new keys and values, rotating on the way:
+ *   q_out = rope(norm(q)),  K <- rope(norm(k)),  V <- v   (fp32 arithmetic)
+ * norm(x) = x * rsqrt(mean(x^2) + 1e-6) * (1 + w) with q_norm / k_norm as w
+ * ([head_dim]; NULL: no norm); rope turns the pairs (i, i + head_dim / 2) by the
+ * position's row of cos / sin ([rope_len][head_dim / 2]; both NULL: no rotation;
+ * rope_len >= max_ctx).
+ * A block's scale becomes the smallest power of two (at least 2^-100) that
+ * holds its new values below 448 * scale, or stays if the block has earlier
+ * tokens under a larger one; earlier tokens are rounded again when it grows.
+ * A token whose key (after the rotation) or value has an infinity or NaN is
+ * stored as a key of NaN and a value of zero: every query that sees it answers
+ * NaN, and no other query or token is affected.
+ * q (num_heads of them, a multiple of num_kv_heads) may be absent: num_heads 0.
+ * q_out may be q itself.  Two tokens of one call must not share a cache slot,
+ * nor two sequences a block that the call writes.  Rows: element (row, head, d)
+ * at row * row_stride + head * head_stride + d (in elements, multiples of 4;
+ * data aligned to 4 elements).  dtype: MG_F32, MG_BF16 or MG_F16; out_dtype
+ * the same, for MG_F32 rows any of them. */
+typedef struct mg_kv8_append_args {
+    int32_t struct_size; /* sizeof(mg_kv8_append_args) */
+    int32_t dtype, out_dtype, num_heads, rope_len;
+    int32_t reserved0;
+    const void *q_dev, *k_dev, *v_dev;
+    void *q_out_dev;
+    int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int64_t out_row_stride, out_head_stride;
+    const float *q_norm_dev, *k_norm_dev, *cos_dev, *sin_dev;
+} mg_kv8_append_args;
+mg_status mg_kv8_append(const mg_kv8_cache *cache, const mg_kv8_batch *batch, const mg_kv8_append_args *args,
+                        void *stream);
+
+/* Attention of the batch's queries over the cache (their own tokens appended
+ * before): out = softmax(scale q K^T) V over the positions (p - window, p] of
+ * each query's position p (window 0: [0, p]), fp32 sums.  A query that sees
+ * nothing answers 0.  dtype of q and out: MG_BF16 or MG_F16; num_heads a
+ * multiple of num_kv_heads, at most 128 per kv head; rows as above with strides
+ * in multiples of 8 elements and 16-byte aligned data.
+ * V codes must be finite (the append writes no others); the cache's content
+ * behind ctx_len is never used.
+ * The workspace (16-byte aligned, mg_kv8_attention_workspace bytes on this
+ * device for these cache dimensions and bounds) needs no initial value and
+ * keeps nothing between calls: calls that may overlap need one each. */
+typedef struct mg_kv8_attention_args {
+    int32_t struct_size; /* sizeof(mg_kv8_attention_args) */
+    int32_t dtype, num_heads, window;
+    float scale;
+    int32_t reserved0;
+    const void *q_dev;
+    void *out_dev;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    void *workspace_dev;
+    int64_t workspace_bytes;
+} mg_kv8_attention_args;
+mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_batch *batch, const mg_kv8_attention_args *args,
+                           void *stream);
+mg_status mg_kv8_attention_workspace(const mg_kv8_cache *cache, const mg_kv8_batch *batch, int32_t num_heads,
+                                     int64_t *bytes_out);
+
 /* ---- Gemma 3n ("nano") decode ----
  * The reference switches to its nano graph when the checkpoint has AltUp
  * routers (src/mo/mogemma/core.mojo:26-31) and runs forward_nano_step

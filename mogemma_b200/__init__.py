@@ -10,9 +10,19 @@ from typing import TYPE_CHECKING
 if TYPE_CHECKING:
     from .config import EmbeddingConfig, GenerationConfig
     from .hub import HubManager
+    from .kv8 import KV8Batch, KV8Cache
     from .model import AsyncGemmaModel, EmbeddingModel, SyncGemmaModel
 
-__all__ = ["AsyncGemmaModel", "EmbeddingConfig", "EmbeddingModel", "GenerationConfig", "HubManager", "SyncGemmaModel"]
+__all__ = [
+    "AsyncGemmaModel",
+    "EmbeddingConfig",
+    "EmbeddingModel",
+    "GenerationConfig",
+    "HubManager",
+    "KV8Batch",
+    "KV8Cache",
+    "SyncGemmaModel",
+]
 
 _WHERE = {
     "AsyncGemmaModel": ".model",
@@ -20,6 +30,8 @@ _WHERE = {
     "EmbeddingModel": ".model",
     "GenerationConfig": ".config",
     "HubManager": ".hub",
+    "KV8Batch": ".kv8",
+    "KV8Cache": ".kv8",
     "SyncGemmaModel": ".model",
 }
 

@@ -113,6 +113,46 @@ class NanoInfo(ctypes.Structure):
         "per_layer_dim", "modalities", "laurel_rank", "kv_share_start", "max_seq_len")]
 
 
+class KV8CacheDesc(ctypes.Structure):
+    """``mg_kv8_cache``."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "struct_size", "num_pages", "page_size", "num_kv_heads", "head_dim", "reserved0")] + [
+        (n, ctypes.c_void_p) for n in ("k_dev", "v_dev", "k_scale_dev", "v_scale_dev")] + [
+        (n, ctypes.c_int64) for n in ("page_stride", "head_stride", "token_stride")]
+
+
+class KV8BatchDesc(ctypes.Structure):
+    """``mg_kv8_batch``."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "struct_size", "batch", "total_q", "max_q", "max_ctx", "reserved0")] + [
+        (n, ctypes.c_void_p) for n in ("q_start_dev", "ctx_len_dev", "page_table_dev")] + [
+        ("table_stride", ctypes.c_int64), ("err_dev", ctypes.c_void_p)]
+
+
+class KV8AppendArgs(ctypes.Structure):
+    """``mg_kv8_append_args``."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "struct_size", "dtype", "out_dtype", "num_heads", "rope_len", "reserved0")] + [
+        (n, ctypes.c_void_p) for n in ("q_dev", "k_dev", "v_dev", "q_out_dev")] + [
+        (n, ctypes.c_int64) for n in (
+            "q_row_stride", "q_head_stride", "k_row_stride", "k_head_stride", "v_row_stride", "v_head_stride",
+            "out_row_stride", "out_head_stride")] + [
+        (n, ctypes.c_void_p) for n in ("q_norm_dev", "k_norm_dev", "cos_dev", "sin_dev")]
+
+
+class KV8AttentionArgs(ctypes.Structure):
+    """``mg_kv8_attention_args``."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("struct_size", "dtype", "num_heads", "window")] + [
+        ("scale", ctypes.c_float), ("reserved0", ctypes.c_int32), ("q_dev", ctypes.c_void_p),
+        ("out_dev", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("q_row_stride", "q_head_stride", "out_row_stride", "out_head_stride")] + [
+        ("workspace_dev", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
 _P = ctypes.c_void_p
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _F32P = ctypes.POINTER(ctypes.c_float)
@@ -154,10 +194,16 @@ TP_HANDLE_BYTES = 64  # MG_TP_HANDLE_BYTES
 _lib.mg_trace_enable.argtypes = [_P, ctypes.c_int32]
 _lib.mg_trace_read.argtypes = [_P, ctypes.POINTER(ctypes.c_uint64), ctypes.c_int64, ctypes.POINTER(ctypes.c_int64)]
 _lib.mg_set_debug.argtypes = [_P, ctypes.c_uint64, ctypes.c_int32]
+_lib.mg_kv8_append.argtypes = [ctypes.POINTER(KV8CacheDesc), ctypes.POINTER(KV8BatchDesc),
+                               ctypes.POINTER(KV8AppendArgs), _P]
+_lib.mg_kv8_attention.argtypes = [ctypes.POINTER(KV8CacheDesc), ctypes.POINTER(KV8BatchDesc),
+                                  ctypes.POINTER(KV8AttentionArgs), _P]
+_lib.mg_kv8_attention_workspace.argtypes = [ctypes.POINTER(KV8CacheDesc), ctypes.POINTER(KV8BatchDesc),
+                                            ctypes.c_int32, ctypes.POINTER(ctypes.c_int64)]
 for _f in ("mg_model_create", "mg_model_info_get", "mg_model_destroy", "mg_set_pos", "mg_get_pos", "mg_step",
            "mg_prefill", "mg_generate", "mg_set_tokens", "mg_sample", "mg_embed", "mg_read_kv",
            "mg_tp_ipc_handle", "mg_tp_connect", "mg_tp_disconnect", "mg_encode", "mg_trace_enable", "mg_trace_read",
-           "mg_set_debug"):
+           "mg_set_debug", "mg_kv8_append", "mg_kv8_attention", "mg_kv8_attention_workspace"):
     getattr(_lib, _f).restype = ctypes.c_int
 
 

@@ -1,0 +1,222 @@
+// kv8.cuh -- the 8-bit paged key/value cache: what its append (kv8_append.cu)
+// and its attention (kv8_attention.cu, kv8_prompt.cu) share.  Kernel
+// parameters, e4m3 conversions, and the schedule that cuts the attention's
+// work into equal shares.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/mogemma_b200.h"
+#include "common.cuh"
+
+namespace mg {
+mg_status report_error(mg_status st, const char *msg);
+
+namespace kv8 {
+
+constexpr int kBlock = MG_KV8_BLOCK;  // tokens per scale
+constexpr int kUnit = 64;             // tokens of one unit of the attention's schedule
+constexpr uint32_t kErrLens = 0x70000u, kErrPage = 0x80000u;  // err_dev codes: bad lengths, bad page id
+
+// The cache and the batch as the kernels see them.
+struct Cache {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    int64_t page_stride, head_stride, token_stride;
+    int num_pages, page_shift, heads;  // page_size = 1 << page_shift
+};
+struct Batch {
+    const int32_t *q_start, *ctx_len, *table;
+    int64_t table_stride;
+    uint32_t *err;
+    int batch, total_q, max_q, max_ctx;
+};
+
+// One sequence, with the device's lengths forced into the host's bounds: rows
+// [q0, q0 + nq) at positions pos0 .. pos0 + nq - 1, of which those in
+// [0, max_ctx) exist.
+struct Seq {
+    int q0, nq, pos0;
+};
+__device__ __forceinline__ Seq load_seq(const Batch &b, int i, bool report) {
+    const int a = b.q_start[i], e = b.q_start[i + 1], ctx = b.ctx_len[i];
+    Seq s;
+    s.q0 = min(max(a, 0), b.total_q);
+    s.nq = min(min(max(e, s.q0), b.total_q) - s.q0, b.max_q);
+    // a length that breaks the bounds hides the whole sequence: positions below 0
+    const bool bad = a < 0 || e < a || e > b.total_q || e - a > b.max_q || ctx < e - a || ctx > b.max_ctx;
+    if (bad && report) set_error(b.err, kErrLens);
+    s.pos0 = bad ? -s.nq : ctx - s.nq;
+    return s;
+}
+
+// ---- e4m3 <-> wider.  Codes convert to fp16 exactly (448 and 2^-9 are both in its range).
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t two) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
+    return r;
+}
+// Both halves of a word: codes 0, 1 and codes 2, 3.
+__device__ __forceinline__ void e4m3x4_to_h2x2(uint32_t four, uint32_t &a, uint32_t &b) {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(four));
+}
+// Four floats to codes (nearest even, beyond 448 to 448, NaN to NaN), a in the lowest byte.
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {  // PTX ex2.approx: one MUFU op, about 2 ulp
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- the attention's schedule
+// An item is (sequence, tile of ROWS query rows, kv head): the rows of a
+// sequence and kv head are its (token, q head of the group) pairs, token major.
+// Its cost is the number of 64-token units its rows see, at least one (rows
+// that see nothing still have an answer to write).  Items are laid out head by
+// head, sequence by sequence; CTA c of G takes the units [c W / G, (c+1) W / G)
+// of all W, so the shares differ by one unit at most, whatever the lengths
+// (with fewer units than CTAs, the first W CTAs take one each).
+// Every CTA finds its place by the same scan over the items.
+struct AttnShape {
+    int group, rows, tiles, window;  // q heads per kv head; rows per tile; tiles per sequence (of max_q tokens)
+};
+struct Item {
+    Seq seq;
+    int row0, nrows;     // rows of the tile
+    int lo, hi;          // positions its rows see lie in [lo, hi)
+    int unit0, units;    // units unit0 .. unit0 + units - 1 (64 tokens each)
+};
+__device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, int pair, bool report) {
+    Item it;
+    const int i = pair / a.tiles, t = pair - i * a.tiles;
+    it.seq = load_seq(b, i, report);
+    it.row0 = t * a.rows;
+    it.nrows = min(a.rows, it.seq.nq * a.group - it.row0);
+    it.units = 0;
+    if (it.nrows <= 0) return it;
+    const int first = it.seq.pos0 + it.row0 / a.group, last = it.seq.pos0 + (it.row0 + it.nrows - 1) / a.group;
+    it.lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
+    it.hi = max(last + 1, it.lo);
+    it.unit0 = it.lo / kUnit;
+    it.units = max(1, (it.hi + kUnit - 1) / kUnit - it.unit0);
+    return it;
+}
+
+// Where CTA `cta` of `ctas` starts: its unit range [w0, w1) of the whole, and
+// the item (head, pair) and the unit within it of w0.  All threads of the CTA
+// call it; THREADS a multiple of 32.
+struct Place {
+    int64_t total, per_head;  // units of all heads, of one
+    int64_t w0, w1;
+    int ctas;  // CTAs that have a share
+    int head, pair, skip;
+};
+template <int THREADS>
+__device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, int heads, int cta, int ctas) {
+    constexpr int kWarps = THREADS / 32;
+    __shared__ int64_t warp_sum_s[kWarps];
+    __shared__ int found_pair, found_skip;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int pairs = b.batch * a.tiles, chunk = (pairs + THREADS - 1) / THREADS;
+    const int p0 = min(pairs, tid * chunk), p1 = min(pairs, p0 + chunk);
+    int64_t mine = 0;
+    for (int p = p0; p < p1; ++p) mine += load_item(b, a, p, cta == 0).units;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t n = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += n;
+    }
+    if (lane == 31) warp_sum_s[warp] = upto;
+    if (tid == 0) found_pair = found_skip = 0;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) upto += warp_sum_s[w];
+        all += warp_sum_s[w];
+    }
+    Place pl;
+    pl.per_head = all;
+    pl.total = all * heads;
+    pl.ctas = static_cast<int>(min(pl.total, static_cast<int64_t>(ctas)));
+    pl.w0 = cta < pl.ctas ? pl.total * cta / pl.ctas : 0;
+    pl.w1 = cta < pl.ctas ? pl.total * (cta + 1) / pl.ctas : 0;
+    pl.head = all > 0 ? static_cast<int>(pl.w0 / all) : 0;
+    const int64_t in_head = pl.w0 - pl.head * all;
+    if (mine > 0 && upto - mine <= in_head && in_head < upto) {
+        int64_t left = in_head - (upto - mine);
+        int p = p0;
+        for (; p < p1 - 1; ++p) {
+            const int u = load_item(b, a, p, false).units;
+            if (left < u) break;
+            left -= u;
+        }
+        found_pair = p;
+        found_skip = static_cast<int>(left);
+    }
+    __syncthreads();
+    pl.pair = found_pair;
+    pl.skip = found_skip;
+    return pl;
+}
+// The CTA that holds unit w.
+__device__ __forceinline__ int owner_of(const Place &pl, int64_t w) {
+    return static_cast<int>(((w + 1) * pl.ctas - 1) / pl.total);
+}
+
+// A CTA's items that reach beyond it are partial: at most its first (slot 2 c)
+// and its last (slot 2 c + 1).  The CTA in which an item starts that others
+// continue names it in split[c], for the combine.
+struct Split {
+    int pair, head, nrows;     // nrows 0: no such item
+    int first_slot, last_cta;  // slot of its first part; the others are first parts of the CTAs up to last_cta
+    int pad[3];
+};
+struct Partials {
+    Split *split;  // [ctas]
+    float *ml;     // [2 ctas][rows][2]: running maximum (log2 units) and sum
+    float *o;      // [2 ctas][rows][head dim], divided by the sum
+};
+inline size_t partials_bytes(int ctas, int rows, int hd) {
+    return static_cast<size_t>(ctas) * (sizeof(Split) + 2 * static_cast<size_t>(rows) * (hd + 2) * sizeof(float));
+}
+inline Partials partials_at(void *ws, int ctas, int rows) {
+    Partials p;
+    p.split = static_cast<Split *>(ws);
+    p.ml = reinterpret_cast<float *>(p.split + ctas);
+    p.o = p.ml + 4 * static_cast<size_t>(ctas) * rows;
+    return p;
+}
+
+struct AttnArgs {
+    Cache c;
+    Batch b;
+    AttnShape a;
+    Partials part;
+    const void *q;
+    void *out;
+    int64_t q_row, q_head, out_row, out_head;
+    float scale_log2;  // scale * log2(e)
+};
+
+
+
+
+}  // namespace kv8
+}  // namespace mg

@@ -1,0 +1,652 @@
+// kv8_attention.cu -- mg_kv8_attention: attention over the 8-bit paged cache
+// (the attention of layers.mojo:63-94), for few query rows per kv head; the
+// combine of partial answers; and the entry points.
+//
+// kv8_rows_kernel takes items of up to 8 query rows.  It is bound by reading
+// the cache: one code byte feeds 8 rows' products, so the legacy warp-level
+// MMA is fast enough and lets every byte go from global memory straight into
+// the registers it is multiplied from -- no shared-memory stage, no copy
+// engine, no layout to keep.  A warp takes 16 tokens (one scale block) at a
+// time and computes transposed products, tokens and head dims on the MMA's 16
+// rows, the query rows on its 8 columns:
+//   S^T[16 tokens][8 rows] = K . Q^T     A = K codes, widened to fp16 (exact)
+//   O^T[16 dims][8 rows]  += V^T . P^T   A = V codes of 4 tokens a lane,
+//                                        byte-interleaved, widened to fp16
+// The k index of an MMA may be any order of the head dims as long as A and B
+// agree, so a lane's K fragment is 16 consecutive bytes of a token's row, and
+// the m index any order of the output dims, so its V fragment is too.
+// S^T's accumulator layout transposes into P^T's operand layout by movmatrix.
+//
+// With s = scale log2(e) k_scale <q, k> the state per row is m = max s,
+// l = sum 2^(s - m) and the sum of P V with P = 2^(s + log2 v_scale - M),
+// M = max(s + log2 v_scale): the value scale rides in the exponent, so that P
+// is at most 1 whatever the scales, and fp16 holds it to 2^-12.
+#include <cstdio>
+
+#include "kv8.cuh"
+
+namespace mg {
+namespace kv8 {
+
+mg_status check_cache_batch(const char *who, const mg_kv8_cache *c, const mg_kv8_batch *b);
+Cache cache_of(const mg_kv8_cache *c);
+Batch batch_of(const mg_kv8_batch *b);
+
+namespace {
+constexpr int kRows = 8;       // query rows of an item
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr float kInf = __builtin_huge_valf();
+
+__device__ __forceinline__ uint4 ldg16(const uint8_t *p) {  // streamed: no reuse within an SM
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg8(const uint8_t *p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+// D += A . B, 16 x 8 x 16, fp16 operands, fp32 accumulators.
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 2 query values of type T as floats.
+template <typename T>
+__device__ __forceinline__ float2 two(uint32_t w);
+template <>
+__device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 two<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ void store_out4(__half *p, float a, float b, float c, float d) {
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_h2(a, b), pack_h2(c, d));
+}
+__device__ __forceinline__ void store_out4(__nv_bfloat16 *p, float a, float b, float c, float d) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
+    *reinterpret_cast<uint2 *>(p) =
+        make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+}
+__device__ __forceinline__ float max_over_rows(float v) {  // over the 8 lanes that share lane % 4
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+template <int HD>
+struct RowsCfg {
+    static constexpr int kTiles = 256 / HD;             // 16-token tiles of a warp's step: 4 KB of K, 4 KB of V
+    static constexpr int kVB = HD / 8 < 16 ? HD / 8 : 16;  // V bytes per load: 8 (hd 64) or 16
+    static constexpr int kVH = HD / (8 * kVB);          // loads along the head dims
+    static constexpr int kM = HD / 16;                  // MMAs along the output dims
+    static constexpr size_t kSmem = sizeof(float) * kWarps * kRows * (HD + 4);
+};
+
+// One tile's codes of a lane.  K: token lane / 4 and that + 8, bytes 64 c + 16 (lane % 4) .. + 15.
+template <int HD>
+struct KTile {
+    uint4 w[HD / 64][2];
+};
+// V: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (t = lane % 4), bytes kVB (8 h + lane / 4) .. of each.
+template <int HD>
+struct VTile {
+    uint32_t w[RowsCfg<HD>::kVH][4][RowsCfg<HD>::kVB / 4];
+};
+
+template <int HD>
+__device__ __forceinline__ void load_k(KTile<HD> &k, const uint8_t *tile, int64_t stride, int live, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const bool on = g + 8 * r < live;
+        const uint8_t *row = tile + (g + 8 * r) * stride + 16 * t;
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) k.w[c][r] = on ? ldg16(row + 64 * c) : make_uint4(0, 0, 0, 0);
+    }
+}
+template <int HD>
+__device__ __forceinline__ void load_v(VTile<HD> &v, const uint8_t *tile, int64_t stride, int live, int lane) {
+    using Cfg = RowsCfg<HD>;
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int tok = 2 * t + (r & 1) + 8 * (r >> 1);
+        const bool on = tok < live;
+        const uint8_t *row = tile + tok * stride + Cfg::kVB * g;
+#pragma unroll
+        for (int h = 0; h < Cfg::kVH; ++h) {
+            if constexpr (Cfg::kVB == 16) {
+                const uint4 w = on ? ldg16(row + 128 * h) : make_uint4(0, 0, 0, 0);
+                v.w[h][r][0] = w.x, v.w[h][r][1] = w.y, v.w[h][r][2] = w.z, v.w[h][r][3] = w.w;
+            } else {
+                const uint2 w = on ? ldg8(row + 64 * h) : make_uint2(0, 0);
+                v.w[h][r][0] = w.x, v.w[h][r][1] = w.y;
+            }
+        }
+    }
+}
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
+    using Cfg = RowsCfg<HD>;
+    extern __shared__ __align__(16) float sm[];  // merge: [warp][row][HD + 4]
+    __shared__ float mlm[kWarps][kRows][3];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int cta = blockIdx.x, ctas = gridDim.x;
+    const Place pl = find_place<kThreads>(p.b, p.a, p.c.heads, cta, ctas);
+    if (threadIdx.x == 0) p.part.split[cta].nrows = 0;
+    int64_t w = pl.w0;
+    int head = pl.head, pair = pl.pair, skip = pl.skip;
+    const int pairs = p.b.batch * p.a.tiles;
+    while (w < pl.w1) {
+        const Item it = load_item(p.b, p.a, pair, false);
+        if (it.units == 0 || it.nrows <= 0) {  // no rows in this tile
+            if (++pair == pairs) pair = 0, ++head;
+            continue;
+        }
+        const int take = static_cast<int>(min(static_cast<int64_t>(it.units - skip), pl.w1 - w));
+        const bool whole = take == it.units;
+        // this CTA's 16-token tiles of the item
+        const int ta = max((it.unit0 + skip) * (kUnit / 16), it.lo / 16);
+        const int tb = min((it.unit0 + skip + take) * (kUnit / 16), (it.hi + 15) / 16);
+        const int si = pair / p.a.tiles;
+        const int32_t *table = p.b.table + si * p.b.table_stride;
+
+        // ---- query rows: B fragments, row g, k order as the K fragments
+        uint32_t qf[HD / 64][4][2];
+        float factor[2];
+        int lo[2], hi[2];
+        {
+            const int r = it.row0 + g;
+            const bool on = g < it.nrows;
+            const int tok = on ? r / p.a.group : 0, h = head * p.a.group + (on ? r - tok * p.a.group : 0);
+            const T *src = static_cast<const T *>(p.q) + (static_cast<int64_t>(it.seq.q0) + tok) * p.q_row +
+                           h * p.q_head + 16 * t;
+            uint4 raw[HD / 64][2];
+            uint32_t most = 0;
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    raw[c][i] = on ? reinterpret_cast<const uint4 *>(src + 64 * c)[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = two<T>((&raw[c][0].x)[i]);
+                    most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+                }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            // a power of two that brings the row's maximum to [2^7, 2^8): fp16 then holds every bf16 value down
+            // to 2^-21 of it exactly.  A row with an infinity or NaN answers NaN.
+            const int e = static_cast<int>(most >> 23);
+            float up = 1.0f, down = 1.0f;
+            if (e >= 255) {
+                down = __int_as_float(0x7fc00000);
+            } else if (e > 0) {
+                const int sh = min(134 - e, 126);  // exponent of `up`; |sh| <= 126 keeps both normal
+                up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
+                down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
+            }
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = two<T>((&raw[c][0].x)[i]);
+                    qf[c][i >> 1][i & 1] = pack_h2(f.x * up, f.y * up);
+                }
+            // columns 2 t, 2 t + 1 of the accumulators are rows held by lanes 8 t, 8 t + 4
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                factor[i] = p.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t + 4 * i);
+                const int ri = 2 * t + i;
+                const int pos = it.seq.pos0 + (it.row0 + ri) / p.a.group;
+                hi[i] = ri < it.nrows ? pos + 1 : 0;
+                lo[i] = p.a.window > 0 ? pos - p.a.window + 1 : 0;
+            }
+        }
+
+        // ---- the warp's tiles, kTiles neighbours per step: its n-th is ta + ((n / kTiles) kWarps + warp) kTiles + n % kTiles
+        float o[Cfg::kM][4];
+#pragma unroll
+        for (int i = 0; i < Cfg::kM; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+        float m[2] = {-kInf, -kInf}, mv[2] = {-kInf, -kInf}, l[2] = {0.f, 0.f};
+        auto tile_at = [&](int n) { return ta + ((n / Cfg::kTiles) * kWarps + warp) * Cfg::kTiles + n % Cfg::kTiles; };
+        // lane i holds the place and scales of tile number base + i; place -1: none
+        int64_t place = -1;
+        float ks = 0.f, lvs = 0.f;
+        auto look_up = [&](int base) {
+            const int tile = tile_at(base + lane);
+            place = -1;
+            ks = 0.f;
+            lvs = 0.f;
+            if (tile < tb) {
+                const int tok = tile * 16, slot = tok & ((1 << p.c.page_shift) - 1);
+                const int page = table[tok >> p.c.page_shift];
+                if (page >= 0 && page < p.c.num_pages) {
+                    const int64_t sc = ((static_cast<int64_t>(page) * p.c.heads + head) << (p.c.page_shift - 4)) +
+                                       (slot >> 4);
+                    place = page * p.c.page_stride + head * p.c.head_stride + slot * p.c.token_stride;
+                    ks = p.c.k_scale[sc];
+                    lvs = __log2f(p.c.v_scale[sc]);
+                } else {
+                    set_error(p.b.err, kErrPage);
+                }
+            }
+        };
+        KTile<HD> kt[Cfg::kTiles];
+        VTile<HD> vt[Cfg::kTiles];
+        int64_t kp[Cfg::kTiles], vp[Cfg::kTiles];
+        float kss[Cfg::kTiles], lvss[Cfg::kTiles];
+        const int steps = (tb - ta + kWarps * Cfg::kTiles - 1) / (kWarps * Cfg::kTiles);
+        auto live_of = [&](int n, int64_t at) { return at < 0 ? 0 : it.hi - tile_at(n) * 16; };
+        auto fetch_k = [&](int n0) {
+#pragma unroll
+            for (int i = 0; i < Cfg::kTiles; ++i) {
+                kp[i] = __shfl_sync(0xffffffffu, place, (n0 + i) & 31);
+                kss[i] = __shfl_sync(0xffffffffu, ks, (n0 + i) & 31);
+                lvss[i] = __shfl_sync(0xffffffffu, lvs, (n0 + i) & 31);
+                load_k<HD>(kt[i], p.c.k + kp[i], p.c.token_stride, live_of(n0 + i, kp[i]), lane);
+            }
+        };
+        auto fetch_v = [&](int n0) {
+#pragma unroll
+            for (int i = 0; i < Cfg::kTiles; ++i)
+                load_v<HD>(vt[i], p.c.v + vp[i], p.c.token_stride, live_of(n0 + i, vp[i]), lane);
+        };
+        if (steps > 0) {
+            look_up(0);
+            fetch_k(0);
+#pragma unroll
+            for (int i = 0; i < Cfg::kTiles; ++i) vp[i] = kp[i];
+            fetch_v(0);
+        }
+        for (int step = 0; step < steps; ++step) {
+            const int n0 = step * Cfg::kTiles;
+            // S^T
+            float s[Cfg::kTiles][4];
+#pragma unroll
+            for (int i = 0; i < Cfg::kTiles; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t a0, a1, a2, a3;
+                        e4m3x4_to_h2x2((&kt[i].w[c][0].x)[j], a0, a2);
+                        e4m3x4_to_h2x2((&kt[i].w[c][1].x)[j], a1, a3);
+                        mma16816(s[i], a0, a1, a2, a3, qf[c][j][0], qf[c][j][1]);
+                    }
+            }
+            // masked, scaled scores; the next step's K loads go out once these registers are free
+            float sk[Cfg::kTiles], lv[Cfg::kTiles];
+            bool seen[Cfg::kTiles];
+#pragma unroll
+            for (int i = 0; i < Cfg::kTiles; ++i) sk[i] = kss[i], lv[i] = lvss[i], seen[i] = kp[i] >= 0;
+            const bool more = step + 1 < steps;
+            if (more) {
+                if (((n0 + Cfg::kTiles) & 31) == 0) look_up(n0 + Cfg::kTiles);
+                fetch_k(n0 + Cfg::kTiles);
+            }
+            float top[2] = {-kInf, -kInf}, topv[2] = {-kInf, -kInf};
+#pragma unroll
+            for (int i = 0; i < Cfg::kTiles; ++i) {
+                const int tok = tile_at(n0 + i) * 16 + g;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int c = e & 1, at = tok + 8 * (e >> 1);
+                    s[i][e] = seen[i] && at >= lo[c] && at < hi[c] ? s[i][e] * (factor[c] * sk[i]) : -kInf;
+                    top[c] = fmaxf(top[c], s[i][e]);
+                    topv[c] = fmaxf(topv[c], s[i][e] + lv[i]);
+                }
+            }
+            float base[2], basev[2];
+            bool moved = false;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float mn = fmaxf(m[c], max_over_rows(top[c])), vn = fmaxf(mv[c], max_over_rows(topv[c]));
+                base[c] = mn == -kInf ? 0.f : mn;
+                basev[c] = vn == -kInf ? 0.f : vn;
+                l[c] *= ex2(m[c] - base[c]);
+                moved |= vn != mv[c];
+                top[c] = ex2(mv[c] - basev[c]);  // O's factor
+                m[c] = mn;
+                mv[c] = vn;
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int i = 0; i < Cfg::kM; ++i) {
+                    o[i][0] *= top[0], o[i][2] *= top[0];
+                    o[i][1] *= top[1], o[i][3] *= top[1];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < Cfg::kTiles; ++i) {
+                float pr[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    l[e & 1] += ex2(s[i][e] - base[e & 1]);
+                    pr[e] = ex2(s[i][e] + lv[i] - basev[e & 1]);
+                }
+                const uint32_t b0 = transpose8x8(pack_h2(pr[0], pr[1])), b1 = transpose8x8(pack_h2(pr[2], pr[3]));
+#pragma unroll
+                for (int h = 0; h < Cfg::kVH; ++h)
+#pragma unroll
+                    for (int j = 0; j < Cfg::kVB / 4; ++j) {
+                        // tokens 2 t and 2 t + 1 (then + 8) of dims 4 j .. 4 j + 3, interleaved
+                        const uint32_t x0 = vt[i].w[h][0][j], x1 = vt[i].w[h][1][j];
+                        const uint32_t y0 = vt[i].w[h][2][j], y1 = vt[i].w[h][3][j];
+                        uint32_t a[4], b[4];
+                        e4m3x4_to_h2x2(__byte_perm(x0, x1, 0x5140), a[0], a[1]);
+                        e4m3x4_to_h2x2(__byte_perm(x0, x1, 0x7362), a[2], a[3]);
+                        e4m3x4_to_h2x2(__byte_perm(y0, y1, 0x5140), b[0], b[1]);
+                        e4m3x4_to_h2x2(__byte_perm(y0, y1, 0x7362), b[2], b[3]);
+                        float(&d0)[4] = o[h * (Cfg::kVB / 2) + 2 * j];
+                        float(&d1)[4] = o[h * (Cfg::kVB / 2) + 2 * j + 1];
+                        mma16816(d0, a[0], a[1], b[0], b[1], b0, b1);
+                        mma16816(d1, a[2], a[3], b[2], b[3], b0, b1);
+                    }
+            }
+            if (more) {
+#pragma unroll
+                for (int i = 0; i < Cfg::kTiles; ++i) vp[i] = kp[i];
+                fetch_v(n0 + Cfg::kTiles);
+            }
+        }
+
+        // ---- merge the warps
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], x);
+            if (g == 0) {
+                mlm[warp][2 * t + c][0] = m[c];
+                mlm[warp][2 * t + c][1] = l[c];
+                mlm[warp][2 * t + c][2] = mv[c];
+            }
+        }
+        // o[..][e]: dim kVB (8 h + g) + 2 j + (e >> 1), row 2 t + (e & 1), for MMA h kVB / 2 + j
+#pragma unroll
+        for (int i = 0; i < Cfg::kM; ++i) {
+            const int h = i / (Cfg::kVB / 2), j = i % (Cfg::kVB / 2);
+            float *dst = sm + (warp * kRows + 2 * t) * (HD + 4) + Cfg::kVB * (8 * h + g) + 2 * j;
+            *reinterpret_cast<float2 *>(dst) = make_float2(o[i][0], o[i][2]);
+            *reinterpret_cast<float2 *>(dst + HD + 4) = make_float2(o[i][1], o[i][3]);
+        }
+        __syncthreads();
+        const int slot = 2 * cta + (w == pl.w0 ? 0 : 1);
+        for (int x = threadIdx.x; x < it.nrows * (HD / 4); x += kThreads) {
+            const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
+            float mm = -kInf, mmv = -kInf, ll = 0.f;
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) mm = fmaxf(mm, mlm[i][r][0]), mmv = fmaxf(mmv, mlm[i][r][2]);
+            const float b = mm == -kInf ? 0.f : mm, bv = mmv == -kInf ? 0.f : mmv;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) {
+                ll += mlm[i][r][1] * ex2(mlm[i][r][0] - b);
+                const float f = ex2(mlm[i][r][2] - bv);
+                const float4 v = *reinterpret_cast<const float4 *>(sm + (i * kRows + r) * (HD + 4) + d);
+                acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+            }
+            // O is in units of 2^M, l in units of 2^m; a row that saw nothing has l = 0
+            const float f = ll == 0.f ? 0.f : ex2(bv - b) / ll;
+            acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+            if (whole) {
+                const int row = it.row0 + r, tok = row / p.a.group, hq = head * p.a.group + row - tok * p.a.group;
+                T *dst = static_cast<T *>(p.out) + (static_cast<int64_t>(it.seq.q0) + tok) * p.out_row +
+                         hq * p.out_head + d;
+                store_out4(dst, acc.x, acc.y, acc.z, acc.w);
+            } else {
+                const int64_t at = static_cast<int64_t>(slot) * kRows + r;
+                *reinterpret_cast<float4 *>(p.part.o + at * HD + d) = acc;
+                if (d == 0) *reinterpret_cast<float2 *>(p.part.ml + 2 * at) = make_float2(mm, ll);
+            }
+        }
+        if (threadIdx.x == 0 && skip == 0 && !whole)
+            p.part.split[cta] = Split{pair, head, it.nrows, slot, owner_of(pl, w + it.units - 1), {0, 0, 0}};
+        __syncthreads();
+        w += take;
+        skip = 0;
+        if (++pair == pairs) pair = 0, ++head;
+    }
+}
+
+// Joins the partial answers of the items that several CTAs share: their
+// weights are l 2^(m - max m).  Tasks (item, row, 64 dims) are dealt over a
+// fixed grid; 16 lanes hold 64 dims of a row and the CTA's 16 such groups take
+// every 16th partial, so that the loads of all partials are in flight at once.
+// The sums run in the order of the CTAs: the same answer every time.
+constexpr int kCombThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArgs p, int hd, int ctas) {
+    extern __shared__ int items[];  // the CTAs whose split entry is in use, rising
+    __shared__ int warp_n[kCombThreads / 32];
+    __shared__ float4 acc_s[16][16];
+    __shared__ float2 ml_s[16];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid >> 4, gl = tid & 15;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int found = 0;
+    for (int i0 = 0; i0 < ctas; i0 += kCombThreads) {
+        const int i = i0 + tid;
+        const bool used = i < ctas && p.part.split[i].nrows > 0;
+        const uint32_t votes = __ballot_sync(0xffffffffu, used);
+        if (lane == 0) warp_n[warp] = __popc(votes);
+        __syncthreads();
+        int at = found + __popc(votes & ((1u << lane) - 1u));
+#pragma unroll
+        for (int w = 0; w < kCombThreads / 32; ++w) {
+            if (w < warp) at += warp_n[w];
+            found += warp_n[w];
+        }
+        if (used) items[at] = i;
+        __syncthreads();
+    }
+    const int chunks = hd / 64, per_item = p.a.rows * chunks;
+    for (int64_t task = blockIdx.x; task < static_cast<int64_t>(found) * per_item; task += gridDim.x) {
+        const int first = items[task / per_item], sub = static_cast<int>(task % per_item);
+        const Split sp = p.part.split[first];
+        const int r = sub / chunks, d = 64 * (sub % chunks) + 4 * gl;
+        if (r >= sp.nrows) continue;  // the whole CTA
+        const int n = sp.last_cta - first + 1;
+        float m = -kInf, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = grp; i < n; i += 16) {
+            const int64_t at = static_cast<int64_t>(i == 0 ? sp.first_slot : 2 * (first + i)) * p.a.rows + r;
+            const float2 ml = *reinterpret_cast<const float2 *>(p.part.ml + 2 * at);
+            const float4 v = *reinterpret_cast<const float4 *>(p.part.o + at * hd + d);
+            const float mn = fmaxf(m, ml.x), b = mn == -kInf ? 0.f : mn;
+            const float fa = ex2(m - b), fb = ml.y * ex2(ml.x - b);
+            acc.x = acc.x * fa + v.x * fb, acc.y = acc.y * fa + v.y * fb;
+            acc.z = acc.z * fa + v.z * fb, acc.w = acc.w * fa + v.w * fb;
+            l = l * fa + fb;
+            m = mn;
+        }
+        acc_s[grp][gl] = acc;
+        if (gl == 0) ml_s[grp] = make_float2(m, l);
+        __syncthreads();
+        if (grp == 0) {
+            float top = -kInf, sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, ml_s[i].x);
+            const float b = top == -kInf ? 0.f : top;
+            float out[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float f = ex2(ml_s[i].x - b);
+                const float4 v = acc_s[i][gl];
+                out[0] += v.x * f, out[1] += v.y * f, out[2] += v.z * f, out[3] += v.w * f;
+                sum += ml_s[i].y * f;
+            }
+            const float f = sum == 0.f ? 0.f : 1.0f / sum;
+            const int si = sp.pair / p.a.tiles, row = (sp.pair - si * p.a.tiles) * p.a.rows + r;
+            const int tok = row / p.a.group, hq = sp.head * p.a.group + row - tok * p.a.group;
+            T *dst = static_cast<T *>(p.out) + (static_cast<int64_t>(load_seq(p.b, si, false).q0) + tok) * p.out_row +
+                     hq * p.out_head + d;
+            store_out4(dst, out[0] * f, out[1] * f, out[2] * f, out[3] * f);
+        }
+        __syncthreads();
+    }
+}
+
+// CTAs per SM of the rows kernel: registers allow two of 128 threads.
+constexpr int kRowsPerSm = 2;
+
+cudaError_t sm_count(int *sms) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    return e != cudaSuccess ? e : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+}
+
+template <int HD, typename T>
+cudaError_t launch_rows(const AttnArgs &p, int ctas, cudaStream_t s) {
+    const size_t smem = RowsCfg<HD>::kSmem;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kv8_rows_kernel<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
+    kv8_rows_kernel<HD, T><<<ctas, kThreads, smem, s>>>(p);
+    return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kCombThreads);
+    cfg.dynamicSmemBytes = sizeof(int) * static_cast<size_t>(ctas);
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv8_combine_kernel<T>, p, hd, ctas);
+}
+template <typename T>
+cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, cudaStream_t s) {
+    const cudaError_t e = hd == 64    ? launch_rows<64, T>(p, ctas, s)
+                          : hd == 128 ? launch_rows<128, T>(p, ctas, s)
+                                      : launch_rows<256, T>(p, ctas, s);
+    return e != cudaSuccess ? e : launch_combine<T>(p, hd, ctas, s);
+}
+
+struct Plan {
+    int rows, tiles, ctas;
+    size_t bytes;
+};
+// How a call runs: set by the cache's dimensions and the batch's bounds alone, so that the workspace's size is too.
+cudaError_t plan_of(int hd, int group, int max_q, Plan *pl) {
+    int sms = 0;
+    const cudaError_t e = sm_count(&sms);
+    if (e != cudaSuccess) return e;
+    pl->rows = kRows;
+    pl->ctas = sms * kRowsPerSm;
+    pl->tiles = static_cast<int>((static_cast<int64_t>(max_q) * group + pl->rows - 1) / pl->rows);
+    pl->bytes = partials_bytes(pl->ctas, pl->rows, hd);
+    return cudaSuccess;
+}
+mg_status cuda_error(const char *who, cudaError_t e) {
+    char buf[160];
+    snprintf(buf, sizeof buf, "%s: %s", who, cudaGetErrorString(e));
+    return report_error(MG_ERR_CUDA, buf);
+}
+mg_status check_heads(const char *who, const mg_kv8_cache *c, const mg_kv8_batch *b, int num_heads) {
+    char buf[200];
+    if (num_heads <= 0 || num_heads % c->num_kv_heads != 0) {
+        snprintf(buf, sizeof buf, "%s: num_heads must be a positive multiple of num_kv_heads", who);
+        return report_error(MG_ERR_INVALID, buf);
+    }
+    if (num_heads / c->num_kv_heads > 128 ||
+        static_cast<int64_t>(b->batch) * b->max_q * (num_heads / c->num_kv_heads) > (1ll << 30)) {
+        snprintf(buf, sizeof buf, "%s: more than 128 heads per kv head, or batch * max_q too large", who);
+        return report_error(MG_ERR_UNSUPPORTED, buf);
+    }
+    return MG_OK;
+}
+}  // namespace
+}  // namespace kv8
+}  // namespace mg
+
+using namespace mg;
+
+extern "C" mg_status mg_kv8_attention_workspace(const mg_kv8_cache *cache, const mg_kv8_batch *batch,
+                                                int32_t num_heads, int64_t *bytes_out) {
+    using namespace kv8;
+    const char *who = "mg_kv8_attention_workspace";
+    mg_status st = check_cache_batch(who, cache, batch);
+    if (st == MG_OK) st = check_heads(who, cache, batch, num_heads);
+    if (st != MG_OK) return st;
+    if (!bytes_out) return report_error(MG_ERR_INVALID, "mg_kv8_attention_workspace: null output");
+    Plan pl;
+    const cudaError_t e = plan_of(cache->head_dim, num_heads / cache->num_kv_heads, batch->max_q, &pl);
+    if (e != cudaSuccess) return cuda_error(who, e);
+    *bytes_out = static_cast<int64_t>(pl.bytes);
+    return MG_OK;
+}
+
+extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_batch *batch,
+                                      const mg_kv8_attention_args *args, void *stream) {
+    using namespace kv8;
+    const char *who = "mg_kv8_attention";
+    mg_status st = check_cache_batch(who, cache, batch);
+    if (st != MG_OK) return st;
+    if (!args || args->struct_size != static_cast<int32_t>(sizeof *args))
+        return report_error(MG_ERR_INVALID, "mg_kv8_attention: null argument or struct_size mismatch");
+    st = check_heads(who, cache, batch, args->num_heads);
+    if (st != MG_OK) return st;
+    if (args->dtype != MG_BF16 && args->dtype != MG_F16)
+        return report_error(MG_ERR_UNSUPPORTED, "mg_kv8_attention: dtype must be MG_BF16 or MG_F16");
+    if (args->window < 0 || !(args->scale >= -3.0e38f && args->scale <= 3.0e38f))
+        return report_error(MG_ERR_INVALID, "mg_kv8_attention: need window >= 0 and a finite scale");
+    if (!args->q_dev || !args->out_dev) return report_error(MG_ERR_INVALID, "mg_kv8_attention: null q or out");
+    if (((reinterpret_cast<uintptr_t>(args->q_dev) | reinterpret_cast<uintptr_t>(args->out_dev)) % 16) != 0 ||
+        ((args->q_row_stride | args->q_head_stride | args->out_row_stride | args->out_head_stride) % 8) != 0)
+        return report_error(MG_ERR_INVALID,
+                            "mg_kv8_attention: q and out must be 16-byte aligned with strides in multiples of 8");
+    const int group = args->num_heads / cache->num_kv_heads;
+    Plan pl;
+    cudaError_t e = plan_of(cache->head_dim, group, batch->max_q, &pl);
+    if (e != cudaSuccess) return cuda_error(who, e);
+    if (!args->workspace_dev || reinterpret_cast<uintptr_t>(args->workspace_dev) % 16 != 0 ||
+        args->workspace_bytes < static_cast<int64_t>(pl.bytes))
+        return report_error(MG_ERR_INVALID, "mg_kv8_attention: workspace missing, unaligned or too small "
+                                            "(mg_kv8_attention_workspace)");
+    AttnArgs p;
+    p.c = cache_of(cache);
+    p.b = batch_of(batch);
+    p.a = AttnShape{group, pl.rows, pl.tiles, args->window};
+    p.part = partials_at(args->workspace_dev, pl.ctas, pl.rows);
+    p.q = args->q_dev, p.out = args->out_dev;
+    p.q_row = args->q_row_stride, p.q_head = args->q_head_stride;
+    p.out_row = args->out_row_stride, p.out_head = args->out_head_stride;
+    p.scale_log2 = args->scale * 1.4426950408889634f;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    e = args->dtype == MG_BF16 ? launch_attention<__nv_bfloat16>(p, cache->head_dim, pl.ctas, s)
+                               : launch_attention<__half>(p, cache->head_dim, pl.ctas, s);
+    return e == cudaSuccess ? MG_OK : cuda_error(who, e);
+}

@@ -1,0 +1,248 @@
+"""The 8-bit paged key/value cache on torch tensors: ``mg_kv8_append`` and ``mg_kv8_attention``.
+
+``KV8Cache`` holds one layer's pages, ``KV8Batch`` the sequences of a step.
+``append`` stores a step's new keys and values (head norm and rotation on the
+way) and rotates its queries; ``attention`` answers them.  The definitions,
+bounds and error rules are those of ``include/mogemma_b200.h``.
+
+    cache = KV8Cache(num_pages=512, page_size=64, kv_heads=4, head_dim=256)
+    batch = KV8Batch(q_start, ctx_len, page_table, max_q=1, max_ctx=8192)
+    cache.append(batch, k, v, q=q, q_out=q, cos=cos, sin=sin, q_norm=wq, k_norm=wk)
+    cache.attention(batch, q, out, scale=256 ** -0.5)
+
+``append_call`` / ``attention_call`` check and bind the same arguments once; the
+object they return launches the call each time it is called (on torch's current
+stream of the cache's device), so a decode loop that keeps its buffers pays for
+the checks once.  A bound call reads the tensors' contents anew every time: new
+rows, lengths and tables are written into the same tensors.  It may be captured
+into a CUDA graph.  An attention call has a workspace of its own unless one is
+given; calls that may run at the same time must not share one.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from collections.abc import Callable
+from typing import Any
+
+import torch
+
+from . import _core
+
+BLOCK = 16  # tokens per scale (MG_KV8_BLOCK)
+_TYPES = {torch.float32: _core.MG_F32, torch.bfloat16: _core.MG_BF16, torch.float16: _core.MG_F16}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _rows(name: str, x: torch.Tensor, device: torch.device, dim: int) -> torch.Tensor:
+    _need(isinstance(x, torch.Tensor) and x.dim() == 3 and x.shape[2] == dim and x.stride(2) == 1,
+          f"{name} must be a [rows, heads, {dim}] tensor, contiguous along its last dimension")
+    _need(x.device == device, f"{name} is on {x.device}, the cache on {device}")
+    _need(x.dtype in _TYPES, f"{name} must be float32, bfloat16 or float16")
+    return x
+
+
+def _strides(x: torch.Tensor) -> tuple[int, int]:
+    """Row and head strides; a dimension of size 1 may report any, and uses none."""
+    return (x.stride(0) if x.shape[0] > 1 else 0), (x.stride(1) if x.shape[1] > 1 else 0)
+
+
+def _written(name: str, x: torch.Tensor) -> None:
+    # one stride spans a vector and the other all of the smaller dimension: rows and heads do not overlap
+    (r, h), (nr, nh, d) = _strides(x), x.shape
+    apart = (nr == 1 or r >= d) and (nh == 1 or h >= d)
+    apart = apart and (nr == 1 or nh == 1 or r >= h * nh or h >= r * nr)
+    _need(apart, f"{name} is written: its rows and heads must not overlap")
+
+
+def _vector(name: str, x: torch.Tensor | None, device: torch.device, shape: tuple[int, ...]) -> int | None:
+    if x is None:
+        return None
+    _need(x.dtype == torch.float32 and x.device == device and x.is_contiguous() and tuple(x.shape) == shape,
+          f"{name} must be a contiguous float32 tensor of shape {shape} on {device}")
+    return x.data_ptr()
+
+
+class KV8Call:
+    """A checked call with its tensors; launches on torch's current stream each time it is called."""
+
+    def __init__(self, fn: Callable[..., int], device: torch.device, structs: tuple[Any, ...], keep: tuple[Any, ...]) -> None:
+        self._fn = fn
+        self._device = device
+        self._structs = structs
+        self._refs = tuple(ctypes.byref(s) for s in structs)
+        self._keep = keep
+
+    def __call__(self) -> None:
+        dev = self._device.index
+        if torch.cuda.current_device() != dev:
+            with torch.cuda.device(dev):
+                status = self._fn(*self._refs, torch.cuda.current_stream().cuda_stream)
+        else:
+            status = self._fn(*self._refs, torch.cuda.current_stream().cuda_stream)
+        if status:
+            _core._check(status)  # noqa: SLF001
+
+
+class KV8Batch:
+    """The sequences of a step: packed new tokens, contexts and page lists (``mg_kv8_batch``).
+
+    ``q_start`` [batch + 1], ``ctx_len`` [batch] and ``page_table`` [batch, pages] are int32 tensors on
+    the cache's device; ``max_q`` and ``max_ctx`` bound the lengths they will ever hold."""
+
+    def __init__(self, q_start: torch.Tensor, ctx_len: torch.Tensor, page_table: torch.Tensor, *, max_q: int,
+                 max_ctx: int) -> None:
+        for name, x, dims in (("q_start", q_start, 1), ("ctx_len", ctx_len, 1), ("page_table", page_table, 2)):
+            _need(isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.dim() == dims and x.is_cuda,
+                  f"{name} must be a {dims}-dimensional int32 tensor on a CUDA device")
+            _need(x.device == q_start.device, "q_start, ctx_len and page_table must be on one device")
+            _need(x.numel() > 0 and x.stride(-1) == 1, f"{name} must be contiguous and not empty")
+        n = ctx_len.shape[0]
+        _need(q_start.shape[0] == n + 1 and page_table.shape[0] == n,
+              "q_start has batch + 1 entries, page_table one row per sequence")
+        self.q_start, self.ctx_len, self.page_table = q_start, ctx_len, page_table
+        self.max_q, self.max_ctx = int(max_q), int(max_ctx)
+        self.device = q_start.device
+        self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+
+    def check(self) -> None:
+        """Raises if a call since the last check met lengths or page ids out of bounds (synchronises)."""
+        code = int(self.err.item())
+        if code:
+            self.err.zero_()
+            msg = "page id out of range" if code == 0x80000 else f"lengths out of bounds (0x{code:x})"
+            raise RuntimeError(f"8-bit cache: {msg}")
+
+    def _desc(self, total_q: int) -> _core.KV8BatchDesc:
+        # a single row may report any stride
+        width = self.page_table.shape[1] if self.ctx_len.shape[0] == 1 else self.page_table.stride(0)
+        return _core.KV8BatchDesc(
+            ctypes.sizeof(_core.KV8BatchDesc), self.ctx_len.shape[0], total_q, self.max_q,
+            min(self.max_ctx, 2**31 - 1), 0, self.q_start.data_ptr(), self.ctx_len.data_ptr(),
+            self.page_table.data_ptr(), width, self.err.data_ptr())
+
+
+class KV8Cache:
+    """One layer's pages of e4m3 codes ``[pages, kv heads, page size, head dim]`` and their scales
+    ``[pages, kv heads, page size / 16]``."""
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
+                 device: torch.device | str = "cuda") -> None:
+        _need(num_pages > 0 and page_size >= BLOCK and page_size % BLOCK == 0 and kv_heads > 0 and head_dim > 0,
+              "need num_pages, kv_heads, head_dim > 0 and page_size a multiple of 16")
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        scales = (num_pages, kv_heads, page_size // BLOCK)
+        self._bind(*(torch.zeros(shape, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)),
+                   *(torch.ones(scales, dtype=torch.float32, device=device) for _ in range(2)))
+
+    @classmethod
+    def wrap(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> KV8Cache:
+        """A cache over existing tensors (float8_e4m3fn or uint8 codes; k and v with equal strides)."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_scale, v_scale)
+        return self
+
+    def _bind(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+        for x in (k, v):
+            _need(isinstance(x, torch.Tensor) and x.dim() == 4 and x.is_cuda
+                  and x.dtype in (torch.float8_e4m3fn, torch.uint8) and x.stride(3) == 1,
+                  "codes must be 4-dimensional float8_e4m3fn or uint8 CUDA tensors, contiguous along the head dim")
+        _need(k.shape == v.shape and k.stride() == v.stride() and k.device == v.device,
+              "k and v must have the same shape, strides and device")
+        pages, heads, size, dim = k.shape
+        _need(k.numel() > 0 and size % BLOCK == 0, "the cache must not be empty; page_size a multiple of 16")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
+        self.device = k.device
+        shape = (pages, heads, size // BLOCK)
+        ks, vs = (_vector(n, x, self.device, shape) for n, x in (("k_scale", k_scale), ("v_scale", v_scale)))
+        # strides of dimensions of size 1 say nothing: give the dense ones
+        token = k.stride(2)
+        head = k.stride(1) if heads > 1 else max(token * size, dim)
+        page = k.stride(0) if pages > 1 else max(head * heads, dim)
+        self._c = _core.KV8CacheDesc(ctypes.sizeof(_core.KV8CacheDesc), pages, size, heads, dim, 0, k.data_ptr(),
+                                     v.data_ptr(), ks, vs, page, head, token)
+
+    def _batch(self, batch: KV8Batch, total_q: int) -> _core.KV8BatchDesc:
+        _need(batch.device == self.device, f"the batch is on {batch.device}, the cache on {self.device}")
+        return batch._desc(total_q)  # noqa: SLF001
+
+    # ------------------------------------------------------------------ append
+    def append_call(self, batch: KV8Batch, k: torch.Tensor, v: torch.Tensor, *, q: torch.Tensor | None = None,
+                    q_out: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                    k_norm: torch.Tensor | None = None, cos: torch.Tensor | None = None,
+                    sin: torch.Tensor | None = None) -> KV8Call:
+        """Binds ``mg_kv8_append``: k, v [rows, kv heads, head dim] and, with its rotated copy q_out (or q itself),
+        q [rows, heads, head dim]; norm weights [head dim]; cos / sin [positions, head dim / 2]."""
+        d = self.head_dim
+        for name, x in (("k", k), ("v", v)):
+            _rows(name, x, self.device, d)
+            _need(x.shape[1] == self.kv_heads and x.dtype == k.dtype and x.shape[0] == k.shape[0],
+                  f"{name} must have {self.kv_heads} heads, and k and v the same rows and type")
+        _need((q is None) == (q_out is None), "q and q_out come together")
+        heads, out_dtype = 0, k.dtype
+        if q is not None:
+            _rows("q", q, self.device, d)
+            _rows("q_out", q_out, self.device, d)
+            _need(q.dtype == k.dtype and q.shape == q_out.shape and q.shape[0] == k.shape[0],
+                  "q must have the rows and type of k, and q_out the shape of q")
+            _written("q_out", q_out)
+            heads, out_dtype = q.shape[1], q_out.dtype
+        length = 0
+        if cos is not None:
+            _need(cos.dim() == 2, "cos and sin must be [positions, head dim / 2]")
+            length = cos.shape[0]
+        args = _core.KV8AppendArgs(
+            ctypes.sizeof(_core.KV8AppendArgs), _TYPES[k.dtype], _TYPES[out_dtype], heads, length, 0,
+            q.data_ptr() if heads else None, k.data_ptr(), v.data_ptr(), q_out.data_ptr() if heads else None,
+            *(_strides(q) if heads else (0, 0)), *_strides(k), *_strides(v),
+            *(_strides(q_out) if heads else (0, 0)),
+            _vector("q_norm", q_norm, self.device, (d,)), _vector("k_norm", k_norm, self.device, (d,)),
+            _vector("cos", cos, self.device, (length, d // 2)), _vector("sin", sin, self.device, (length, d // 2)))
+        return KV8Call(_core.lib().mg_kv8_append, self.device, (self._c, self._batch(batch, k.shape[0]), args),
+                       (self, batch, q, k, v, q_out, q_norm, k_norm, cos, sin))
+
+    def append(self, batch: KV8Batch, k: torch.Tensor, v: torch.Tensor, **more: Any) -> None:
+        """``append_call`` with the same arguments, launched once."""
+        self.append_call(batch, k, v, **more)()
+
+    # --------------------------------------------------------------- attention
+    def workspace_bytes(self, batch: KV8Batch, heads: int) -> int:
+        """Bytes of workspace that an attention call with these bounds needs."""
+        n = ctypes.c_int64()
+        with torch.cuda.device(self.device):
+            _core._check(_core.lib().mg_kv8_attention_workspace(  # noqa: SLF001
+                ctypes.byref(self._c), ctypes.byref(self._batch(batch, 1)), heads, ctypes.byref(n)))
+        return n.value
+
+    def attention_call(self, batch: KV8Batch, q: torch.Tensor, out: torch.Tensor, *, scale: float | None = None,
+                       window: int = 0, workspace: torch.Tensor | None = None) -> KV8Call:
+        """Binds ``mg_kv8_attention``: q and out [rows, heads, head dim]; scale defaults to head_dim ** -0.5; window 0:
+        every earlier position.  workspace: a uint8 tensor of at least ``workspace_bytes``."""
+        d = self.head_dim
+        _rows("q", q, self.device, d)
+        _rows("out", out, self.device, d)
+        _need(q.shape == out.shape and q.dtype == out.dtype, "out must have the shape and type of q")
+        _written("out", out)
+        size = self.workspace_bytes(batch, q.shape[1])
+        if workspace is None:
+            workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
+        _need(workspace.dtype == torch.uint8 and workspace.device == self.device and workspace.is_contiguous(),
+              f"workspace must be a contiguous uint8 tensor on {self.device}")
+        args = _core.KV8AttentionArgs(
+            ctypes.sizeof(_core.KV8AttentionArgs), _TYPES[q.dtype], q.shape[1], int(window),
+            d ** -0.5 if scale is None else float(scale), 0, q.data_ptr(), out.data_ptr(), *_strides(q),
+            *_strides(out), workspace.data_ptr(), workspace.numel())
+        return KV8Call(_core.lib().mg_kv8_attention, self.device, (self._c, self._batch(batch, q.shape[0]), args),
+                       (self, batch, q, out, workspace))
+
+    def attention(self, batch: KV8Batch, q: torch.Tensor, out: torch.Tensor | None = None, **more: Any) -> torch.Tensor:
+        """``attention_call`` with the same arguments, launched once; returns out (a new tensor if none is given)."""
+        if out is None:
+            out = torch.zeros_like(q, memory_format=torch.contiguous_format)
+        self.attention_call(batch, q, out, **more)()
+        return out
