@@ -22,6 +22,7 @@
 // M = max(s + log2 v_scale): the value scale rides in the exponent, so that P
 // is at most 1 whatever the scales, and fp16 holds it to 2^-12.
 #include <cstdio>
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -31,6 +32,10 @@ namespace kv8 {
 mg_status check_cache_batch(const char *who, const mg_kv8_cache *c, const mg_kv8_batch *b);
 Cache cache_of(const mg_kv8_cache *c);
 Batch batch_of(const mg_kv8_batch *b);
+// kv8_prompt.cu
+constexpr int kPromptRows = 128;
+int prompt_ctas_per_sm(int hd);
+cudaError_t launch_prompt(const AttnArgs &p, int hd, bool f16, int ctas, cudaStream_t s);
 
 namespace {
 constexpr int kRows = 8;       // query rows of an item
@@ -549,7 +554,9 @@ cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, cudaStream_t s) 
 }
 template <typename T>
 cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, cudaStream_t s) {
-    const cudaError_t e = hd == 64    ? launch_rows<64, T>(p, ctas, s)
+    const cudaError_t e = p.a.rows == kPromptRows
+                              ? launch_prompt(p, hd, std::is_same<T, __half>::value, ctas, s)
+                          : hd == 64  ? launch_rows<64, T>(p, ctas, s)
                           : hd == 128 ? launch_rows<128, T>(p, ctas, s)
                                       : launch_rows<256, T>(p, ctas, s);
     return e != cudaSuccess ? e : launch_combine<T>(p, hd, ctas, s);
@@ -564,8 +571,9 @@ cudaError_t plan_of(int hd, int group, int max_q, Plan *pl) {
     int sms = 0;
     const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
-    pl->rows = kRows;
-    pl->ctas = sms * kRowsPerSm;
+    const bool prompt = static_cast<int64_t>(max_q) * group > kRows;
+    pl->rows = prompt ? kPromptRows : kRows;
+    pl->ctas = sms * (prompt ? prompt_ctas_per_sm(hd) : kRowsPerSm);
     pl->tiles = static_cast<int>((static_cast<int64_t>(max_q) * group + pl->rows - 1) / pl->rows);
     pl->bytes = partials_bytes(pl->ctas, pl->rows, hd);
     return cudaSuccess;
