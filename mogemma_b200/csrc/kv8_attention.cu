@@ -33,8 +33,7 @@ mg_status check_cache_batch(const char *who, const mg_kv8_cache *c, const mg_kv8
 Cache cache_of(const mg_kv8_cache *c);
 Batch batch_of(const mg_kv8_batch *b);
 // kv8_prompt.cu
-constexpr int kPromptRows = 128;
-int prompt_ctas_per_sm(int hd);
+int prompt_rows(int hd);
 cudaError_t launch_prompt(const AttnArgs &p, int hd, bool f16, int ctas, cudaStream_t s);
 
 namespace {
@@ -441,80 +440,112 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
 }
 
 // Joins the partial answers of the items that several CTAs share: their
-// weights are l 2^(m - max m).  Tasks (item, row, 64 dims) are dealt over a
-// fixed grid; 16 lanes hold 64 dims of a row and the CTA's 16 such groups take
-// every 16th partial, so that the loads of all partials are in flight at once.
-// The sums run in the order of the CTAs: the same answer every time.
+// weights are l 2^(m - max m).  16 lanes hold 64 dims of a row; the CTA's 16
+// such groups take a row each where an item has few parts (prompts: 2 or 3),
+// or share one row's parts where it has many (one long context: hundreds), so
+// that the loads of all parts are in flight at once.  Tasks (item, rows, 64
+// dims) are dealt over a fixed grid; the sums run in the order of the CTAs, the
+// same every time.
 constexpr int kCombThreads = 256;
+constexpr int kFewParts = 8;
+constexpr int kCombPerSm = 4;
+
+struct Joined {  // a running join of parts
+    float m = -kInf, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void add(float pm, float pl, float4 v) {
+        const float mn = fmaxf(m, pm), b = mn == -kInf ? 0.f : mn;
+        const float fa = ex2(m - b), fb = pl * ex2(pm - b);
+        acc.x = acc.x * fa + v.x * fb, acc.y = acc.y * fa + v.y * fb;
+        acc.z = acc.z * fa + v.z * fb, acc.w = acc.w * fa + v.w * fb;
+        l = l * fa + fb;
+        m = mn;
+    }
+};
+
 template <typename T>
 __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArgs p, int hd, int ctas) {
-    extern __shared__ int items[];  // the CTAs whose split entry is in use, rising
+    extern __shared__ int sm_i[];  // [ctas] tasks of the entries before this one
     __shared__ int warp_n[kCombThreads / 32];
     __shared__ float4 acc_s[16][16];
     __shared__ float2 ml_s[16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid >> 4, gl = tid & 15;
+    const int chunks = hd / 64;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    int found = 0;
+    int tasks = 0;
     for (int i0 = 0; i0 < ctas; i0 += kCombThreads) {
         const int i = i0 + tid;
-        const bool used = i < ctas && p.part.split[i].nrows > 0;
-        const uint32_t votes = __ballot_sync(0xffffffffu, used);
-        if (lane == 0) warp_n[warp] = __popc(votes);
+        int mine = 0;
+        if (i < ctas) {
+            const Split sp = p.part.split[i];
+            if (sp.nrows > 0) mine = (sp.last_cta - i < kFewParts ? (sp.nrows + 15) / 16 : sp.nrows) * chunks;
+        }
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int n = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += n;
+        }
+        if (lane == 31) warp_n[warp] = upto;
         __syncthreads();
-        int at = found + __popc(votes & ((1u << lane) - 1u));
+        int before = tasks + upto - mine;
 #pragma unroll
         for (int w = 0; w < kCombThreads / 32; ++w) {
-            if (w < warp) at += warp_n[w];
-            found += warp_n[w];
+            if (w < warp) before += warp_n[w];
+            tasks += warp_n[w];
         }
-        if (used) items[at] = i;
+        if (i < ctas) sm_i[i] = before;
         __syncthreads();
     }
-    const int chunks = hd / 64, per_item = p.a.rows * chunks;
-    for (int64_t task = blockIdx.x; task < static_cast<int64_t>(found) * per_item; task += gridDim.x) {
-        const int first = items[task / per_item], sub = static_cast<int>(task % per_item);
-        const Split sp = p.part.split[first];
-        const int r = sub / chunks, d = 64 * (sub % chunks) + 4 * gl;
-        if (r >= sp.nrows) continue;  // the whole CTA
-        const int n = sp.last_cta - first + 1;
-        float m = -kInf, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int i = grp; i < n; i += 16) {
-            const int64_t at = static_cast<int64_t>(i == 0 ? sp.first_slot : 2 * (first + i)) * p.a.rows + r;
-            const float2 ml = *reinterpret_cast<const float2 *>(p.part.ml + 2 * at);
-            const float4 v = *reinterpret_cast<const float4 *>(p.part.o + at * hd + d);
-            const float mn = fmaxf(m, ml.x), b = mn == -kInf ? 0.f : mn;
-            const float fa = ex2(m - b), fb = ml.y * ex2(ml.x - b);
-            acc.x = acc.x * fa + v.x * fb, acc.y = acc.y * fa + v.y * fb;
-            acc.z = acc.z * fa + v.z * fb, acc.w = acc.w * fa + v.w * fb;
-            l = l * fa + fb;
-            m = mn;
+    for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+        int first = 0, end = ctas;  // the last entry with sm_i <= task: the one that has it, as empty ones follow it
+        while (end - first > 1) {
+            const int mid = (first + end) >> 1;
+            if (sm_i[mid] <= task) first = mid;
+            else end = mid;
         }
-        acc_s[grp][gl] = acc;
-        if (gl == 0) ml_s[grp] = make_float2(m, l);
-        __syncthreads();
-        if (grp == 0) {
-            float top = -kInf, sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, ml_s[i].x);
-            const float b = top == -kInf ? 0.f : top;
-            float out[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float f = ex2(ml_s[i].x - b);
-                const float4 v = acc_s[i][gl];
-                out[0] += v.x * f, out[1] += v.y * f, out[2] += v.z * f, out[3] += v.w * f;
-                sum += ml_s[i].y * f;
+        const Split sp = p.part.split[first];
+        const int sub = task - sm_i[first], n = sp.last_cta - first + 1;
+        const bool few = n <= kFewParts;
+        const int r = few ? 16 * (sub / chunks) + grp : sub / chunks, d = 64 * (sub % chunks) + 4 * gl;
+        Joined j;
+        if (r < sp.nrows) {
+            const int i0 = few ? 0 : grp, step = few ? 1 : 16;
+#pragma unroll 4
+            for (int i = i0; i < n; i += step) {
+                const int64_t at = static_cast<int64_t>(i == 0 ? sp.first_slot : 2 * (first + i)) * p.a.rows + r;
+                const float2 ml = *reinterpret_cast<const float2 *>(p.part.ml + 2 * at);
+                j.add(ml.x, ml.y, *reinterpret_cast<const float4 *>(p.part.o + at * hd + d));
             }
-            const float f = sum == 0.f ? 0.f : 1.0f / sum;
+        }
+        if (!few) {  // join the groups
+            acc_s[grp][gl] = j.acc;
+            if (gl == 0) ml_s[grp] = make_float2(j.m, j.l);
+            __syncthreads();
+            if (grp == 0) {
+                j = Joined();
+                float top = -kInf;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, ml_s[i].x);
+                const float b = top == -kInf ? 0.f : top;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float f = ex2(ml_s[i].x - b);
+                    const float4 v = acc_s[i][gl];
+                    j.acc.x += v.x * f, j.acc.y += v.y * f, j.acc.z += v.z * f, j.acc.w += v.w * f;
+                    j.l += ml_s[i].y * f;
+                }
+            }
+            __syncthreads();
+        }
+        if (r < sp.nrows && (few || grp == 0)) {
+            const float f = j.l == 0.f ? 0.f : 1.0f / j.l;
             const int si = sp.pair / p.a.tiles, row = (sp.pair - si * p.a.tiles) * p.a.rows + r;
             const int tok = row / p.a.group, hq = sp.head * p.a.group + row - tok * p.a.group;
             T *dst = static_cast<T *>(p.out) + (static_cast<int64_t>(load_seq(p.b, si, false).q0) + tok) * p.out_row +
                      hq * p.out_head + d;
-            store_out4(dst, out[0] * f, out[1] * f, out[2] * f, out[3] * f);
+            store_out4(dst, j.acc.x * f, j.acc.y * f, j.acc.z * f, j.acc.w * f);
         }
-        __syncthreads();
     }
 }
 
@@ -539,9 +570,9 @@ cudaError_t launch_rows(const AttnArgs &p, int ctas, cudaStream_t s) {
     return cudaGetLastError();
 }
 template <typename T>
-cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, cudaStream_t s) {
+cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
+    cfg.gridDim = dim3(kCombPerSm * sms);
     cfg.blockDim = dim3(kCombThreads);
     cfg.dynamicSmemBytes = sizeof(int) * static_cast<size_t>(ctas);
     cfg.stream = s;
@@ -553,17 +584,17 @@ cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, cudaStream_t s) 
     return cudaLaunchKernelEx(&cfg, kv8_combine_kernel<T>, p, hd, ctas);
 }
 template <typename T>
-cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, cudaStream_t s) {
-    const cudaError_t e = p.a.rows == kPromptRows
+cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {
+    const cudaError_t e = p.a.rows != kRows
                               ? launch_prompt(p, hd, std::is_same<T, __half>::value, ctas, s)
                           : hd == 64  ? launch_rows<64, T>(p, ctas, s)
                           : hd == 128 ? launch_rows<128, T>(p, ctas, s)
                                       : launch_rows<256, T>(p, ctas, s);
-    return e != cudaSuccess ? e : launch_combine<T>(p, hd, ctas, s);
+    return e != cudaSuccess ? e : launch_combine<T>(p, hd, ctas, sms, s);
 }
 
 struct Plan {
-    int rows, tiles, ctas;
+    int rows, tiles, ctas, sms;
     size_t bytes;
 };
 // How a call runs: set by the cache's dimensions and the batch's bounds alone, so that the workspace's size is too.
@@ -572,8 +603,9 @@ cudaError_t plan_of(int hd, int group, int max_q, Plan *pl) {
     const cudaError_t e = sm_count(&sms);
     if (e != cudaSuccess) return e;
     const bool prompt = static_cast<int64_t>(max_q) * group > kRows;
-    pl->rows = prompt ? kPromptRows : kRows;
-    pl->ctas = sms * (prompt ? prompt_ctas_per_sm(hd) : kRowsPerSm);
+    pl->sms = sms;
+    pl->rows = prompt ? prompt_rows(hd) : kRows;
+    pl->ctas = prompt ? sms : sms * kRowsPerSm;
     pl->tiles = static_cast<int>((static_cast<int64_t>(max_q) * group + pl->rows - 1) / pl->rows);
     pl->bytes = partials_bytes(pl->ctas, pl->rows, hd);
     return cudaSuccess;
@@ -654,7 +686,7 @@ extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_ba
     p.out_row = args->out_row_stride, p.out_head = args->out_head_stride;
     p.scale_log2 = args->scale * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    e = args->dtype == MG_BF16 ? launch_attention<__nv_bfloat16>(p, cache->head_dim, pl.ctas, s)
-                               : launch_attention<__half>(p, cache->head_dim, pl.ctas, s);
+    e = args->dtype == MG_BF16 ? launch_attention<__nv_bfloat16>(p, cache->head_dim, pl.ctas, pl.sms, s)
+                               : launch_attention<__half>(p, cache->head_dim, pl.ctas, pl.sms, s);
     return e == cudaSuccess ? MG_OK : cuda_error(who, e);
 }
