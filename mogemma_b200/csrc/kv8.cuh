@@ -19,7 +19,6 @@ mg_status report_error(mg_status st, const char *msg);
 namespace kv8 {
 
 constexpr int kBlock = MG_KV8_BLOCK;  // tokens per scale
-constexpr int kUnit = 64;             // tokens of one unit of the attention's schedule
 constexpr uint32_t kErrLens = 0x70000u, kErrPage = 0x80000u;  // err_dev codes: bad lengths, bad page id
 
 // The cache and the batch as the kernels see them.
@@ -86,20 +85,21 @@ __device__ __forceinline__ float ex2(float x) {  // PTX ex2.approx: one MUFU op,
 // ---- the attention's schedule
 // An item is (sequence, tile of ROWS query rows, kv head): the rows of a
 // sequence and kv head are its (token, q head of the group) pairs, token major.
-// Its cost is the number of 64-token units its rows see, at least one (rows
-// that see nothing still have an answer to write).  Items are laid out head by
+// Its cost is the number of units of 64 or 128 tokens its rows see, at least
+// one (rows that see nothing still have an answer to write).  Items are laid out head by
 // head, sequence by sequence; CTA c of G takes the units [c W / G, (c+1) W / G)
 // of all W, so the shares differ by one unit at most, whatever the lengths
 // (with fewer units than CTAs, the first W CTAs take one each).
 // Every CTA finds its place by the same scan over the items.
 struct AttnShape {
     int group, rows, tiles, window;  // q heads per kv head; rows per tile; tiles per sequence (of max_q tokens)
+    int unit;                        // tokens of a unit of the schedule
 };
 struct Item {
     Seq seq;
     int row0, nrows;     // rows of the tile
     int lo, hi;          // positions its rows see lie in [lo, hi)
-    int unit0, units;    // units unit0 .. unit0 + units - 1 (64 tokens each)
+    int unit0, units;    // units unit0 .. unit0 + units - 1
 };
 __device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, int pair, bool report) {
     Item it;
@@ -112,8 +112,8 @@ __device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, in
     const int first = it.seq.pos0 + it.row0 / a.group, last = it.seq.pos0 + (it.row0 + it.nrows - 1) / a.group;
     it.lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
     it.hi = max(last + 1, it.lo);
-    it.unit0 = it.lo / kUnit;
-    it.units = max(1, (it.hi + kUnit - 1) / kUnit - it.unit0);
+    it.unit0 = it.lo / a.unit;
+    it.units = max(1, (it.hi + a.unit - 1) / a.unit - it.unit0);
     return it;
 }
 

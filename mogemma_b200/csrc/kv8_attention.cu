@@ -33,11 +33,13 @@ mg_status check_cache_batch(const char *who, const mg_kv8_cache *c, const mg_kv8
 Cache cache_of(const mg_kv8_cache *c);
 Batch batch_of(const mg_kv8_batch *b);
 // kv8_prompt.cu
+constexpr int kPromptUnit = 128;
 int prompt_rows(int hd);
 cudaError_t launch_prompt(const AttnArgs &p, int hd, bool f16, int ctas, cudaStream_t s);
 
 namespace {
 constexpr int kRows = 8;       // query rows of an item
+constexpr int kUnit = 64;      // tokens of a unit of the schedule
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kInf = __builtin_huge_valf();
@@ -594,7 +596,7 @@ cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, int sms, cudaS
 }
 
 struct Plan {
-    int rows, tiles, ctas, sms;
+    int rows, unit, tiles, ctas, sms;
     size_t bytes;
 };
 // How a call runs: set by the cache's dimensions and the batch's bounds alone, so that the workspace's size is too.
@@ -605,6 +607,7 @@ cudaError_t plan_of(int hd, int group, int max_q, Plan *pl) {
     const bool prompt = static_cast<int64_t>(max_q) * group > kRows;
     pl->sms = sms;
     pl->rows = prompt ? prompt_rows(hd) : kRows;
+    pl->unit = prompt ? kPromptUnit : kUnit;
     pl->ctas = prompt ? sms : sms * kRowsPerSm;
     pl->tiles = static_cast<int>((static_cast<int64_t>(max_q) * group + pl->rows - 1) / pl->rows);
     pl->bytes = partials_bytes(pl->ctas, pl->rows, hd);
@@ -679,7 +682,7 @@ extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_ba
     AttnArgs p;
     p.c = cache_of(cache);
     p.b = batch_of(batch);
-    p.a = AttnShape{group, pl.rows, pl.tiles, args->window};
+    p.a = AttnShape{group, pl.rows, pl.tiles, args->window, pl.unit};
     p.part = partials_at(args->workspace_dev, pl.ctas, pl.rows);
     p.q = args->q_dev, p.out = args->out_dev;
     p.q_row = args->q_row_stride, p.q_head = args->q_head_stride;

@@ -4,9 +4,9 @@
 //
 // An item's query rows ((token, q head of the group) pairs of one kv head) are
 // one or two tiles of 128 (two for head dims 64 and 128, which then share every
-// widened key and value); its keys run in units of 64 tokens.  Both products
+// widened key and value); its keys run in units of 128 tokens.  Both products
 // are tcgen05.mma kind::f16 with fp32 accumulators in TMEM:
-//   S [128 x 64] = Q . K^T        Q and K fp16 in shared memory, K-major
+//   S [128 x 128] = Q . K^T       Q and K fp16 in shared memory, K-major
 //   O [128 x hd] += P . V         P fp16 in TMEM (over S), V fp16 MN-major
 // The cache's codes are widened to fp16, which is exact, on their way into
 // shared memory; q is brought into fp16's range by a power of two per row.  The
@@ -18,23 +18,31 @@
 // Warps of a CTA (640 threads, one CTA per SM):
 //  * warps 0-7: softmax.  Two row tiles: warpgroup g has tile g, a row per
 //    thread (TMEM lane = row).  One row tile (hd 256): warpgroup g has columns
-//    32 g .. 32 g + 31 of every row, and the two threads of a row exchange their
+//    64 g .. 64 g + 63 of every row, and the two threads of a row exchange their
 //    maxima.  They also bring the item's Q into shared memory and write the
 //    answers;
-//  * warps 8-11 load K, 12-15 V: codes from the pages into registers one or two units
-//    ahead (page ids one further), widened and stored in the 128-byte swizzled
-//    layout (token rows of 64 dims); tokens that no row sees become zeros, so
-//    that stale codes behind the context cannot reach a product;
-//  * warp 16: allocates TMEM; one lane issues the MMAs: S of unit j + 1 before
-//    P V of unit j, so that it runs under the softmax of unit j;
+//  * warps 8-11 load K, 12-15 V, by halves of 64 tokens: codes from the pages
+//    into registers one or two halves ahead (page ids one further), widened and
+//    stored in the 128-byte swizzled layout (token rows of 64 dims); tokens
+//    that no row sees become zeros, so that stale codes behind the context
+//    cannot reach a product;
+//  * warp 16: allocates TMEM and issues the MMAs;
 //  * warp 17: one lane walks the CTA's share of the schedule and hands the
-//    items to the others through a ring in shared memory.  Warps 18 and 19 only
-//    complete the warpgroup, whose registers go to the softmax.
-// K, V and each tile's S have two stages.  P overwrites the S stage it was made
-// from; the tensor pipe runs one thread's MMAs in order, so S of unit j + 2
-// lands after P V of unit j has read it.  O is rescaled only when M grows by
-// more than 8 (P stays below 2^8, within fp16's range).  A row tile takes no
-// part in units that none of its rows see.
+//    items to the others through a ring in shared memory.
+//
+// Two row tiles have one S stage each and take turns: P V and the next S of one
+// run under the softmax of the other.  One row tile has two S stages: S of unit
+// j + 1 is issued before P V of unit j and runs under its softmax.  P overwrites
+// the S it was made from; the tensor pipe runs one thread's MMAs in order, so
+// the next S on a stage lands after P V has read P.  K and V have two stages
+// each (hd 256: one; S and P V alternate, and either is reloaded under the
+// other).  O is rescaled only when M grows by more than 8 (P stays below 2^8,
+// within fp16's range).  A row tile takes no part in units that none of its
+// rows see.
+//
+// Units of 64 tokens were the first form: N = 64 reads Q from shared memory for
+// half the work (48 cycles per MMA against 64 for N = 128), and the waits
+// between roles (200 to 300 cycles each) came twice as often.
 //
 // Every wait is bounded; on expiry the kernel records kErrWait, every role
 // leaves its loop, TMEM is freed and the kernel returns.
@@ -48,15 +56,13 @@ namespace mg {
 namespace kv8 {
 namespace {
 constexpr int kM = 128;   // rows of a tile
-constexpr int kN = kUnit; // tokens of a unit
+constexpr int kN = 128;   // tokens of a unit
+constexpr int kHalf = 64; // tokens that a loader moves at a time
 constexpr int kThreads = 640;
-// Registers per thread: the block is launched with 96 (5 warps on an SM sub-partition); loaders and the issuing
-// warpgroup give up what the softmax takes: 2 x 120 + 2 x 80 + 80 = 5 x 96.
-constexpr int kSoftmaxRegs = 120, kLoadRegs = 80, kIssueRegs = 80;
 constexpr uint32_t kErrWait = 0x90000u;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kRescale = 8.0f;
-constexpr int kRing = 8;  // units whose scales are at hand: K's loader runs up to five units ahead of a softmax
+constexpr int kRing = 4;  // units whose scales are at hand
 
 template <int HD>
 struct Cfg {
@@ -64,10 +70,12 @@ struct Cfg {
     static constexpr int kRows = kTwo ? 2 * kM : kM;        // rows of an item
     static constexpr int kCols = kTwo ? kN : kN / 2;        // score columns of a softmax thread
     static constexpr int kAtoms = HD / 64;
-    static constexpr int kDepth = HD == 256 ? 1 : 2;        // units of codes that a loader holds: 32 registers at most
+    static constexpr int kDepth = HD == 256 ? 1 : 2;        // halves of codes that a loader holds: 32 registers at most
+    static constexpr int kStages = kTwo ? 2 : 1;            // of K and of V
+    static constexpr int kSStages = kTwo ? 1 : 2;           // of each tile's S
     static constexpr uint32_t kQBytes = kRows * HD * 2, kTileBytes = kN * HD * 2;
-    static constexpr uint32_t kS = (kTwo ? 2 : 1) * HD;     // TMEM: O of each tile, then S stages
-    static constexpr size_t kSmem = 1024 + kQBytes + 4 * kTileBytes;
+    static constexpr uint32_t kS = (kTwo ? 2 : 1) * HD;     // TMEM: O of each tile, then the S stages
+    static constexpr size_t kSmem = 1024 + kQBytes + 2 * kStages * kTileBytes;
 };
 constexpr uint32_t kTmemCols = 512;
 
@@ -82,29 +90,30 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lead)
     return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lead >> 4) << 16) | (64ull << 32) |
            (1ull << 46) | (2ull << 61);
 }
-// The issuing warp runs converged and one elected lane issues.  The instruction takes its operands from uniform
-// registers: they are constants off a few bases, with the stage a template argument and the accumulate flag a
-// constant; computed per MMA from loop variables, moving them there took longer than the MMA itself.
+// The whole issuing warp runs this code and lane 0 (`lead`) issues: one thread's MMAs run in order, and nothing depends
+// on the warp being converged, as an elect.sync here would.  The operands are constants off a few bases, with the
+// stage a template argument and the accumulate flag a constant.
 template <uint32_t IDESC, bool ACC>
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b) {
+__device__ __forceinline__ void umma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %3, 0;\n\t"
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %4, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "n"(ACC ? 1 : 0), "r"(IDESC)
+        "l"(a), "l"(b), "n"(ACC ? 1 : 0), "r"(IDESC), "r"(lead)
         : "memory");
 }
 template <uint32_t IDESC, bool ACC>
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b) {
+__device__ __forceinline__ void umma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %3, 0;\n\t"
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %4, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "n"(ACC ? 1 : 0), "r"(IDESC)
+        "r"(a), "l"(b), "n"(ACC ? 1 : 0), "r"(IDESC), "r"(lead)
         : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t *bar) {
+__device__ __forceinline__ void commit_if(uint32_t lead, uint64_t *bar) {
     asm volatile(
-        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(lead)
         : "memory");
 }
 // 32 columns of this thread's TMEM row; the caller waits (tmem_ld_wait) before it reads them.
@@ -152,8 +161,7 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
 }
 
 // Bounded wait.  err_dev may hold a bad page's code already, so a stop is announced in shared memory.
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err) {
-    if (mbar_try_wait(bar, parity)) return true;
+__device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err) {
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t n = 1;; ++n) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -166,6 +174,9 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
             }
         }
     }
+}
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err) {
+    return mbar_try_wait(bar, parity) || wait_long(bar, parity, stop, err);
 }
 
 // Two floats in one register pair: the packed fp32 operations.
@@ -266,16 +277,16 @@ constexpr int kItems = 4;
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs p) {
     using C = Cfg<HD>;
-    constexpr int kAtoms = C::kAtoms, kTiles = C::kTwo ? 2 : 1, kCols = C::kCols;
+    constexpr int kAtoms = C::kAtoms, kTiles = C::kTwo ? 2 : 1, kCols = C::kCols, kSt = C::kStages, kSS = C::kSStages;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[kRing], q_full[2], pair_bar[4][2], q_pair[4];
     __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems];
+    __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [tile][S stage]
     __shared__ Desc items_s[kItems];
-    __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [tile][stage]
-    __shared__ float sc_k[kRing][4], sc_v[kRing][4];  // scales of a unit's four blocks: K, log2 of V
-    __shared__ int sc_ok[kRing][4];
+    __shared__ float sc_k[kRing][8], sc_v[kRing][8];  // scales of a unit's eight blocks: K, log2 of V
+    __shared__ int sc_ok[kRing][8];
     __shared__ float q_down[C::kRows];
-    __shared__ float2 xch[2][2][kM];  // one row tile: the two halves' maxima (by unit parity)
+    __shared__ float2 xch[2][2][kM];  // one row tile: the two halves' maxima (by S stage)
     __shared__ uint32_t tmem_slot;
     __shared__ int stop_s;
     volatile int *stop = &stop_s;
@@ -283,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     asm volatile("griddepcontrol.launch_dependents;");
     const uintptr_t base = (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023);
     unsigned char *gen = reinterpret_cast<unsigned char *>(base);
-    const uint32_t sq = smem_u32(gen), sk = sq + C::kQBytes, sv = sk + 2 * C::kTileBytes;
+    const uint32_t sq = smem_u32(gen), sk = sq + C::kQBytes, sv = sk + kSt * C::kTileBytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cta = blockIdx.x;
 
@@ -324,7 +335,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const uint32_t units = static_cast<uint32_t>(pl.w1 - pl.w0);
     // The i-th item; null at the end of the share, or (stop set) when a wait ran out.
     auto item = [&](uint32_t i) -> const Desc * {
         const bool ok = wait(&item_full[i % kItems], (i / kItems) & 1u, stop, err);
@@ -339,75 +349,112 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         return __all_sync(0xffffffffu, wait(bar, parity, stop, err));
     };
 
-    if (warp >= 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        if (warp == 16) {  // ---- MMA issuer
-            constexpr uint32_t kIdS = idesc_f16(kM, kN, 0), kIdO = idesc_f16(kM, HD, 1);
-            // descriptors count in 16 bytes; shared memory ends below their 2^14
-            const uint64_t qd = tc::sw128_desc(sq), kd = tc::sw128_desc(sk), vd = sw128_mn_desc(sv, kN * 128);
-            uint32_t n = 0;                                       // units so far
-            uint32_t acts[2] = {0, 0};                            // a tile's items so far in which it sees something
-            uint32_t uses[2][2] = {{0, 0}, {0, 0}};               // [tile][stage] P V issued
-            bool ok = true;
-            for (uint32_t i = 0; ok; ++i) {
-                const Desc *d = warp_item(i);
-                if (!d) break;
-                const int take = d->take;
-                bool begun[2] = {false, false};
-                auto s_of = [&](auto stage, uint32_t u, int j) -> bool {  // S of unit u, the item's j-th
-                    constexpr uint32_t ST = decltype(stage)::value;
-                    if (!warp_wait(&k_full[ST], (u >> 1) & 1u)) return false;
-                    tc::tc_fence_after();
+    if (warp == 16) {  // ---- MMA issuer
+        constexpr uint32_t kIdS = idesc_f16(kM, kN, 0), kIdO = idesc_f16(kM, HD, 1);
+        // descriptors count in 16 bytes; shared memory ends below their 2^14
+        const uint64_t qd = tc::sw128_desc(sq), kd = tc::sw128_desc(sk), vd = sw128_mn_desc(sv, kN * 128);
+        const uint32_t lead = lane == 0 ? 1u : 0u;
+        auto commit = [&](uint64_t *bar) { commit_if(lead, bar); };
+        uint32_t n = 0;              // units so far
+        uint32_t acts[2] = {0, 0};   // a tile's items so far in which it sees something
+        uint32_t uses[2][2] = {{0, 0}, {0, 0}};  // [tile][S stage]: P V issued
+        bool ok = true;
+        for (uint32_t i = 0; ok; ++i) {
+            const Desc *d = warp_item(i);
+            if (!d) break;
+            const int take = d->take;
+            bool begun[2] = {false, false};
+            // S of tile g and the unit on K stage KS into S stage SS
+            auto s_of = [&](auto kstage, auto sstage, auto tile) {
+                constexpr uint32_t KS = decltype(kstage)::value, SS = decltype(sstage)::value, G = decltype(tile)::value;
+                const uint32_t t = tmem + C::kS + (kSS * G + SS) * kN;
 #pragma unroll
-                    for (int g = 0; g < kTiles; ++g) {
-                        if (!d->sees(g, d->token(j))) continue;
-                        const uint32_t t = tmem + C::kS + (2 * g + ST) * kN;
-#pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk) {
-                            const uint64_t qa = qd + (((kk >> 2) * C::kRows * 128 + g * kM * 128 + (kk & 3) * 32) >> 4);
-                            const uint64_t kb = kd + ((ST * C::kTileBytes + (kk >> 2) * kN * 128 + (kk & 3) * 32) >> 4);
-                            if (kk == 0) umma_ss<kIdS, false>(t, qa, kb);
-                            else umma_ss<kIdS, true>(t, qa, kb);
-                        }
-                        commit(&s_full[g][ST]);
-                    }
-                    commit(&k_empty[ST]);
-                    return true;
-                };
-                auto pv_of = [&](auto stage, uint32_t u, int j) -> bool {  // P V of unit u
-                    constexpr uint32_t ST = decltype(stage)::value;
-                    if (!warp_wait(&v_full[ST], (u >> 1) & 1u)) return false;
-#pragma unroll
-                    for (int g = 0; g < kTiles; ++g) {
-                        if (!d->sees(g, d->token(j))) continue;
-                        if (!warp_wait(&p_full[g][ST], uses[g][ST]++ & 1u)) return false;
-                        tc::tc_fence_after();
-                        const uint32_t o = tmem + g * HD, t = tmem + C::kS + (2 * g + ST) * kN;
-                        const uint64_t vb = vd + ((ST * C::kTileBytes) >> 4);
-                        if (begun[g]) umma_ts<kIdO, true>(o, t, vb);
-                        else umma_ts<kIdO, false>(o, t, vb);
-                        begun[g] = true;
-#pragma unroll
-                        for (int kk = 1; kk < kN / 16; ++kk) umma_ts<kIdO, true>(o, t + kk * 8, vb + ((kk * 2048) >> 4));
-                        commit(&pv_done[g][ST]);
-                    }
-                    commit(&v_empty[ST]);
-                    return true;
-                };
-                using S0 = std::integral_constant<uint32_t, 0>;
-                using S1 = std::integral_constant<uint32_t, 1>;
-#pragma unroll
-                for (int g = 0; g < kTiles; ++g)
-                    if (d->sees(g, d->tok0, take)) ok = ok && warp_wait(&q_full[g], acts[g]++ & 1u);
-                if (ok) ok = n & 1 ? s_of(S1(), n, 0) : s_of(S0(), n, 0);
-                for (int j = 0; ok && j < take; ++j, ++n) {
-                    if (n & 1) ok = (j + 1 == take || s_of(S0(), n + 1, j + 1)) && pv_of(S1(), n, j);
-                    else ok = (j + 1 == take || s_of(S1(), n + 1, j + 1)) && pv_of(S0(), n, j);
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    const uint64_t qa = qd + (((kk >> 2) * C::kRows * 128 + G * kM * 128 + (kk & 3) * 32) >> 4);
+                    const uint64_t kb = kd + ((KS * C::kTileBytes + (kk >> 2) * kN * 128 + (kk & 3) * 32) >> 4);
+                    if (kk == 0) umma_ss<kIdS, false>(lead, t, qa, kb);
+                    else umma_ss<kIdS, true>(lead, t, qa, kb);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&item_empty[i % kItems]);
+                commit(&s_full[G][SS]);
+            };
+            // P V of tile g: P in S stage SS, V stage VS
+            auto pv_of = [&](auto vstage, auto sstage, auto tile) -> bool {
+                constexpr uint32_t VS = decltype(vstage)::value, SS = decltype(sstage)::value, G = decltype(tile)::value;
+                if (!warp_wait(&p_full[G][SS], uses[G][SS]++ & 1u)) return false;
+                tc::tc_fence_after();
+                const uint32_t o = tmem + G * HD, t = tmem + C::kS + (kSS * G + SS) * kN;
+                const uint64_t vb = vd + ((VS * C::kTileBytes) >> 4);
+                if (begun[G]) umma_ts<kIdO, true>(lead, o, t, vb);
+                else umma_ts<kIdO, false>(lead, o, t, vb);
+                begun[G] = true;
+#pragma unroll
+                for (int kk = 1; kk < kN / 16; ++kk) {
+                    // P's columns: 8 per step of 16 tokens; one row tile: the second half's behind column kN / 2
+                    const uint32_t col = C::kTwo || kk < 4 ? kk * 8 : kN / 2 + (kk - 4) * 8;
+                    umma_ts<kIdO, true>(lead, o, t + col, vb + ((kk * 2048) >> 4));
+                }
+                commit(&pv_done[G][SS]);
+                return true;
+            };
+            using I0 = std::integral_constant<uint32_t, 0>;
+            using I1 = std::integral_constant<uint32_t, 1>;
+            auto sees = [&](int g, int j) { return j < take && d->sees(g, d->token(j)); };
+#pragma unroll
+            for (int g = 0; g < kTiles; ++g)
+                if (d->sees(g, d->tok0, take)) ok = ok && warp_wait(&q_full[g], acts[g]++ & 1u);
+            if constexpr (C::kTwo) {
+                // K of unit u, the item's j-th, has landed
+                auto k_wait = [&](uint32_t u) -> bool {
+                    if (!warp_wait(&k_full[u & 1], (u >> 1) & 1u)) return false;
+                    tc::tc_fence_after();
+                    return true;
+                };
+                ok = ok && k_wait(n);
+                if (!ok) break;
+                auto first = [&](auto st) {
+                    if (sees(0, 0)) s_of(st, I0(), I0());
+                    if (sees(1, 0)) s_of(st, I0(), I1());
+                    commit(&k_empty[decltype(st)::value]);
+                };
+                if (n & 1) first(I1());
+                else first(I0());
+                // unit j: P V of a tile, then its next S
+                auto step = [&](auto st, auto nx, int j) -> bool {
+                    constexpr uint32_t ST = decltype(st)::value, NX = decltype(nx)::value;
+                    if (!warp_wait(&v_full[ST], (n >> 1) & 1u)) return false;
+                    if (sees(0, j) && !pv_of(st, I0(), I0())) return false;
+                    if (j + 1 < take && !k_wait(n + 1)) return false;
+                    if (sees(0, j + 1)) s_of(nx, I0(), I0());
+                    if (sees(1, j) && !pv_of(st, I0(), I1())) return false;
+                    commit(&v_empty[ST]);
+                    if (sees(1, j + 1)) s_of(nx, I0(), I1());
+                    if (j + 1 < take) commit(&k_empty[NX]);
+                    return true;
+                };
+                for (int j = 0; ok && j < take; ++j, ++n) ok = n & 1 ? step(I1(), I0(), j) : step(I0(), I1(), j);
+            } else {
+                auto s_unit = [&](auto ss, uint32_t u, int j) -> bool {
+                    if (!warp_wait(&k_full[0], u & 1u)) return false;
+                    tc::tc_fence_after();
+                    if (sees(0, j)) s_of(I0(), ss, I0());
+                    commit(&k_empty[0]);
+                    return true;
+                };
+                auto step = [&](auto ss, auto nx, int j) -> bool {
+                    if (j + 1 < take && !s_unit(nx, n + 1, j + 1)) return false;
+                    if (!warp_wait(&v_full[0], n & 1u)) return false;
+                    if (sees(0, j) && !pv_of(I0(), ss, I0())) return false;
+                    commit(&v_empty[0]);
+                    return true;
+                };
+                if (ok) ok = n & 1 ? s_unit(I1(), n, 0) : s_unit(I0(), n, 0);
+                for (int j = 0; ok && j < take; ++j, ++n) ok = n & 1 ? step(I1(), I0(), j) : step(I0(), I1(), j);
             }
-        } else if (warp == 17 && lane == 0) {  // ---- walker
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[i % kItems]);
+        }
+    } else if (warp == 17) {  // ---- walker
+        if (lane == 0) {
             Walk wk;
             p.part.split[cta].nrows = 0;
             bool more = wk.start(p, pl);
@@ -440,31 +487,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                     }
                     d.slot = whole ? -1 : slot;
                     if (wk.skip == 0 && !whole)
-                        p.part.split[cta] = Split{wk.pair, wk.head, it.nrows, slot, owner_of(pl, wk.w + it.units - 1), {0, 0, 0}};
+                        p.part.split[cta] =
+                            Split{wk.pair, wk.head, it.nrows, slot, owner_of(pl, wk.w + it.units - 1), {0, 0, 0}};
                 }
                 mbar_arrive(&item_full[i % kItems]);
                 if (!more) break;
                 more = wk.next(p);
             }
         }
-    } else if (warp >= 8) {  // ---- loaders: K or V
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+    } else if (warp >= 8 && warp < 16) {  // ---- loaders: K or V
         const bool is_k = warp < 12;
         const int u = (threadIdx.x - 256) & 127, quad = u >> 2, sub = u & 3;
-        const bool leader = sub == 0 && (quad & 15) == 0;  // holds the scales of blocks quad / 16 and quad / 16 + 2
+        const bool leader = sub == 0 && (quad & 15) == 0;  // holds the scales of a half's blocks quad / 16 and quad / 16 + 2
         const uint8_t *codes = (is_k ? p.c.k : p.c.v) + 16 * sub;
         const float *scales = is_k ? p.c.k_scale : p.c.v_scale;
         uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
-        unsigned char *stage0 = gen + C::kQBytes + (is_k ? 0 : 2 * C::kTileBytes);
+        unsigned char *stage0 = gen + C::kQBytes + (is_k ? 0 : kSt * C::kTileBytes);
         const int slot_mask = (1 << p.c.page_shift) - 1;
-        // the unit whose page ids are being read: the j-th of item i_at
+        // the half whose page ids are being read: the j-th of item i_at
         int j = 0, pg[2], pg_tok = 0, pg_head = 0;
         uint32_t i_at = 0;
         bool pg_on[2] = {false, false};
         const Desc *d = warp_item(0);
         auto read_pages = [&]() {
             if (!d) return;
-            pg_tok = d->token(j) + quad;
+            pg_tok = d->tok0 + j * kHalf + quad;
             pg_head = d->head;
             const int32_t *table = p.b.table + d->seq * p.b.table_stride;
 #pragma unroll
@@ -473,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                 pg_on[i] = tok >= d->lo && tok < d->hi;  // pages before a window may be gone
                 pg[i] = pg_on[i] ? table[tok >> p.c.page_shift] : 0;
             }
-            if (++j == d->take) {
+            if (++j == 2 * d->take) {
                 j = 0;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&item_empty[i_at % kItems]);
@@ -503,12 +550,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                 }
             }
         };
-        // unit n from buffer b; false when a wait ran out
-        auto store = [&](uint32_t n, int b) -> bool {
+        // the h-th half (unit h / 2) from buffer b; false when a wait ran out
+        auto store = [&](uint32_t h, int b) -> bool {
+            const uint32_t n = h >> 1, hh = h & 1, st = n % kSt;
+            if (hh == 0 && n >= kSt && !warp_wait(&empty[st], (n / kSt - 1) & 1u)) return false;
             if (leader) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int blk = (quad >> 4) + 2 * i;
+                    const int blk = 4 * hh + (quad >> 4) + 2 * i;
                     if (is_k) {
                         sc_k[n % kRing][blk] = sc[b][i];
                         sc_ok[n % kRing][blk] = ok_b[b][i];
@@ -517,14 +566,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sc_full[n % kRing]);
-            const uint32_t st = n & 1;
-            if (n >= 2 && !warp_wait(&empty[st], ((n >> 1) - 1) & 1u)) return false;
             unsigned char *tile = stage0 + st * C::kTileBytes;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int row = quad + 32 * i;
+                const int row = kHalf * hh + quad + 32 * i;
 #pragma unroll
                 for (int a = 0; a < kAtoms; ++a) {  // 16 codes -> two 16-byte chunks of the 128-byte row, swizzled
                     uint4 lo, hi;
@@ -537,106 +582,95 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                     *reinterpret_cast<uint4 *>(dst + (((2 * sub + 1) ^ (row & 7)) << 4)) = hi;
                 }
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[st]);
+            if (hh == 1) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sc_full[n % kRing]);
+                    mbar_arrive(&full[st]);
+                }
+            }
             return true;
         };
+        const uint32_t halves = 2 * static_cast<uint32_t>(pl.w1 - pl.w0);
         read_pages();
 #pragma unroll
         for (int b = 0; b < C::kDepth; ++b) {
-            if (static_cast<uint32_t>(b) < units) read_codes(b);
+            if (static_cast<uint32_t>(b) < halves) read_codes(b);
             read_pages();
         }
         bool ok = true;
-        for (uint32_t n0 = 0; ok && n0 < units; n0 += C::kDepth) {
+        for (uint32_t h0 = 0; ok && h0 < halves; h0 += C::kDepth) {
 #pragma unroll
             for (int b = 0; b < C::kDepth; ++b) {
-                const uint32_t n = n0 + b;
-                if (!ok || n >= units) continue;
-                ok = store(n, b);
-                if (ok && n + C::kDepth < units) read_codes(b);
+                const uint32_t h = h0 + b;
+                if (!ok) continue;  // halves is a multiple of kDepth
+                ok = store(h, b);
+                if (ok && h + C::kDepth < halves) read_codes(b);
                 read_pages();
             }
         }
-    } else {  // ---- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    } else if (warp < 8) {  // ---- softmax
         const int wg = warp >> 2, tg = C::kTwo ? wg : 0, r = 32 * (warp & 3) + lane;  // tile and row of this thread
         const int col0 = C::kTwo ? 0 : wg * kCols;
         const uint32_t lane_off = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t t_o = tmem + tg * HD + lane_off, t_s0 = tmem + C::kS + 2 * tg * kN + lane_off;
+        const uint32_t t_o = tmem + tg * HD + lane_off, t_s0 = tmem + C::kS + kSS * tg * kN + lane_off;
         uint32_t n = 0, acts = 0;         // units of the share; items in which this tile sees something
-        uint32_t uses = 0;                // bit st: parity of the tile's uses of stage st
+        uint32_t uses = 0;                // bit st: parity of the tile's uses of S stage st
         bool ok = true;
         for (uint32_t i_at = 0;; ++i_at) {
             const Desc *d = warp_item(i_at);
             if (!d) break;
             const int t_rows = d->t_rows[tg], take = d->take;
             const bool active = d->sees(tg, d->tok0, take);
-            // Q: a warp brings kQR rows, lane d with HD / 32 values of each; a row's largest becomes 2^7 .. 2^8
             if (active) {
-                constexpr int kW = HD / 64, kQR = C::kTwo ? 32 : 16, kBatch = kW == 4 ? 8 : 16;
-                const int qr0 = kQR * warp;  // of the item
-                int64_t off = 0;
+                // Q: a warp brings kQR rows, 8 at a time, 4 lanes to a row; a row's largest becomes 2^7 .. 2^8
+                constexpr int kQR = C::kTwo ? 32 : 16, kCh = HD / 32;  // 16-byte chunks of a lane: 4 i + lane % 4
                 const int nrows = d->nrows;
-                if (lane < kQR && qr0 + lane < nrows) {
-                    const int row = d->row0 + qr0 + lane, tok = row / p.a.group;
-                    off = (static_cast<int64_t>(d->q0) + tok) * p.q_row +
-                          (d->head * p.a.group + row - tok * p.a.group) * p.q_head;
-                }
 #pragma unroll 1
-                for (int r0 = 0; r0 < kQR && qr0 + r0 < nrows; r0 += kBatch) {
-                    uint32_t q[kBatch][kW];
+                for (int r0 = kQR * warp; r0 < kQR * (warp + 1) && r0 < nrows; r0 += 8) {
+                    const int lr = r0 + (lane >> 2), sub = lane & 3;  // row of the item
+                    const bool on = lr < nrows;
+                    const int row = d->row0 + (on ? lr : r0), tok = row / p.a.group;
+                    const T *src = static_cast<const T *>(p.q) + (static_cast<int64_t>(d->q0) + tok) * p.q_row +
+                                   (d->head * p.a.group + row - tok * p.a.group) * p.q_head + 8 * sub;
+                    uint4 q[kCh];
+                    uint32_t most = 0;
 #pragma unroll
-                    for (int i = 0; i < kBatch; ++i) {
-                        const T *src = static_cast<const T *>(p.q) + __shfl_sync(0xffffffffu, off, r0 + i) + lane * 2 * kW;
+                    for (int i = 0; i < kCh; ++i) q[i] = *reinterpret_cast<const uint4 *>(src + 32 * i);
 #pragma unroll
-                        for (int w = 0; w < kW; ++w) q[i][w] = 0;
-                        if (qr0 + r0 + i < nrows) {
-                            if constexpr (kW == 1) {
-                                q[i][0] = *reinterpret_cast<const uint32_t *>(src);
-                            } else if constexpr (kW == 2) {
-                                const uint2 v = *reinterpret_cast<const uint2 *>(src);
-                                q[i][0] = v.x, q[i][1] = v.y;
-                            } else {
-                                const uint4 v = *reinterpret_cast<const uint4 *>(src);
-                                q[i][0] = v.x, q[i][1] = v.y, q[i][2] = v.z, q[i][3] = v.w;
-                            }
-                        }
-                    }
+                    for (int i = 0; i < kCh; ++i)
 #pragma unroll
-                    for (int i = 0; i < kBatch; ++i) {
-                        const int lr = qr0 + r0 + i;
-                        uint32_t most = 0;
-#pragma unroll
-                        for (int w = 0; w < kW; ++w) {
-                            const float2 f = two<T>(q[i][w]);
+                        for (int w = 0; w < 4; ++w) {
+                            const float2 f = two<T>((&q[i].x)[w]);
                             most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
                         }
-                        most = __reduce_max_sync(0xffffffffu, most);
-                        const int e = static_cast<int>(most >> 23);
-                        float up = 1.0f, down = 1.0f;
-                        if (e >= 255) {  // a row with an infinity or NaN answers NaN
-                            down = __int_as_float(0x7fc00000);
-                        } else if (e > 0) {
-                            const int sh = min(134 - e, 126);
-                            up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
-                            down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
-                        }
-                        if (p.scale_log2 < 0.f) up = -up;  // factors of S stay positive
-                        if (lane == 0) q_down[lr] = down;
-                        uint32_t hw[kW];
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    const int e = static_cast<int>(most >> 23);
+                    float up = 1.0f, down = 1.0f;
+                    if (e >= 255) {  // a row with an infinity or NaN answers NaN
+                        down = __int_as_float(0x7fc00000);
+                    } else if (e > 0) {
+                        const int sh = min(134 - e, 126);
+                        up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
+                        down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
+                    }
+                    if (p.scale_log2 < 0.f) up = -up;  // factors of S stay positive
+                    if (on) {
+                        if (sub == 0) q_down[lr] = down;
 #pragma unroll
-                        for (int w = 0; w < kW; ++w) {
-                            const float2 f = two<T>(q[i][w]);
-                            hw[w] = pack(f.x * up, f.y * up, __half());
+                        for (int i = 0; i < kCh; ++i) {
+                            uint4 hw;
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                const float2 f = two<T>((&q[i].x)[w]);
+                                (&hw.x)[w] = pack(f.x * up, f.y * up, __half());
+                            }
+                            const int chunk = 4 * (i & 1) + sub;  // of atom i / 2
+                            *reinterpret_cast<uint4 *>(gen + (i >> 1) * C::kRows * 128 + lr * 128 +
+                                                       ((chunk ^ (lr & 7)) << 4)) = hw;
                         }
-                        // byte 4 kW lane of the row: atom, chunk and offset
-                        const int byte = 4 * kW * lane, atom = byte >> 7, chunk = (byte >> 4) & 7, in = byte & 15;
-                        unsigned char *dst = gen + atom * C::kRows * 128 + lr * 128 + ((chunk ^ (lr & 7)) << 4) + in;
-                        if constexpr (kW == 1) *reinterpret_cast<uint32_t *>(dst) = hw[0];
-                        else if constexpr (kW == 2) *reinterpret_cast<uint2 *>(dst) = make_uint2(hw[0], hw[1]);
-                        else *reinterpret_cast<uint4 *>(dst) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
                     }
                 }
                 fence_proxy_async_smem();
@@ -652,51 +686,56 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
 
             float m = -kInf, mref = -kInf, l = 0.f;
             bool begun = false;
-            uint32_t last = 0;  // stage of the tile's latest unit
+            uint32_t last = 0;  // S stage of the tile's latest unit
             for (int j = 0; j < take; ++j, ++n) {
                 const int t0 = d->token(j);
                 if (!d->sees(tg, t0)) continue;
-                const uint32_t st = n & 1, ph = uses >> st & 1u;
+                const uint32_t st = n % kSS, ph = uses >> st & 1u, ring = n % kRing;
                 // S first: a tile that sat out many units is then within one phase of the scales' barrier
-                ok = warp_wait(&s_full[tg][st], ph) && warp_wait(&sc_full[n % kRing], (n / kRing) & 1u);
+                ok = warp_wait(&s_full[tg][st], ph) && warp_wait(&sc_full[ring], (n / kRing) & 1u);
                 if (!ok) break;
                 tc::tc_fence_after();
                 if (any_rows) {
-                    const uint32_t t_s = t_s0 + st * kN;
-                    constexpr int kB = kCols / 16;  // scale blocks of this thread's columns
-                    float s[kCols], cf[kB], lv[kB];
-                    tmem_ld32_async(t_s + col0, s);
-                    if constexpr (kCols == 64) tmem_ld32_async(t_s + 32, s + 32);
+                    const uint32_t t_s = t_s0 + st * kN + col0;
+                    const int tc0 = t0 + col0;
                     bool blocks_ok = true;
 #pragma unroll
-                    for (int b = 0; b < kB; ++b) {
-                        cf[b] = factor * sc_k[n % kRing][col0 / 16 + b];
-                        lv[b] = sc_v[n % kRing][col0 / 16 + b];
-                        blocks_ok = blocks_ok && sc_ok[n % kRing][col0 / 16 + b] != 0;
-                    }
-                    tmem_ld_wait(s);
-                    const int tc0 = t0 + col0;
-                    const bool all = !row_on || (blocks_ok && lo <= tc0 && tc0 + kCols <= hi);
-                    if (!__all_sync(0xffffffffu, all)) {
+                    for (int b = 0; b < kCols / 16; ++b) blocks_ok = blocks_ok && sc_ok[ring][col0 / 16 + b] != 0;
+                    const bool full =
+                        __all_sync(0xffffffffu, !row_on || (blocks_ok && lo <= tc0 && tc0 + kCols <= hi));
+                    // 32 columns: scores, or (partly seen units) the masked products with the factors folded in
+                    auto scores = [&](int x, float (&s)[32], float (&cf)[2]) {
+                        tmem_ld32_async(t_s + 32 * x, s);
+                        cf[0] = factor * sc_k[ring][col0 / 16 + 2 * x];
+                        cf[1] = factor * sc_k[ring][col0 / 16 + 2 * x + 1];
+                        tmem_ld_wait(s);
+                        if (!full) {
 #pragma unroll
-                        for (int b = 0; b < kB; ++b) {
-                            const bool on = sc_ok[n % kRing][col0 / 16 + b] != 0;
+                            for (int b = 0; b < 2; ++b) {
+                                const bool on = sc_ok[ring][col0 / 16 + 2 * x + b] != 0;
+                                const int at = tc0 + 32 * x;
 #pragma unroll
-                            for (int i = 16 * b; i < 16 * b + 16; ++i)
-                                s[i] = on && tc0 + i >= lo && tc0 + i < hi ? s[i] * cf[b] : -kInf;
-                            cf[b] = 1.0f;
+                                for (int i = 16 * b; i < 16 * b + 16; ++i)
+                                    s[i] = on && at + i >= lo && at + i < hi ? s[i] * cf[b] : -kInf;
+                                cf[b] = 1.0f;
+                            }
                         }
-                    }
+                    };
                     float mn = -kInf, vn = -kInf;
+#pragma unroll 1
+                    for (int x = 0; x < kCols / 32; ++x) {
+                        float s[32], cf[2];
+                        scores(x, s, cf);
 #pragma unroll
-                    for (int b = 0; b < kB; ++b) {
-                        const float *x = s + 16 * b;
-                        float a0 = max3(x[0], x[1], x[2]), a1 = max3(x[3], x[4], x[5]);
-                        a0 = max3(a0, x[6], x[7]), a1 = max3(a1, x[8], x[9]);
-                        a0 = max3(a0, x[10], x[11]), a1 = max3(a1, x[12], x[13]);
-                        const float t = fmaxf(max3(a0, x[14], x[15]), a1) * cf[b];
-                        mn = fmaxf(mn, t);
-                        vn = fmaxf(vn, t + lv[b]);
+                        for (int b = 0; b < 2; ++b) {
+                            const float *y = s + 16 * b;
+                            float a0 = max3(y[0], y[1], y[2]), a1 = max3(y[3], y[4], y[5]);
+                            a0 = max3(a0, y[6], y[7]), a1 = max3(a1, y[8], y[9]);
+                            a0 = max3(a0, y[10], y[11]), a1 = max3(a1, y[12], y[13]);
+                            const float t = fmaxf(max3(a0, y[14], y[15]), a1) * cf[b];
+                            mn = fmaxf(mn, t);
+                            vn = fmaxf(vn, t + sc_v[ring][col0 / 16 + 2 * x + b]);
+                        }
                     }
                     if constexpr (!C::kTwo) {  // the other half's columns
                         xch[st][wg][r] = make_float2(mn, vn);
@@ -717,10 +756,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                     if (move) mref = vn;
                     const float rb = finite_or_0(mref);
                     if (begun && __any_sync(0xffffffffu, move)) {
-                        // O holds P V of this tile's units so far once the last one is done
-                        ok = warp_wait(&pv_done[tg][st ^ 1], (uses >> (st ^ 1) & 1u) ^ 1u);
-                        if (!ok) break;
-                        tc::tc_fence_after();
+                        // O must hold P V of all this tile's units so far.  One S stage: S of this unit was issued
+                        // after them, so it does.
+                        if constexpr (!C::kTwo) {
+                            ok = warp_wait(&pv_done[tg][st ^ 1], (uses >> (st ^ 1) & 1u) ^ 1u);
+                            if (!ok) break;
+                            tc::tc_fence_after();
+                        }
                         const float f = move ? ex2(old - rb) : 1.0f;
                         constexpr int kOc = C::kTwo ? HD : HD / 2;
 #pragma unroll 1
@@ -733,27 +775,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                             tc::tmem_st32(at, o);
                         }
                     }
-                    uint32_t pk[kCols / 2];
                     F2 sum = f2(0.f, 0.f);
                     const F2 nm = f2(-mb, -mb);
+#pragma unroll 1
+                    for (int x = 0; x < kCols / 32; ++x) {
+                        float s[32], cf[2];
+                        uint32_t pk[16];
+                        scores(x, s, cf);
 #pragma unroll
-                    for (int b = 0; b < kB; ++b) {
-                        const float wv = ex2(fminf(lv[b] + mb - rb, 126.f));
-                        const F2 w2 = f2(wv, wv), c2 = f2(cf[b], cf[b]);
+                        for (int b = 0; b < 2; ++b) {
+                            const float wv = ex2(fminf(sc_v[ring][col0 / 16 + 2 * x + b] + mb - rb, 126.f));
+                            const F2 w2 = f2(wv, wv), c2 = f2(cf[b], cf[b]);
 #pragma unroll
-                        for (int i = 16 * b; i < 16 * b + 16; i += 2) {
-                            float e0, e1;
-                            un2(fma2(f2(s[i], s[i + 1]), c2, nm), e0, e1);
-                            const F2 e = f2(ex2(e0), ex2(e1));
-                            sum = add2(sum, e);
-                            un2(mul2(e, w2), e0, e1);
-                            pk[i / 2] = pack(e0, e1, __half());
+                            for (int i = 16 * b; i < 16 * b + 16; i += 2) {
+                                float e0, e1;
+                                un2(fma2(f2(s[i], s[i + 1]), c2, nm), e0, e1);
+                                const F2 e = f2(ex2(e0), ex2(e1));
+                                sum = add2(sum, e);
+                                un2(mul2(e, w2), e0, e1);
+                                pk[i / 2] = pack(e0, e1, __half());
+                            }
                         }
+                        tmem_st(t_s + 16 * x, pk);  // over columns that have been read
                     }
                     float s0, s1;
                     un2(sum, s0, s1);
                     l += s0 + s1;
-                    tmem_st(t_s + col0 / 2, pk);
                 }
                 begun = true;
                 tc::tc_fence_before();
@@ -768,13 +815,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                 if (!ok) break;
                 tc::tc_fence_after();
             }
-            if constexpr (!C::kTwo) {  // the two halves' sums; the pair's barrier has another phase per item
-                xch[0][wg][r] = make_float2(l, 0.f);
+            if constexpr (!C::kTwo) {  // the two halves' sums
+                xch[i_at & 1][wg][r] = make_float2(l, 0.f);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_pair[warp & 3]);
                 ok = warp_wait(&q_pair[warp & 3], i_at & 1u);
                 if (!ok) break;
-                l = xch[0][0][r].x + xch[0][1][r].x;
+                l = xch[i_at & 1][0][r].x + xch[i_at & 1][1][r].x;
             }
             if (any_rows) {
                 const int slot = d->slot;
