@@ -86,20 +86,22 @@ __device__ __forceinline__ float ex2(float x) {  // PTX ex2.approx: one MUFU op,
 // An item is (sequence, tile of ROWS query rows, kv head): the rows of a
 // sequence and kv head are its (token, q head of the group) pairs, token major.
 // Its cost is the number of units of 64 or 128 tokens its rows see, at least
-// one (rows that see nothing still have an answer to write).  Items are laid out head by
+// one (rows that see nothing still have an answer to write), plus a constant
+// for its start and end that counts as units before the first.  Items are laid out head by
 // head, sequence by sequence; CTA c of G takes the units [c W / G, (c+1) W / G)
 // of all W, so the shares differ by one unit at most, whatever the lengths
 // (with fewer units than CTAs, the first W CTAs take one each).
 // Every CTA finds its place by the same scan over the items.
 struct AttnShape {
     int group, rows, tiles, window;  // q heads per kv head; rows per tile; tiles per sequence (of max_q tokens)
-    int unit;                        // tokens of a unit of the schedule
+    int unit, extra;                 // tokens of a unit of the schedule; cost of an item beside its units
 };
 struct Item {
     Seq seq;
     int row0, nrows;     // rows of the tile
     int lo, hi;          // positions its rows see lie in [lo, hi)
     int unit0, units;    // units unit0 .. unit0 + units - 1
+    int cost;            // extra + units; 0: no rows
 };
 __device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, int pair, bool report) {
     Item it;
@@ -107,21 +109,22 @@ __device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, in
     it.seq = load_seq(b, i, report);
     it.row0 = t * a.rows;
     it.nrows = min(a.rows, it.seq.nq * a.group - it.row0);
-    it.units = 0;
+    it.units = it.cost = 0;
     if (it.nrows <= 0) return it;
     const int first = it.seq.pos0 + it.row0 / a.group, last = it.seq.pos0 + (it.row0 + it.nrows - 1) / a.group;
     it.lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
     it.hi = max(last + 1, it.lo);
     it.unit0 = it.lo / a.unit;
     it.units = max(1, (it.hi + a.unit - 1) / a.unit - it.unit0);
+    it.cost = it.units + a.extra;
     return it;
 }
 
-// Where CTA `cta` of `ctas` starts: its unit range [w0, w1) of the whole, and
-// the item (head, pair) and the unit within it of w0.  All threads of the CTA
+// Where CTA `cta` of `ctas` starts: its range [w0, w1) of the whole cost, and
+// the item (head, pair) and the place within it of w0.  All threads of the CTA
 // call it; THREADS a multiple of 32.
 struct Place {
-    int64_t total, per_head;  // units of all heads, of one
+    int64_t total, per_head;  // cost of all heads, of one
     int64_t w0, w1;
     int ctas;  // CTAs that have a share
     int head, pair, skip;
@@ -135,7 +138,7 @@ __device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, 
     const int pairs = b.batch * a.tiles, chunk = (pairs + THREADS - 1) / THREADS;
     const int p0 = min(pairs, tid * chunk), p1 = min(pairs, p0 + chunk);
     int64_t mine = 0;
-    for (int p = p0; p < p1; ++p) mine += load_item(b, a, p, cta == 0).units;
+    for (int p = p0; p < p1; ++p) mine += load_item(b, a, p, cta == 0).cost;
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -163,7 +166,7 @@ __device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, 
         int64_t left = in_head - (upto - mine);
         int p = p0;
         for (; p < p1 - 1; ++p) {
-            const int u = load_item(b, a, p, false).units;
+            const int u = load_item(b, a, p, false).cost;
             if (left < u) break;
             left -= u;
         }
@@ -175,18 +178,54 @@ __device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, 
     pl.skip = found_skip;
     return pl;
 }
-// The CTA that holds unit w.
+// The CTA that holds place w of the whole.
 __device__ __forceinline__ int owner_of(const Place &pl, int64_t w) {
     return static_cast<int>(((w + 1) * pl.ctas - 1) / pl.total);
 }
 
-// A CTA's items that reach beyond it are partial: at most its first (slot 2 c)
-// and its last (slot 2 c + 1).  The CTA in which an item starts that others
-// continue names it in split[c], for the combine.
+// The CTA's share, item by item: of the item's units, first .. first + take - 1.
+struct Walk {
+    int64_t w, w1;
+    int head, pair, skip;  // skip: places of the current item before w
+    int first, take;
+    Item it;
+    // The current item, or the next one of which the CTA has a unit; false at the end of the share.
+    __device__ __forceinline__ bool settle(const Batch &b, const AttnShape &a) {
+        while (w < w1) {
+            it = load_item(b, a, pair, false);
+            const int64_t end = min(static_cast<int64_t>(it.cost), skip + (w1 - w));
+            first = max(0, skip - a.extra);
+            take = max(0, static_cast<int>(end) - a.extra) - first;
+            if (it.cost > 0 && take > 0) return true;
+            step(b, a);
+        }
+        return false;
+    }
+    __device__ __forceinline__ void step(const Batch &b, const AttnShape &a) {
+        w += it.cost > 0 ? it.cost - skip : 0;
+        skip = 0;
+        if (++pair == b.batch * a.tiles) pair = 0, ++head;
+    }
+    __device__ __forceinline__ bool start(const Batch &b, const AttnShape &a, const Place &pl) {
+        w = pl.w0, w1 = pl.w1, head = pl.head, pair = pl.pair, skip = pl.skip;
+        return settle(b, a);
+    }
+    __device__ __forceinline__ bool next(const Batch &b, const AttnShape &a) {
+        step(b, a);
+        return settle(b, a);
+    }
+    __device__ __forceinline__ bool whole() const { return take == it.units; }
+    // The item's units after this CTA's are others': the CTA of the last one.
+    __device__ __forceinline__ int last_cta(const Place &pl) const { return owner_of(pl, w - skip + it.cost - 1); }
+    // The partial answer's slot: a part with the item's first unit, or a later one; a CTA has one of each at most.
+    __device__ __forceinline__ int slot(int cta) const { return 2 * cta + (first == 0 ? 1 : 0); }
+};
+
+// Items of which several CTAs have a part: the CTA with the first unit names it
+// in split[c], for the combine; the others are the CTAs up to last_cta.
 struct Split {
-    int pair, head, nrows;     // nrows 0: no such item
-    int first_slot, last_cta;  // slot of its first part; the others are first parts of the CTAs up to last_cta
-    int pad[3];
+    int pair, head, nrows;  // nrows 0: no such item
+    int last_cta;
 };
 struct Partials {
     Split *split;  // [ctas]

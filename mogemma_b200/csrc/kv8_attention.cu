@@ -33,7 +33,7 @@ mg_status check_cache_batch(const char *who, const mg_kv8_cache *c, const mg_kv8
 Cache cache_of(const mg_kv8_cache *c);
 Batch batch_of(const mg_kv8_batch *b);
 // kv8_prompt.cu
-constexpr int kPromptUnit = 128;
+constexpr int kPromptUnit = 128, kPromptExtra = 3;
 int prompt_rows(int hd);
 cudaError_t launch_prompt(const AttnArgs &p, int hd, bool f16, int ctas, cudaStream_t s);
 
@@ -160,20 +160,14 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
     const int cta = blockIdx.x, ctas = gridDim.x;
     const Place pl = find_place<kThreads>(p.b, p.a, p.c.heads, cta, ctas);
     if (threadIdx.x == 0) p.part.split[cta].nrows = 0;
-    int64_t w = pl.w0;
-    int head = pl.head, pair = pl.pair, skip = pl.skip;
-    const int pairs = p.b.batch * p.a.tiles;
-    while (w < pl.w1) {
-        const Item it = load_item(p.b, p.a, pair, false);
-        if (it.units == 0 || it.nrows <= 0) {  // no rows in this tile
-            if (++pair == pairs) pair = 0, ++head;
-            continue;
-        }
-        const int take = static_cast<int>(min(static_cast<int64_t>(it.units - skip), pl.w1 - w));
-        const bool whole = take == it.units;
+    Walk wk;
+    for (bool more = wk.start(p.b, p.a, pl); more; more = wk.next(p.b, p.a)) {
+        const Item &it = wk.it;
+        const int head = wk.head, pair = wk.pair;
+        const bool whole = wk.whole();
         // this CTA's 16-token tiles of the item
-        const int ta = max((it.unit0 + skip) * (kUnit / 16), it.lo / 16);
-        const int tb = min((it.unit0 + skip + take) * (kUnit / 16), (it.hi + 15) / 16);
+        const int ta = max((it.unit0 + wk.first) * (kUnit / 16), it.lo / 16);
+        const int tb = min((it.unit0 + wk.first + wk.take) * (kUnit / 16), (it.hi + 15) / 16);
         const int si = pair / p.a.tiles;
         const int32_t *table = p.b.table + si * p.b.table_stride;
 
@@ -403,7 +397,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
             *reinterpret_cast<float2 *>(dst + HD + 4) = make_float2(o[i][1], o[i][3]);
         }
         __syncthreads();
-        const int slot = 2 * cta + (w == pl.w0 ? 0 : 1);
+        const int slot = wk.slot(cta);
         for (int x = threadIdx.x; x < it.nrows * (HD / 4); x += kThreads) {
             const int r = x / (HD / 4), d = 4 * (x % (HD / 4));
             float mm = -kInf, mmv = -kInf, ll = 0.f;
@@ -432,12 +426,9 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                 if (d == 0) *reinterpret_cast<float2 *>(p.part.ml + 2 * at) = make_float2(mm, ll);
             }
         }
-        if (threadIdx.x == 0 && skip == 0 && !whole)
-            p.part.split[cta] = Split{pair, head, it.nrows, slot, owner_of(pl, w + it.units - 1), {0, 0, 0}};
+        if (threadIdx.x == 0 && wk.first == 0 && !whole)
+            p.part.split[cta] = Split{pair, head, it.nrows, wk.last_cta(pl)};
         __syncthreads();
-        w += take;
-        skip = 0;
-        if (++pair == pairs) pair = 0, ++head;
     }
 }
 
@@ -515,7 +506,7 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
             const int i0 = few ? 0 : grp, step = few ? 1 : 16;
 #pragma unroll 4
             for (int i = i0; i < n; i += step) {
-                const int64_t at = static_cast<int64_t>(i == 0 ? sp.first_slot : 2 * (first + i)) * p.a.rows + r;
+                const int64_t at = static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r;
                 const float2 ml = *reinterpret_cast<const float2 *>(p.part.ml + 2 * at);
                 j.add(ml.x, ml.y, *reinterpret_cast<const float4 *>(p.part.o + at * hd + d));
             }
@@ -596,7 +587,7 @@ cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, int sms, cudaS
 }
 
 struct Plan {
-    int rows, unit, tiles, ctas, sms;
+    int rows, unit, extra, tiles, ctas, sms;
     size_t bytes;
 };
 // How a call runs: set by the cache's dimensions and the batch's bounds alone, so that the workspace's size is too.
@@ -608,6 +599,7 @@ cudaError_t plan_of(int hd, int group, int max_q, Plan *pl) {
     pl->sms = sms;
     pl->rows = prompt ? prompt_rows(hd) : kRows;
     pl->unit = prompt ? kPromptUnit : kUnit;
+    pl->extra = prompt ? kPromptExtra : 0;
     pl->ctas = prompt ? sms : sms * kRowsPerSm;
     pl->tiles = static_cast<int>((static_cast<int64_t>(max_q) * group + pl->rows - 1) / pl->rows);
     pl->bytes = partials_bytes(pl->ctas, pl->rows, hd);
@@ -682,7 +674,7 @@ extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_ba
     AttnArgs p;
     p.c = cache_of(cache);
     p.b = batch_of(batch);
-    p.a = AttnShape{group, pl.rows, pl.tiles, args->window, pl.unit};
+    p.a = AttnShape{group, pl.rows, pl.tiles, args->window, pl.unit, pl.extra};
     p.part = partials_at(args->workspace_dev, pl.ctas, pl.rows);
     p.q = args->q_dev, p.out = args->out_dev;
     p.q_row = args->q_row_stride, p.q_head = args->q_head_stride;

@@ -26,8 +26,9 @@
 //    stored in the 128-byte swizzled layout (token rows of 64 dims); tokens
 //    that no row sees become zeros, so that stale codes behind the context
 //    cannot reach a product;
-//  * warp 16: allocates TMEM and issues the MMAs;
-//  * warp 17: one lane walks the CTA's share of the schedule and hands the
+//  * warps 16 and 17: issue the MMAs, one warp per row tile (16 also allocates
+//    TMEM);
+//  * warp 18: one lane walks the CTA's share of the schedule and hands the
 //    items to the others through a ring in shared memory.
 //
 // Two row tiles have one S stage each and take turns: P V and the next S of one
@@ -161,7 +162,8 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
 }
 
 // Bounded wait.  err_dev may hold a bad page's code already, so a stop is announced in shared memory.
-__device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err) {
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err) {
+    if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t n = 1;; ++n) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -174,9 +176,6 @@ __device__ __noinline__ bool wait_long(uint64_t *bar, uint32_t parity, volatile 
             }
         }
     }
-}
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err) {
-    return mbar_try_wait(bar, parity) || wait_long(bar, parity, stop, err);
 }
 
 // Two floats in one register pair: the packed fp32 operations.
@@ -227,37 +226,6 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[N]) 
     }
 }
 
-// The CTA's share of the schedule, item by item.
-struct Walk {
-    int64_t w, w1;
-    int head, pair, skip, take;
-    bool first;
-    Item it;
-    // The current item, or the next one with rows; false at the end of the share.
-    __device__ __forceinline__ bool settle(const AttnArgs &p) {
-        const int pairs = p.b.batch * p.a.tiles;
-        while (w < w1) {
-            it = load_item(p.b, p.a, pair, false);
-            if (it.units > 0) {
-                take = static_cast<int>(min(static_cast<int64_t>(it.units - skip), w1 - w));
-                return true;
-            }
-            if (++pair == pairs) pair = 0, ++head;
-        }
-        return false;
-    }
-    __device__ __forceinline__ bool start(const AttnArgs &p, const Place &pl) {
-        w = pl.w0, w1 = pl.w1, head = pl.head, pair = pl.pair, skip = pl.skip, first = true;
-        return settle(p);
-    }
-    __device__ __forceinline__ bool next(const AttnArgs &p) {
-        w += take;
-        skip = 0;
-        first = false;
-        if (++pair == p.b.batch * p.a.tiles) pair = 0, ++head;
-        return settle(p);
-    }
-};
 // An item as the walker hands it out.
 struct Desc {
     int take;              // units of this CTA's share; 0: the share has ended
@@ -284,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [tile][S stage]
     __shared__ Desc items_s[kItems];
     __shared__ float sc_k[kRing][8], sc_v[kRing][8];  // scales of a unit's eight blocks: K, log2 of V
-    __shared__ int sc_ok[kRing][8];
+    __shared__ __align__(8) uint8_t sc_ok[kRing][8];
     __shared__ float q_down[C::kRows];
     __shared__ float2 xch[2][2][kM];  // one row tile: the two halves' maxima (by S stage)
     __shared__ uint32_t tmem_slot;
@@ -301,9 +269,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], 4);
-            mbar_init(&k_empty[i], 1);
+            mbar_init(&k_empty[i], kTiles);
             mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&v_empty[i], kTiles);
             mbar_init(&q_full[i], C::kTwo ? 4 : 8);
             for (int g = 0; g < 2; ++g) {
                 mbar_init(&s_full[g][i], 1);
@@ -314,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         for (int i = 0; i < kRing; ++i) mbar_init(&sc_full[i], 8);
         for (int i = 0; i < kItems; ++i) {
             mbar_init(&item_full[i], 1);
-            mbar_init(&item_empty[i], 17);  // 8 softmax warps, 8 loaders, the MMA issuer
+            mbar_init(&item_empty[i], 16 + kTiles);  // 8 softmax warps, 8 loaders, the MMA issuers
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&pair_bar[i][0], 2);
@@ -349,124 +317,89 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         return __all_sync(0xffffffffu, wait(bar, parity, stop, err));
     };
 
-    if (warp == 16) {  // ---- MMA issuer
+    if (warp >= 16 && warp < 16 + kTiles) {  // ---- MMA issuers: warp 16 + g has row tile g
         constexpr uint32_t kIdS = idesc_f16(kM, kN, 0), kIdO = idesc_f16(kM, HD, 1);
-        // descriptors count in 16 bytes; shared memory ends below their 2^14
-        const uint64_t qd = tc::sw128_desc(sq), kd = tc::sw128_desc(sk), vd = sw128_mn_desc(sv, kN * 128);
+        const int g = warp - 16;
         const uint32_t lead = lane == 0 ? 1u : 0u;
         auto commit = [&](uint64_t *bar) { commit_if(lead, bar); };
-        uint32_t n = 0;              // units so far
-        uint32_t acts[2] = {0, 0};   // a tile's items so far in which it sees something
-        uint32_t uses[2][2] = {{0, 0}, {0, 0}};  // [tile][S stage]: P V issued
+        // descriptors count in 16 bytes; shared memory ends below their 2^14
+        const uint64_t qd = tc::sw128_desc(sq + g * kM * 128), kd = tc::sw128_desc(sk), vd = sw128_mn_desc(sv, kN * 128);
+        const uint32_t t_o = tmem + g * HD, t_s = tmem + C::kS + kSS * g * kN;
+        uint32_t n = 0;     // units so far
+        uint32_t acts = 0;  // the tile's items so far in which it sees something
+        uint32_t uses = 0;  // bit st: parity of the tile's uses of S stage st
         bool ok = true;
         for (uint32_t i = 0; ok; ++i) {
             const Desc *d = warp_item(i);
             if (!d) break;
             const int take = d->take;
-            bool begun[2] = {false, false};
-            // S of tile g and the unit on K stage KS into S stage SS
-            auto s_of = [&](auto kstage, auto sstage, auto tile) {
-                constexpr uint32_t KS = decltype(kstage)::value, SS = decltype(sstage)::value, G = decltype(tile)::value;
-                const uint32_t t = tmem + C::kS + (kSS * G + SS) * kN;
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint64_t qa = qd + (((kk >> 2) * C::kRows * 128 + G * kM * 128 + (kk & 3) * 32) >> 4);
-                    const uint64_t kb = kd + ((KS * C::kTileBytes + (kk >> 2) * kN * 128 + (kk & 3) * 32) >> 4);
-                    if (kk == 0) umma_ss<kIdS, false>(lead, t, qa, kb);
-                    else umma_ss<kIdS, true>(lead, t, qa, kb);
-                }
-                commit(&s_full[G][SS]);
-            };
-            // P V of tile g: P in S stage SS, V stage VS
-            auto pv_of = [&](auto vstage, auto sstage, auto tile) -> bool {
-                constexpr uint32_t VS = decltype(vstage)::value, SS = decltype(sstage)::value, G = decltype(tile)::value;
-                if (!warp_wait(&p_full[G][SS], uses[G][SS]++ & 1u)) return false;
+            bool begun = false;
+            auto sees = [&](int j) { return d->sees(g, d->token(j)); };
+            // S of unit u, the item's j-th
+            auto s_of = [&](uint32_t u, int j) -> bool {
+                const uint32_t st = u % kSt, ss = u % kSS;
+                if (!warp_wait(&k_full[st], (u / kSt) & 1u)) return false;
                 tc::tc_fence_after();
-                const uint32_t o = tmem + G * HD, t = tmem + C::kS + (kSS * G + SS) * kN;
-                const uint64_t vb = vd + ((VS * C::kTileBytes) >> 4);
-                if (begun[G]) umma_ts<kIdO, true>(lead, o, t, vb);
-                else umma_ts<kIdO, false>(lead, o, t, vb);
-                begun[G] = true;
+                if (sees(j)) {
+                    const uint64_t kb = kd + ((st * C::kTileBytes) >> 4);
 #pragma unroll
-                for (int kk = 1; kk < kN / 16; ++kk) {
-                    // P's columns: 8 per step of 16 tokens; one row tile: the second half's behind column kN / 2
-                    const uint32_t col = C::kTwo || kk < 4 ? kk * 8 : kN / 2 + (kk - 4) * 8;
-                    umma_ts<kIdO, true>(lead, o, t + col, vb + ((kk * 2048) >> 4));
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint64_t a = qd + (((kk >> 2) * C::kRows * 128 + (kk & 3) * 32) >> 4);
+                        const uint64_t b = kb + (((kk >> 2) * kN * 128 + (kk & 3) * 32) >> 4);
+                        if (kk == 0) umma_ss<kIdS, false>(lead, t_s + ss * kN, a, b);
+                        else umma_ss<kIdS, true>(lead, t_s + ss * kN, a, b);
+                    }
+                    commit(&s_full[g][ss]);
                 }
-                commit(&pv_done[G][SS]);
+                commit(&k_empty[st]);
                 return true;
             };
-            using I0 = std::integral_constant<uint32_t, 0>;
-            using I1 = std::integral_constant<uint32_t, 1>;
-            auto sees = [&](int g, int j) { return j < take && d->sees(g, d->token(j)); };
+            // P V of unit n, the item's j-th
+            auto pv_of = [&](int j) -> bool {
+                const uint32_t st = n % kSt, ss = n % kSS;
+                if (!warp_wait(&v_full[st], (n / kSt) & 1u)) return false;
+                if (sees(j)) {
+                    if (!warp_wait(&p_full[g][ss], uses >> ss & 1u)) return false;
+                    uses ^= 1u << ss;
+                    tc::tc_fence_after();
+                    const uint32_t t = t_s + ss * kN;
+                    const uint64_t vb = vd + ((st * C::kTileBytes) >> 4);
+                    if (begun) umma_ts<kIdO, true>(lead, t_o, t, vb);
+                    else umma_ts<kIdO, false>(lead, t_o, t, vb);
+                    begun = true;
 #pragma unroll
-            for (int g = 0; g < kTiles; ++g)
-                if (d->sees(g, d->tok0, take)) ok = ok && warp_wait(&q_full[g], acts[g]++ & 1u);
-            if constexpr (C::kTwo) {
-                // K of unit u, the item's j-th, has landed
-                auto k_wait = [&](uint32_t u) -> bool {
-                    if (!warp_wait(&k_full[u & 1], (u >> 1) & 1u)) return false;
-                    tc::tc_fence_after();
-                    return true;
-                };
-                ok = ok && k_wait(n);
-                if (!ok) break;
-                auto first = [&](auto st) {
-                    if (sees(0, 0)) s_of(st, I0(), I0());
-                    if (sees(1, 0)) s_of(st, I0(), I1());
-                    commit(&k_empty[decltype(st)::value]);
-                };
-                if (n & 1) first(I1());
-                else first(I0());
-                // unit j: P V of a tile, then its next S
-                auto step = [&](auto st, auto nx, int j) -> bool {
-                    constexpr uint32_t ST = decltype(st)::value, NX = decltype(nx)::value;
-                    if (!warp_wait(&v_full[ST], (n >> 1) & 1u)) return false;
-                    if (sees(0, j) && !pv_of(st, I0(), I0())) return false;
-                    if (j + 1 < take && !k_wait(n + 1)) return false;
-                    if (sees(0, j + 1)) s_of(nx, I0(), I0());
-                    if (sees(1, j) && !pv_of(st, I0(), I1())) return false;
-                    commit(&v_empty[ST]);
-                    if (sees(1, j + 1)) s_of(nx, I0(), I1());
-                    if (j + 1 < take) commit(&k_empty[NX]);
-                    return true;
-                };
-                for (int j = 0; ok && j < take; ++j, ++n) ok = n & 1 ? step(I1(), I0(), j) : step(I0(), I1(), j);
-            } else {
-                auto s_unit = [&](auto ss, uint32_t u, int j) -> bool {
-                    if (!warp_wait(&k_full[0], u & 1u)) return false;
-                    tc::tc_fence_after();
-                    if (sees(0, j)) s_of(I0(), ss, I0());
-                    commit(&k_empty[0]);
-                    return true;
-                };
-                auto step = [&](auto ss, auto nx, int j) -> bool {
-                    if (j + 1 < take && !s_unit(nx, n + 1, j + 1)) return false;
-                    if (!warp_wait(&v_full[0], n & 1u)) return false;
-                    if (sees(0, j) && !pv_of(I0(), ss, I0())) return false;
-                    commit(&v_empty[0]);
-                    return true;
-                };
-                if (ok) ok = n & 1 ? s_unit(I1(), n, 0) : s_unit(I0(), n, 0);
-                for (int j = 0; ok && j < take; ++j, ++n) ok = n & 1 ? step(I1(), I0(), j) : step(I0(), I1(), j);
+                    for (int kk = 1; kk < kN / 16; ++kk) {
+                        // P's columns: 8 per step of 16 tokens; one row tile: the second half's behind column kN / 2
+                        const uint32_t col = C::kTwo || kk < 4 ? kk * 8 : kN / 2 + (kk - 4) * 8;
+                        umma_ts<kIdO, true>(lead, t_o, t + col, vb + ((kk * 2048) >> 4));
+                    }
+                    commit(&pv_done[g][ss]);
+                }
+                commit(&v_empty[st]);
+                return true;
+            };
+            if (d->sees(g, d->tok0, take)) ok = warp_wait(&q_full[g], acts++ & 1u);
+            ok = ok && s_of(n, 0);
+            for (int j = 0; ok && j < take; ++j, ++n) {
+                if constexpr (C::kTwo) ok = pv_of(j) && (j + 1 == take || s_of(n + 1, j + 1));
+                else ok = (j + 1 == take || s_of(n + 1, j + 1)) && pv_of(j);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&item_empty[i % kItems]);
         }
-    } else if (warp == 17) {  // ---- walker
+    } else if (warp == 18) {  // ---- walker
         if (lane == 0) {
             Walk wk;
             p.part.split[cta].nrows = 0;
-            bool more = wk.start(p, pl);
+            bool more = wk.start(p.b, p.a, pl);
             for (uint32_t i = 0;; ++i) {
                 if (i >= kItems && !wait(&item_empty[i % kItems], (i / kItems - 1) & 1u, stop, err)) break;
                 Desc &d = items_s[i % kItems];
                 d.take = more ? wk.take : 0;
                 if (more) {
                     const Item &it = wk.it;
-                    const bool whole = wk.take == it.units;
-                    const int slot = 2 * cta + (wk.first ? 0 : 1);
-                    d.tok0 = (it.unit0 + wk.skip) * kN;
+                    const bool whole = wk.whole();
+                    d.tok0 = (it.unit0 + wk.first) * kN;
                     d.lo = it.lo & ~(kBlock - 1);
                     d.hi = it.hi;
                     d.seq = wk.pair / p.a.tiles;
@@ -485,14 +418,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                             d.t_hi[g] = it.seq.pos0 + (it.row0 + g * kM + rows - 1) / p.a.group + 1;
                         }
                     }
-                    d.slot = whole ? -1 : slot;
-                    if (wk.skip == 0 && !whole)
-                        p.part.split[cta] =
-                            Split{wk.pair, wk.head, it.nrows, slot, owner_of(pl, wk.w + it.units - 1), {0, 0, 0}};
+                    d.slot = whole ? -1 : wk.slot(cta);
+                    if (wk.first == 0 && !whole) p.part.split[cta] = Split{wk.pair, wk.head, it.nrows, wk.last_cta(pl)};
                 }
                 mbar_arrive(&item_full[i % kItems]);
                 if (!more) break;
-                more = wk.next(p);
+                more = wk.next(p.b, p.a);
             }
         }
     } else if (warp >= 8 && warp < 16) {  // ---- loaders: K or V
@@ -509,8 +440,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         uint32_t i_at = 0;
         bool pg_on[2] = {false, false};
         const Desc *d = warp_item(0);
-        auto read_pages = [&]() {
-            if (!d) return;
+        auto read_pages = [&]() -> bool {  // false: the share has ended
+            if (!d) return false;
             pg_tok = d->tok0 + j * kHalf + quad;
             pg_head = d->head;
             const int32_t *table = p.b.table + d->seq * p.b.table_stride;
@@ -526,6 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                 if (lane == 0) mbar_arrive(&item_empty[i_at % kItems]);
                 d = warp_item(++i_at);
             }
+            return true;
         };
         uint4 r[C::kDepth][2][kAtoms];
         float sc[C::kDepth][2];
@@ -560,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                     const int blk = 4 * hh + (quad >> 4) + 2 * i;
                     if (is_k) {
                         sc_k[n % kRing][blk] = sc[b][i];
-                        sc_ok[n % kRing][blk] = ok_b[b][i];
+                        sc_ok[n % kRing][blk] = static_cast<uint8_t>(ok_b[b][i]);
                     } else {
                         sc_v[n % kRing][blk] = __log2f(sc[b][i]);
                     }
@@ -592,22 +524,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             }
             return true;
         };
-        const uint32_t halves = 2 * static_cast<uint32_t>(pl.w1 - pl.w0);
-        read_pages();
+        bool have = read_pages(), held[C::kDepth], ok = true;
 #pragma unroll
         for (int b = 0; b < C::kDepth; ++b) {
-            if (static_cast<uint32_t>(b) < halves) read_codes(b);
-            read_pages();
+            held[b] = have;
+            if (have) read_codes(b);
+            have = read_pages();
         }
-        bool ok = true;
-        for (uint32_t h0 = 0; ok && h0 < halves; h0 += C::kDepth) {
+        for (uint32_t h0 = 0; ok && held[0]; h0 += C::kDepth) {  // halves come in pairs: held[1] follows held[0]
 #pragma unroll
             for (int b = 0; b < C::kDepth; ++b) {
-                const uint32_t h = h0 + b;
-                if (!ok) continue;  // halves is a multiple of kDepth
-                ok = store(h, b);
-                if (ok && h + C::kDepth < halves) read_codes(b);
-                read_pages();
+                if (!ok) continue;
+                ok = store(h0 + b, b);
+                held[b] = have;
+                if (ok && have) read_codes(b);
+                have = read_pages();
             }
         }
     } else if (warp < 8) {  // ---- softmax
@@ -624,53 +555,64 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             const int t_rows = d->t_rows[tg], take = d->take;
             const bool active = d->sees(tg, d->tok0, take);
             if (active) {
-                // Q: a warp brings kQR rows, 8 at a time, 4 lanes to a row; a row's largest becomes 2^7 .. 2^8
+                // Q: a warp brings kQR rows, kBatch at a time, 4 lanes to a row; a row's largest becomes 2^7 .. 2^8
                 constexpr int kQR = C::kTwo ? 32 : 16, kCh = HD / 32;  // 16-byte chunks of a lane: 4 i + lane % 4
-                const int nrows = d->nrows;
+                constexpr int kB = kCh >= 8 ? 1 : 8 / kCh < kQR / 8 ? 8 / kCh : kQR / 8;  // rows of a lane: 32 registers
+                const int nrows = d->nrows, sub = lane & 3;
 #pragma unroll 1
-                for (int r0 = kQR * warp; r0 < kQR * (warp + 1) && r0 < nrows; r0 += 8) {
-                    const int lr = r0 + (lane >> 2), sub = lane & 3;  // row of the item
-                    const bool on = lr < nrows;
-                    const int row = d->row0 + (on ? lr : r0), tok = row / p.a.group;
-                    const T *src = static_cast<const T *>(p.q) + (static_cast<int64_t>(d->q0) + tok) * p.q_row +
-                                   (d->head * p.a.group + row - tok * p.a.group) * p.q_head + 8 * sub;
-                    uint4 q[kCh];
-                    uint32_t most = 0;
+                for (int r0 = kQR * warp; r0 < kQR * (warp + 1) && r0 < nrows; r0 += 8 * kB) {
+                    uint4 q[kB][kCh];
 #pragma unroll
-                    for (int i = 0; i < kCh; ++i) q[i] = *reinterpret_cast<const uint4 *>(src + 32 * i);
+                    for (int y = 0; y < kB; ++y) {
+                        const int lr = min(r0 + 8 * y + (lane >> 2), nrows - 1);  // row of the item
+                        const int row = d->row0 + lr, tok = row / p.a.group;
+                        const T *src = static_cast<const T *>(p.q) + (static_cast<int64_t>(d->q0) + tok) * p.q_row +
+                                       (d->head * p.a.group + row - tok * p.a.group) * p.q_head + 8 * sub;
 #pragma unroll
-                    for (int i = 0; i < kCh; ++i)
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const float2 f = two<T>((&q[i].x)[w]);
-                            most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
-                        }
-                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    const int e = static_cast<int>(most >> 23);
-                    float up = 1.0f, down = 1.0f;
-                    if (e >= 255) {  // a row with an infinity or NaN answers NaN
-                        down = __int_as_float(0x7fc00000);
-                    } else if (e > 0) {
-                        const int sh = min(134 - e, 126);
-                        up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
-                        down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
+                        for (int i = 0; i < kCh; ++i) q[y][i] = *reinterpret_cast<const uint4 *>(src + 32 * i);
                     }
-                    if (p.scale_log2 < 0.f) up = -up;  // factors of S stay positive
-                    if (on) {
-                        if (sub == 0) q_down[lr] = down;
+#pragma unroll
+                    for (int y = 0; y < kB; ++y) {
+                        const int lr = r0 + 8 * y + (lane >> 2);
+                        uint32_t most = 0;
 #pragma unroll
                         for (int i = 0; i < kCh; ++i) {
-                            uint4 hw;
+                            const uint32_t w[4] = {q[y][i].x, q[y][i].y, q[y][i].z, q[y][i].w};
 #pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                const float2 f = two<T>((&q[i].x)[w]);
-                                (&hw.x)[w] = pack(f.x * up, f.y * up, __half());
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 f = two<T>(w[e]);
+                                most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
                             }
-                            const int chunk = 4 * (i & 1) + sub;  // of atom i / 2
-                            *reinterpret_cast<uint4 *>(gen + (i >> 1) * C::kRows * 128 + lr * 128 +
-                                                       ((chunk ^ (lr & 7)) << 4)) = hw;
                         }
+                        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                        const int e = static_cast<int>(most >> 23);
+                        float up = 1.0f, down = 1.0f;
+                        if (e >= 255) {  // a row with an infinity or NaN answers NaN
+                            down = __int_as_float(0x7fc00000);
+                        } else if (e > 0) {
+                            const int sh = min(134 - e, 126);
+                            up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
+                            down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
+                        }
+                        if (p.scale_log2 < 0.f) up = -up;  // factors of S stay positive
+                        if (lr < nrows) {
+                            if (sub == 0) q_down[lr] = down;
+#pragma unroll
+                            for (int i = 0; i < kCh; ++i) {
+                                const uint32_t w[4] = {q[y][i].x, q[y][i].y, q[y][i].z, q[y][i].w};
+                                uint32_t h[4];
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+                                    const float2 f = two<T>(w[x]);
+                                    h[x] = pack(f.x * up, f.y * up, __half());
+                                }
+                                const int chunk = 4 * (i & 1) + sub;  // of atom i / 2
+                                *reinterpret_cast<uint4 *>(gen + (i >> 1) * C::kRows * 128 + lr * 128 +
+                                                           ((chunk ^ (lr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                            }
+                        }
+                        __syncwarp();
                     }
                 }
                 fence_proxy_async_smem();
@@ -698,22 +640,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                 if (any_rows) {
                     const uint32_t t_s = t_s0 + st * kN + col0;
                     const int tc0 = t0 + col0;
-                    bool blocks_ok = true;
-#pragma unroll
-                    for (int b = 0; b < kCols / 16; ++b) blocks_ok = blocks_ok && sc_ok[ring][col0 / 16 + b] != 0;
+                    const uint64_t flags = *reinterpret_cast<const uint64_t *>(sc_ok[ring]);
+                    const bool blocks_ok =
+                        C::kTwo ? flags == 0x0101010101010101ull : static_cast<uint32_t>(flags >> (4 * col0 / 8)) == 0x01010101u;
                     const bool full =
                         __all_sync(0xffffffffu, !row_on || (blocks_ok && lo <= tc0 && tc0 + kCols <= hi));
-                    // 32 columns: scores, or (partly seen units) the masked products with the factors folded in
-                    auto scores = [&](int x, float (&s)[32], float (&cf)[2]) {
+                    // 32 columns: scores and their factors; in partly seen units the masked products with factors of 1
+                    auto scores = [&](int x, float (&s)[32], float (&cf)[2], float (&lv)[2]) {
                         tmem_ld32_async(t_s + 32 * x, s);
-                        cf[0] = factor * sc_k[ring][col0 / 16 + 2 * x];
-                        cf[1] = factor * sc_k[ring][col0 / 16 + 2 * x + 1];
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            cf[b] = factor * sc_k[ring][col0 / 16 + 2 * x + b];
+                            lv[b] = sc_v[ring][col0 / 16 + 2 * x + b];
+                        }
                         tmem_ld_wait(s);
                         if (!full) {
+                            const int at = tc0 + 32 * x;
 #pragma unroll
                             for (int b = 0; b < 2; ++b) {
                                 const bool on = sc_ok[ring][col0 / 16 + 2 * x + b] != 0;
-                                const int at = tc0 + 32 * x;
 #pragma unroll
                                 for (int i = 16 * b; i < 16 * b + 16; ++i)
                                     s[i] = on && at + i >= lo && at + i < hi ? s[i] * cf[b] : -kInf;
@@ -721,11 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                             }
                         }
                     };
-                    float mn = -kInf, vn = -kInf;
-#pragma unroll 1
-                    for (int x = 0; x < kCols / 32; ++x) {
-                        float s[32], cf[2];
-                        scores(x, s, cf);
+                    // their maxima: of the scores, and with log2 of the value scales
+                    auto maxima = [&](const float (&s)[32], const float (&cf)[2], const float (&lv)[2], float &mn, float &vn) {
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
                             const float *y = s + 16 * b;
@@ -734,57 +676,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                             a0 = max3(a0, y[10], y[11]), a1 = max3(a1, y[12], y[13]);
                             const float t = fmaxf(max3(a0, y[14], y[15]), a1) * cf[b];
                             mn = fmaxf(mn, t);
-                            vn = fmaxf(vn, t + sc_v[ring][col0 / 16 + 2 * x + b]);
+                            vn = fmaxf(vn, t + lv[b]);
                         }
-                    }
-                    if constexpr (!C::kTwo) {  // the other half's columns
-                        xch[st][wg][r] = make_float2(mn, vn);
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&pair_bar[warp & 3][st]);
-                        ok = warp_wait(&pair_bar[warp & 3][st], ph);
-                        if (!ok) break;
-                        const float2 o = xch[st][wg ^ 1][r];
-                        mn = fmaxf(mn, o.x);
-                        vn = fmaxf(vn, o.y);
-                    }
-                    mn = fmaxf(mn, m);
-                    const float mb = finite_or_0(mn);
-                    l *= ex2(m - mb);
-                    m = mn;
-                    const bool move = vn > mref + kRescale || (mref == -kInf && vn > -kInf);
-                    const float old = mref;
-                    if (move) mref = vn;
-                    const float rb = finite_or_0(mref);
-                    if (begun && __any_sync(0xffffffffu, move)) {
-                        // O must hold P V of all this tile's units so far.  One S stage: S of this unit was issued
-                        // after them, so it does.
-                        if constexpr (!C::kTwo) {
-                            ok = warp_wait(&pv_done[tg][st ^ 1], (uses >> (st ^ 1) & 1u) ^ 1u);
-                            if (!ok) break;
-                            tc::tc_fence_after();
-                        }
-                        const float f = move ? ex2(old - rb) : 1.0f;
-                        constexpr int kOc = C::kTwo ? HD : HD / 2;
-#pragma unroll 1
-                        for (int x = 0; x < kOc; x += 32) {
-                            uint32_t o[32];
-                            const uint32_t at = t_o + (C::kTwo ? 0 : wg * kOc) + x;
-                            tc::tmem_ld32(at, o);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tc::tmem_st32(at, o);
-                        }
-                    }
-                    F2 sum = f2(0.f, 0.f);
-                    const F2 nm = f2(-mb, -mb);
-#pragma unroll 1
-                    for (int x = 0; x < kCols / 32; ++x) {
-                        float s[32], cf[2];
+                    };
+                    // P of 32 columns, and their sum
+                    auto weigh = [&](int x, const float (&s)[32], const float (&cf)[2], const float (&lv)[2]) {
+                        const float mb = finite_or_0(m), rb = finite_or_0(mref);
+                        const F2 nm = f2(-mb, -mb);
+                        F2 sum = f2(0.f, 0.f);
                         uint32_t pk[16];
-                        scores(x, s, cf);
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
-                            const float wv = ex2(fminf(sc_v[ring][col0 / 16 + 2 * x + b] + mb - rb, 126.f));
+                            const float wv = ex2(fminf(lv[b] + mb - rb, 126.f));
                             const F2 w2 = f2(wv, wv), c2 = f2(cf[b], cf[b]);
 #pragma unroll
                             for (int i = 16 * b; i < 16 * b + 16; i += 2) {
@@ -796,11 +699,90 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                                 pk[i / 2] = pack(e0, e1, __half());
                             }
                         }
+                        float s0, s1;
+                        un2(sum, s0, s1);
+                        l += s0 + s1;
                         tmem_st(t_s + 16 * x, pk);  // over columns that have been read
+                    };
+                    // m and mref move to mn and vn for the rows in which either grows by more than kRescale (P and the
+                    // terms of l stay below 2^8); what was formed with the old ones follows: l, O, and P of `done` chunks
+                    // of this unit.  O must hold P V of all this tile's units so far: with one S stage S of this unit was
+                    // issued after them.
+                    auto move_to = [&](float mn, float vn, int done) -> bool {
+                        const bool move = mn > m + kRescale || vn > mref + kRescale || (m == -kInf && mn > -kInf);
+                        if (!__any_sync(0xffffffffu, move)) return true;
+                        float fl = 1.0f, fo = 1.0f;
+                        if (move) {
+                            const float m2 = fmaxf(m, mn), r2 = fmaxf(mref, vn);
+                            fl = ex2(m - finite_or_0(m2));
+                            fo = ex2(mref - finite_or_0(r2));
+                            m = m2;
+                            mref = r2;
+                        }
+                        l *= fl;
+                        if (begun) {
+                            if constexpr (!C::kTwo) {
+                                if (!warp_wait(&pv_done[tg][st ^ 1], (uses >> (st ^ 1) & 1u) ^ 1u)) return false;
+                                tc::tc_fence_after();
+                            }
+                            constexpr int kOc = C::kTwo ? HD : HD / 2;
+#pragma unroll 1
+                            for (int x = 0; x < kOc; x += 32) {
+                                uint32_t o[32];
+                                const uint32_t at = t_o + (C::kTwo ? 0 : wg * kOc) + x;
+                                tc::tmem_ld32(at, o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fo);
+                                tc::tmem_st32(at, o);
+                            }
+                        }
+                        if constexpr (C::kTwo) {
+#pragma unroll 1
+                            for (int x = 0; x < done; x += 2) {  // 32 columns of P pairs: two chunks (the second may be S still)
+                                uint32_t o[32];
+                                tc::tmem_ld32(t_s + 16 * x, o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&o[i]));
+                                    if (i < 16 || x + 1 < done) o[i] = pack(f.x * fo, f.y * fo, __half());
+                                }
+                                tc::tmem_st32(t_s + 16 * x, o);
+                            }
+                        }
+                        return true;
+                    };
+                    if constexpr (C::kTwo) {  // one pass, chunk by chunk
+#pragma unroll 1
+                        for (int x = 0; x < kCols / 32; ++x) {
+                            float s[32], cf[2], lv[2], mn = -kInf, vn = -kInf;
+                            scores(x, s, cf, lv);
+                            maxima(s, cf, lv, mn, vn);
+                            ok = move_to(mn, vn, x);
+                            weigh(x, s, cf, lv);
+                        }
+                    } else {  // the maxima first: the other half's columns share O's scale
+                        float mn = -kInf, vn = -kInf;
+#pragma unroll 1
+                        for (int x = 0; x < kCols / 32; ++x) {
+                            float s[32], cf[2], lv[2];
+                            scores(x, s, cf, lv);
+                            maxima(s, cf, lv, mn, vn);
+                        }
+                        xch[st][wg][r] = make_float2(mn, vn);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&pair_bar[warp & 3][st]);
+                        ok = warp_wait(&pair_bar[warp & 3][st], ph);
+                        if (!ok) break;
+                        const float2 o = xch[st][wg ^ 1][r];
+                        ok = move_to(fmaxf(mn, o.x), fmaxf(vn, o.y), 0);
+                        if (!ok) break;
+#pragma unroll 1
+                        for (int x = 0; x < kCols / 32; ++x) {
+                            float s[32], cf[2], lv[2];
+                            scores(x, s, cf, lv);
+                            weigh(x, s, cf, lv);
+                        }
                     }
-                    float s0, s1;
-                    un2(sum, s0, s1);
-                    l += s0 + s1;
                 }
                 begun = true;
                 tc::tc_fence_before();
@@ -842,21 +824,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         tmem_ld32_async(t_o + x, o);
                         tmem_ld_wait(o);
                     }
-                    if (!row_on) continue;
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] *= f;
-                    if (whole) {
+                    if (row_on && whole) {
                         uint4 *d4 = reinterpret_cast<uint4 *>(dst + x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             d4[i] = make_uint4(pack(o[8 * i], o[8 * i + 1], T()), pack(o[8 * i + 2], o[8 * i + 3], T()),
                                                pack(o[8 * i + 4], o[8 * i + 5], T()), pack(o[8 * i + 6], o[8 * i + 7], T()));
-                    } else {
+                    } else if (row_on) {
                         float4 *d4 = reinterpret_cast<float4 *>(p.part.o + at * HD + x);
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             d4[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
+                    __syncwarp();  // the TMEM loads are warp-wide
                 }
             }
             tc::tc_fence_before();
