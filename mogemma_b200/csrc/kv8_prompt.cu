@@ -21,11 +21,12 @@
 //    64 g .. 64 g + 63 of every row, and the two threads of a row exchange their
 //    maxima.  They also bring the item's Q into shared memory and write the
 //    answers;
-//  * warps 8-11 load K, 12-15 V, by halves of 64 tokens: codes from the pages
-//    into registers one or two halves ahead (page ids one further), widened and
-//    stored in the 128-byte swizzled layout (token rows of 64 dims); tokens
-//    that no row sees become zeros, so that stale codes behind the context
-//    cannot reach a product;
+//  * warps 8-11 load K, 12-15 V: a unit's codes from the pages into registers
+//    one unit ahead (page ids two ahead), widened and stored in the 128-byte
+//    swizzled layout (token rows of 64 dims); tokens that no row sees become
+//    zeros, so that stale codes behind the context cannot reach a product.  The
+//    loads go out behind the fence that publishes the unit before: a fence waits
+//    for the loads in flight;
 //  * warps 16 and 17: issue the MMAs, one warp per row tile (16 also allocates
 //    TMEM);
 //  * warp 18: one lane walks the CTA's share of the schedule and hands the
@@ -58,11 +59,10 @@ namespace kv8 {
 namespace {
 constexpr int kM = 128;   // rows of a tile
 constexpr int kN = 128;   // tokens of a unit
-constexpr int kHalf = 64; // tokens that a loader moves at a time
 constexpr int kThreads = 640;
 constexpr uint32_t kErrWait = 0x90000u;
 constexpr float kInf = __builtin_huge_valf();
-constexpr float kRescale = 8.0f;
+constexpr float kRescale = 15.0f;  // P stays below 2^15, within fp16
 constexpr int kRing = 4;  // units whose scales are at hand
 
 template <int HD>
@@ -70,8 +70,9 @@ struct Cfg {
     static constexpr bool kTwo = HD <= 128;                 // two row tiles (O and S of both fit TMEM)
     static constexpr int kRows = kTwo ? 2 * kM : kM;        // rows of an item
     static constexpr int kCols = kTwo ? kN : kN / 2;        // score columns of a softmax thread
-    static constexpr int kAtoms = HD / 64;
-    static constexpr int kDepth = HD == 256 ? 1 : 2;        // halves of codes that a loader holds: 32 registers at most
+    // Registers per thread: the block is launched with 96 (5 warps on an SM sub-partition).  hd 256: a loader holds 64
+    // registers of codes; the issuing warpgroup gives up what it takes: 2 x 96 + 2 x 112 + 64 = 5 x 96.
+    static constexpr int kLoadRegs = HD == 256 ? 112 : 96, kIssueRegs = HD == 256 ? 64 : 96;
     static constexpr int kStages = kTwo ? 2 : 1;            // of K and of V
     static constexpr int kSStages = kTwo ? 1 : 2;           // of each tile's S
     static constexpr uint32_t kQBytes = kRows * HD * 2, kTileBytes = kN * HD * 2;
@@ -245,7 +246,7 @@ constexpr int kItems = 4;
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs p) {
     using C = Cfg<HD>;
-    constexpr int kAtoms = C::kAtoms, kTiles = C::kTwo ? 2 : 1, kCols = C::kCols, kSt = C::kStages, kSS = C::kSStages;
+    constexpr int kTiles = C::kTwo ? 2 : 1, kCols = C::kCols, kSt = C::kStages, kSS = C::kSStages;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[kRing], q_full[2], pair_bar[4][2], q_pair[4];
     __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems];
@@ -317,6 +318,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         return __all_sync(0xffffffffu, wait(bar, parity, stop, err));
     };
 
+    if constexpr (C::kIssueRegs != 96)
+        if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));
     if (warp >= 16 && warp < 16 + kTiles) {  // ---- MMA issuers: warp 16 + g has row tile g
         constexpr uint32_t kIdS = idesc_f16(kM, kN, 0), kIdO = idesc_f16(kM, HD, 1);
         const int g = warp - 16;
@@ -427,31 +430,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             }
         }
     } else if (warp >= 8 && warp < 16) {  // ---- loaders: K or V
+        if constexpr (C::kLoadRegs != 96) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kLoadRegs));
         const bool is_k = warp < 12;
-        const int u = (threadIdx.x - 256) & 127, quad = u >> 2, sub = u & 3;
-        const bool leader = sub == 0 && (quad & 15) == 0;  // holds the scales of a half's blocks quad / 16 and quad / 16 + 2
+        const int u = (threadIdx.x - 256) & 127, quad = u >> 2, sub = u & 3;  // tokens quad + 32 i, 16 bytes of each 64
+        const bool leader = sub == 0 && (quad & 15) == 0;  // holds the scales of blocks quad / 16 + 2 i
         const uint8_t *codes = (is_k ? p.c.k : p.c.v) + 16 * sub;
         const float *scales = is_k ? p.c.k_scale : p.c.v_scale;
         uint64_t *full = is_k ? k_full : v_full, *empty = is_k ? k_empty : v_empty;
         unsigned char *stage0 = gen + C::kQBytes + (is_k ? 0 : kSt * C::kTileBytes);
         const int slot_mask = (1 << p.c.page_shift) - 1;
-        // the half whose page ids are being read: the j-th of item i_at
-        int j = 0, pg[2], pg_tok = 0, pg_head = 0;
+        // the unit whose page ids are being read: the j-th of item i_at
+        int j = 0, pg[4] = {0, 0, 0, 0}, pg_tok = 0, pg_head = 0, pg_lo = 0, pg_hi = 0;
         uint32_t i_at = 0;
-        bool pg_on[2] = {false, false};
         const Desc *d = warp_item(0);
+        auto seen = [&](int i) { return pg_tok + 32 * i >= pg_lo && pg_tok + 32 * i < pg_hi; };
         auto read_pages = [&]() -> bool {  // false: the share has ended
             if (!d) return false;
-            pg_tok = d->tok0 + j * kHalf + quad;
+            pg_tok = d->token(j) + quad;
             pg_head = d->head;
+            pg_lo = d->lo;  // pages before a window may be gone
+            pg_hi = d->hi;
             const int32_t *table = p.b.table + d->seq * p.b.table_stride;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int tok = pg_tok + 32 * i;
-                pg_on[i] = tok >= d->lo && tok < d->hi;  // pages before a window may be gone
-                pg[i] = pg_on[i] ? table[tok >> p.c.page_shift] : 0;
-            }
-            if (++j == 2 * d->take) {
+            for (int i = 0; i < 4; ++i)
+                if (seen(i)) pg[i] = table[(pg_tok + 32 * i) >> p.c.page_shift];
+            if (++j == d->take) {
                 j = 0;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&item_empty[i_at % kItems]);
@@ -459,87 +462,76 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             }
             return true;
         };
-        uint4 r[C::kDepth][2][kAtoms];
-        float sc[C::kDepth][2];
-        int ok_b[C::kDepth][2];
-        auto read_codes = [&](int b) {
+        uint4 r[4][HD / 64];
+        float sc[4];
+        uint32_t ok_b = 0;  // bit i: block quad / 16 + 2 i is there
+        auto read_codes = [&]() {
+            ok_b = 0;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 4; ++i) {
                 const int page = pg[i], slot = (pg_tok + 32 * i) & slot_mask;
-                bool on = pg_on[i];
+                bool on = seen(i);
                 if (on && (page < 0 || page >= p.c.num_pages)) {
                     set_error(err, kErrPage);
                     on = false;
                 }
                 const uint8_t *src = codes + page * p.c.page_stride + pg_head * p.c.head_stride + slot * p.c.token_stride;
 #pragma unroll
-                for (int a = 0; a < kAtoms; ++a) r[b][i][a] = on ? ldg16(src + 64 * a) : make_uint4(0, 0, 0, 0);
-                if (leader) {
-                    const int64_t at =
-                        ((static_cast<int64_t>(page) * p.c.heads + pg_head) << (p.c.page_shift - 4)) + (slot >> 4);
-                    sc[b][i] = on ? scales[at] : 1.f;
-                    ok_b[b][i] = on ? 1 : 0;
+                for (int a = 0; a < HD / 64; ++a) r[i][a] = on ? ldg16(src + 64 * a) : make_uint4(0, 0, 0, 0);
+                sc[i] = 1.0f;
+                if (leader && on) {
+                    sc[i] = scales[((static_cast<int64_t>(page) * p.c.heads + pg_head) << (p.c.page_shift - 4)) + (slot >> 4)];
+                    ok_b |= 1u << i;
                 }
             }
         };
-        // the h-th half (unit h / 2) from buffer b; false when a wait ran out
-        auto store = [&](uint32_t h, int b) -> bool {
-            const uint32_t n = h >> 1, hh = h & 1, st = n % kSt;
-            if (hh == 0 && n >= kSt && !warp_wait(&empty[st], (n / kSt - 1) & 1u)) return false;
+        // unit n; false when a wait ran out
+        auto store = [&](uint32_t n) -> bool {
+            const uint32_t st = n % kSt;
+            if (n >= kSt && !warp_wait(&empty[st], (n / kSt - 1) & 1u)) return false;
             if (leader) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int blk = 4 * hh + (quad >> 4) + 2 * i;
+                for (int i = 0; i < 4; ++i) {
+                    const int blk = (quad >> 4) + 2 * i;
                     if (is_k) {
-                        sc_k[n % kRing][blk] = sc[b][i];
-                        sc_ok[n % kRing][blk] = static_cast<uint8_t>(ok_b[b][i]);
+                        sc_k[n % kRing][blk] = sc[i];
+                        sc_ok[n % kRing][blk] = static_cast<uint8_t>(ok_b >> i & 1u);
                     } else {
-                        sc_v[n % kRing][blk] = __log2f(sc[b][i]);
+                        sc_v[n % kRing][blk] = __log2f(sc[i]);
                     }
                 }
             }
-            unsigned char *tile = stage0 + st * C::kTileBytes;
+            unsigned char *row = stage0 + st * C::kTileBytes + quad * 128;  // token quad + 32 i: (quad + 32 i) & 7 = quad & 7
+            const int lo_at = ((2 * sub) ^ (quad & 7)) << 4, hi_at = ((2 * sub + 1) ^ (quad & 7)) << 4;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int row = kHalf * hh + quad + 32 * i;
+            for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int a = 0; a < kAtoms; ++a) {  // 16 codes -> two 16-byte chunks of the 128-byte row, swizzled
+                for (int a = 0; a < HD / 64; ++a) {  // 16 codes -> two 16-byte chunks of the 128-byte row, swizzled
                     uint4 lo, hi;
-                    e4m3x4_to_h2x2(r[b][i][a].x, lo.x, lo.y);
-                    e4m3x4_to_h2x2(r[b][i][a].y, lo.z, lo.w);
-                    e4m3x4_to_h2x2(r[b][i][a].z, hi.x, hi.y);
-                    e4m3x4_to_h2x2(r[b][i][a].w, hi.z, hi.w);
-                    unsigned char *dst = tile + a * kN * 128 + row * 128;
-                    *reinterpret_cast<uint4 *>(dst + (((2 * sub) ^ (row & 7)) << 4)) = lo;
-                    *reinterpret_cast<uint4 *>(dst + (((2 * sub + 1) ^ (row & 7)) << 4)) = hi;
+                    e4m3x4_to_h2x2(r[i][a].x, lo.x, lo.y);
+                    e4m3x4_to_h2x2(r[i][a].y, lo.z, lo.w);
+                    e4m3x4_to_h2x2(r[i][a].z, hi.x, hi.y);
+                    e4m3x4_to_h2x2(r[i][a].w, hi.z, hi.w);
+                    *reinterpret_cast<uint4 *>(row + a * kN * 128 + i * 32 * 128 + lo_at) = lo;
+                    *reinterpret_cast<uint4 *>(row + a * kN * 128 + i * 32 * 128 + hi_at) = hi;
                 }
             }
-            if (hh == 1) {
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sc_full[n % kRing]);
-                    mbar_arrive(&full[st]);
-                }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sc_full[n % kRing]);
+                mbar_arrive(&full[st]);
             }
             return true;
         };
-        bool have = read_pages(), held[C::kDepth], ok = true;
-#pragma unroll
-        for (int b = 0; b < C::kDepth; ++b) {
-            held[b] = have;
-            if (have) read_codes(b);
+        bool held = read_pages(), ok = true;
+        if (held) read_codes();
+        bool have = read_pages();
+        for (uint32_t n = 0; ok && held; ++n) {
+            ok = store(n);
+            held = have;
+            if (ok && have) read_codes();
             have = read_pages();
-        }
-        for (uint32_t h0 = 0; ok && held[0]; h0 += C::kDepth) {  // halves come in pairs: held[1] follows held[0]
-#pragma unroll
-            for (int b = 0; b < C::kDepth; ++b) {
-                if (!ok) continue;
-                ok = store(h0 + b, b);
-                held[b] = have;
-                if (ok && have) read_codes(b);
-                have = read_pages();
-            }
         }
     } else if (warp < 8) {  // ---- softmax
         const int wg = warp >> 2, tg = C::kTwo ? wg : 0, r = 32 * (warp & 3) + lane;  // tile and row of this thread
@@ -705,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         tmem_st(t_s + 16 * x, pk);  // over columns that have been read
                     };
                     // m and mref move to mn and vn for the rows in which either grows by more than kRescale (P and the
-                    // terms of l stay below 2^8); what was formed with the old ones follows: l, O, and P of `done` chunks
+                    // terms of l stay below 2^15); what was formed with the old ones follows: l, O, and P of `done` chunks
                     // of this unit.  O must hold P V of all this tile's units so far: with one S stage S of this unit was
                     // issued after them.
                     auto move_to = [&](float mn, float vn, int done) -> bool {
