@@ -70,9 +70,10 @@ struct Cfg {
     static constexpr bool kTwo = HD <= 128;                 // two row tiles (O and S of both fit TMEM)
     static constexpr int kRows = kTwo ? 2 * kM : kM;        // rows of an item
     static constexpr int kCols = kTwo ? kN : kN / 2;        // score columns of a softmax thread
-    // Registers per thread: the block is launched with 96 (5 warps on an SM sub-partition).  hd 256: a loader holds 64
-    // registers of codes; the issuing warpgroup gives up what it takes: 2 x 96 + 2 x 112 + 64 = 5 x 96.
-    static constexpr int kLoadRegs = HD == 256 ? 112 : 96, kIssueRegs = HD == 256 ? 64 : 96;
+    static constexpr int kChunk = kTwo ? 64 : 32;           // of which it holds so many at a time
+    // Registers per thread: the block is launched with 96 (5 warps on an SM sub-partition); the softmax holds kChunk
+    // scores, a loader 32 registers of codes (hd 256: 64).  2 softmax + 2 load + issue = 5 x 96.
+    static constexpr int kSoftmaxRegs = kTwo ? 120 : 96, kLoadRegs = kTwo ? 80 : 104, kIssueRegs = 80;
     static constexpr int kStages = kTwo ? 2 : 1;            // of K and of V
     static constexpr int kSStages = kTwo ? 1 : 2;           // of each tile's S
     static constexpr uint32_t kQBytes = kRows * HD * 2, kTileBytes = kN * HD * 2;
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems];
     __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [tile][S stage]
     __shared__ Desc items_s[kItems];
-    __shared__ float sc_k[kRing][8], sc_v[kRing][8];  // scales of a unit's eight blocks: K, log2 of V
+    __shared__ __align__(16) float sc_k[kRing][8], sc_v[kRing][8];  // scales of a unit's eight blocks: K, log2 of V
     __shared__ __align__(8) uint8_t sc_ok[kRing][8];
     __shared__ float q_down[C::kRows];
     __shared__ float2 xch[2][2][kM];  // one row tile: the two halves' maxima (by S stage)
@@ -318,8 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         return __all_sync(0xffffffffu, wait(bar, parity, stop, err));
     };
 
-    if constexpr (C::kIssueRegs != 96)
-        if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));
+    if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));
     if (warp >= 16 && warp < 16 + kTiles) {  // ---- MMA issuers: warp 16 + g has row tile g
         constexpr uint32_t kIdS = idesc_f16(kM, kN, 0), kIdO = idesc_f16(kM, HD, 1);
         const int g = warp - 16;
@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             }
         }
     } else if (warp >= 8 && warp < 16) {  // ---- loaders: K or V
-        if constexpr (C::kLoadRegs != 96) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kLoadRegs));
+        if constexpr (C::kLoadRegs < 96) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kLoadRegs));
+        if constexpr (C::kLoadRegs > 96) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kLoadRegs));
         const bool is_k = warp < 12;
         const int u = (threadIdx.x - 256) & 127, quad = u >> 2, sub = u & 3;  // tokens quad + 32 i, 16 bytes of each 64
         const bool leader = sub == 0 && (quad & 15) == 0;  // holds the scales of blocks quad / 16 + 2 i
@@ -534,6 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             have = read_pages();
         }
     } else if (warp < 8) {  // ---- softmax
+        if constexpr (C::kSoftmaxRegs > 96) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
         const int wg = warp >> 2, tg = C::kTwo ? wg : 0, r = 32 * (warp & 3) + lane;  // tile and row of this thread
         const int col0 = C::kTwo ? 0 : wg * kCols;
         const uint32_t lane_off = static_cast<uint32_t>(32 * (warp & 3)) << 16;
@@ -637,20 +639,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         C::kTwo ? flags == 0x0101010101010101ull : static_cast<uint32_t>(flags >> (4 * col0 / 8)) == 0x01010101u;
                     const bool full =
                         __all_sync(0xffffffffu, !row_on || (blocks_ok && lo <= tc0 && tc0 + kCols <= hi));
-                    // 32 columns: scores and their factors; in partly seen units the masked products with factors of 1
-                    auto scores = [&](int x, float (&s)[32], float (&cf)[2], float (&lv)[2]) {
-                        tmem_ld32_async(t_s + 32 * x, s);
+                    constexpr int kCh = C::kChunk, kB = kCh / 16;
+                    // kChunk columns: scores and their factors; in partly seen units the masked products with factors of 1
+                    auto scores = [&](int x, float (&s)[kCh], float (&cf)[kB], float (&lv)[kB]) {
+                        tmem_ld32_async(t_s + kCh * x, s);
+                        if constexpr (kCh == 64) tmem_ld32_async(t_s + kCh * x + 32, s + 32);
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            cf[b] = factor * sc_k[ring][col0 / 16 + 2 * x + b];
-                            lv[b] = sc_v[ring][col0 / 16 + 2 * x + b];
+                        for (int b = 0; b < kB; ++b) {
+                            cf[b] = factor * sc_k[ring][col0 / 16 + kB * x + b];
+                            lv[b] = sc_v[ring][col0 / 16 + kB * x + b];
                         }
                         tmem_ld_wait(s);
                         if (!full) {
-                            const int at = tc0 + 32 * x;
+                            const int at = tc0 + kCh * x;
 #pragma unroll
-                            for (int b = 0; b < 2; ++b) {
-                                const bool on = sc_ok[ring][col0 / 16 + 2 * x + b] != 0;
+                            for (int b = 0; b < kB; ++b) {
+                                const bool on = sc_ok[ring][col0 / 16 + kB * x + b] != 0;
 #pragma unroll
                                 for (int i = 16 * b; i < 16 * b + 16; ++i)
                                     s[i] = on && at + i >= lo && at + i < hi ? s[i] * cf[b] : -kInf;
@@ -659,9 +663,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         }
                     };
                     // their maxima: of the scores, and with log2 of the value scales
-                    auto maxima = [&](const float (&s)[32], const float (&cf)[2], const float (&lv)[2], float &mn, float &vn) {
+                    auto maxima = [&](const float (&s)[kCh], const float (&cf)[kB], const float (&lv)[kB], float &mn, float &vn) {
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
+                        for (int b = 0; b < kB; ++b) {
                             const float *y = s + 16 * b;
                             float a0 = max3(y[0], y[1], y[2]), a1 = max3(y[3], y[4], y[5]);
                             a0 = max3(a0, y[6], y[7]), a1 = max3(a1, y[8], y[9]);
@@ -671,30 +675,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                             vn = fmaxf(vn, t + lv[b]);
                         }
                     };
-                    // P of 32 columns, and their sum
-                    auto weigh = [&](int x, const float (&s)[32], const float (&cf)[2], const float (&lv)[2]) {
+                    // P of kChunk columns, and their sum
+                    auto weigh = [&](int x, const float (&s)[kCh], const float (&cf)[kB], const float (&lv)[kB]) {
                         const float mb = finite_or_0(m), rb = finite_or_0(mref);
                         const F2 nm = f2(-mb, -mb);
-                        F2 sum = f2(0.f, 0.f);
-                        uint32_t pk[16];
+                        F2 sum[kB];
+                        uint32_t pk[kCh / 2];
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
+                        for (int b = 0; b < kB; ++b) {
                             const float wv = ex2(fminf(lv[b] + mb - rb, 126.f));
                             const F2 w2 = f2(wv, wv), c2 = f2(cf[b], cf[b]);
+                            sum[b] = f2(0.f, 0.f);
 #pragma unroll
                             for (int i = 16 * b; i < 16 * b + 16; i += 2) {
                                 float e0, e1;
                                 un2(fma2(f2(s[i], s[i + 1]), c2, nm), e0, e1);
                                 const F2 e = f2(ex2(e0), ex2(e1));
-                                sum = add2(sum, e);
+                                sum[b] = add2(sum[b], e);
                                 un2(mul2(e, w2), e0, e1);
                                 pk[i / 2] = pack(e0, e1, __half());
                             }
                         }
                         float s0, s1;
-                        un2(sum, s0, s1);
+                        F2 all = add2(sum[0], sum[1]);
+                        if constexpr (kB == 4) all = add2(all, add2(sum[2], sum[3]));
+                        un2(all, s0, s1);
                         l += s0 + s1;
-                        tmem_st(t_s + 16 * x, pk);  // over columns that have been read
+                        tmem_st(t_s + kCh / 2 * x, pk);  // over columns that have been read
                     };
                     // m and mref move to mn and vn for the rows in which either grows by more than kRescale (P and the
                     // terms of l stay below 2^15); what was formed with the old ones follows: l, O, and P of `done` chunks
@@ -730,33 +737,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         }
                         if constexpr (C::kTwo) {
 #pragma unroll 1
-                            for (int x = 0; x < done; x += 2) {  // 32 columns of P pairs: two chunks (the second may be S still)
+                            for (int x = 0; x < done; ++x) {
                                 uint32_t o[32];
-                                tc::tmem_ld32(t_s + 16 * x, o);
+                                tc::tmem_ld32(t_s + 32 * x, o);
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
                                     const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&o[i]));
-                                    if (i < 16 || x + 1 < done) o[i] = pack(f.x * fo, f.y * fo, __half());
+                                    o[i] = pack(f.x * fo, f.y * fo, __half());
                                 }
-                                tc::tmem_st32(t_s + 16 * x, o);
+                                tc::tmem_st32(t_s + 32 * x, o);
                             }
                         }
                         return true;
                     };
                     if constexpr (C::kTwo) {  // one pass, chunk by chunk
 #pragma unroll 1
-                        for (int x = 0; x < kCols / 32; ++x) {
-                            float s[32], cf[2], lv[2], mn = -kInf, vn = -kInf;
+                        for (int x = 0; x < kCols / kCh; ++x) {
+                            float s[kCh], cf[kB], lv[kB], mn = -kInf, vn = -kInf;
                             scores(x, s, cf, lv);
                             maxima(s, cf, lv, mn, vn);
-                            ok = move_to(mn, vn, x);
+                            move_to(mn, vn, x);
                             weigh(x, s, cf, lv);
                         }
                     } else {  // the maxima first: the other half's columns share O's scale
                         float mn = -kInf, vn = -kInf;
 #pragma unroll 1
-                        for (int x = 0; x < kCols / 32; ++x) {
-                            float s[32], cf[2], lv[2];
+                        for (int x = 0; x < kCols / kCh; ++x) {
+                            float s[kCh], cf[kB], lv[kB];
                             scores(x, s, cf, lv);
                             maxima(s, cf, lv, mn, vn);
                         }
@@ -769,8 +776,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         ok = move_to(fmaxf(mn, o.x), fmaxf(vn, o.y), 0);
                         if (!ok) break;
 #pragma unroll 1
-                        for (int x = 0; x < kCols / 32; ++x) {
-                            float s[32], cf[2], lv[2];
+                        for (int x = 0; x < kCols / kCh; ++x) {
+                            float s[kCh], cf[kB], lv[kB];
                             scores(x, s, cf, lv);
                             weigh(x, s, cf, lv);
                         }
