@@ -4,11 +4,9 @@
 //
 // kv8_rows_kernel takes items of up to 8 query rows.  It is bound by reading
 // the cache: one code byte feeds 8 rows' products, so the legacy warp-level
-// MMA is fast enough and lets every byte go from global memory straight into
-// the registers it is multiplied from -- no shared-memory stage, no copy
-// engine, no layout to keep.  A warp takes 16 tokens (one scale block) at a
-// time and computes transposed products, tokens and head dims on the MMA's 16
-// rows, the query rows on its 8 columns:
+// MMA is fast enough.  A warp takes 16 tokens (one scale block) at a time and
+// computes transposed products, tokens and head dims on the MMA's 16 rows, the
+// query rows on its 8 columns:
 //   S^T[16 tokens][8 rows] = K . Q^T     A = K codes, widened to fp16 (exact)
 //   O^T[16 dims][8 rows]  += V^T . P^T   A = V codes of 4 tokens a lane,
 //                                        byte-interleaved, widened to fp16
@@ -16,6 +14,13 @@
 // agree, so a lane's K fragment is 16 consecutive bytes of a token's row, and
 // the m index any order of the output dims, so its V fragment is too.
 // S^T's accumulator layout transposes into P^T's operand layout by movmatrix.
+//
+// Every warp has a ring of its own in shared memory, filled by asynchronous
+// 16-byte copies kStages - 1 steps (8 KB each, hd 64: 4 KB) ahead, and nothing but its own
+// copies to wait for; token rows are padded by 16 bytes, so that the fragments'
+// loads meet no bank twice.  With the codes in registers instead, one step
+// ahead, 64 KB per SM at most were in flight: 4.3 TB/s where the ring reaches
+// RING_RATE.
 //
 // With s = scale log2(e) k_scale <q, k> the state per row is m = max s,
 // l = sum 2^(s - m) and the sum of P V with P = 2^(s + log2 v_scale - M),
@@ -44,18 +49,6 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kInf = __builtin_huge_valf();
 
-__device__ __forceinline__ uint4 ldg16(const uint8_t *p) {  // streamed: no reuse within an SM
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 ldg8(const uint8_t *p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
 // D += A . B, 16 x 8 x 16, fp16 operands, fp32 accumulators.
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -99,65 +92,49 @@ __device__ __forceinline__ float max_over_rows(float v) {  // over the 8 lanes t
 
 template <int HD>
 struct RowsCfg {
-    static constexpr int kTiles = 256 / HD;             // 16-token tiles of a warp's step: 4 KB of K, 4 KB of V
+    static constexpr int kTiles = HD == 256 ? 1 : 2;    // 16-token tiles of a warp's step
     static constexpr int kVB = HD / 8 < 16 ? HD / 8 : 16;  // V bytes per load: 8 (hd 64) or 16
     static constexpr int kVH = HD / (8 * kVB);          // loads along the head dims
     static constexpr int kM = HD / 16;                  // MMAs along the output dims
-    static constexpr size_t kSmem = sizeof(float) * kWarps * kRows * (HD + 4);
+    static constexpr int kRow = HD + 16;                // bytes of a token's padded row
+    static constexpr int kStep = 2 * kTiles * 16 * kRow;  // K rows, then V rows
+    static constexpr int kStages = HD == 64 ? 5 : 3;    // 100 to 110 KB for four warps: two CTAs per SM
+    static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kStages * kStep;
+    static_assert(sizeof(float) * kRows * (HD + 4) <= kStages * kStep, "the merge takes the place of a warp's ring");
 };
 
-// One tile's codes of a lane.  K: token lane / 4 and that + 8, bytes 64 c + 16 (lane % 4) .. + 15.
-template <int HD>
-struct KTile {
-    uint4 w[HD / 64][2];
-};
-// V: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (t = lane % 4), bytes kVB (8 h + lane / 4) .. of each.
-template <int HD>
-struct VTile {
-    uint32_t w[RowsCfg<HD>::kVH][4][RowsCfg<HD>::kVB / 4];
-};
-
-template <int HD>
-__device__ __forceinline__ void load_k(KTile<HD> &k, const uint8_t *tile, int64_t stride, int live, int lane) {
-    const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const bool on = g + 8 * r < live;
-        const uint8_t *row = tile + (g + 8 * r) * stride + 16 * t;
-#pragma unroll
-        for (int c = 0; c < HD / 64; ++c) k.w[c][r] = on ? ldg16(row + 64 * c) : make_uint4(0, 0, 0, 0);
-    }
+// 16 bytes to shared memory, asynchronously; zeros where !on.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src, bool on) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {  // all but the latest N groups have landed
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// A tile's 16 token rows (K or V) of which the first `live` are real.
 template <int HD>
-__device__ __forceinline__ void load_v(VTile<HD> &v, const uint8_t *tile, int64_t stride, int live, int lane) {
-    using Cfg = RowsCfg<HD>;
-    const int g = lane >> 2, t = lane & 3;
+__device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t *tile, int64_t stride, int live, int lane) {
+    constexpr int kChunks = HD / 16, kRowsAt = 32 / kChunks;  // 16-byte chunks of a row; rows per pass of the warp
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int tok = 2 * t + (r & 1) + 8 * (r >> 1);
-        const bool on = tok < live;
-        const uint8_t *row = tile + tok * stride + Cfg::kVB * g;
-#pragma unroll
-        for (int h = 0; h < Cfg::kVH; ++h) {
-            if constexpr (Cfg::kVB == 16) {
-                const uint4 w = on ? ldg16(row + 128 * h) : make_uint4(0, 0, 0, 0);
-                v.w[h][r][0] = w.x, v.w[h][r][1] = w.y, v.w[h][r][2] = w.z, v.w[h][r][3] = w.w;
-            } else {
-                const uint2 w = on ? ldg8(row + 64 * h) : make_uint2(0, 0);
-                v.w[h][r][0] = w.x, v.w[h][r][1] = w.y;
-            }
-        }
+    for (int r0 = 0; r0 < 16; r0 += kRowsAt) {
+        const int r = r0 + lane / kChunks, c = lane % kChunks;
+        const bool on = r < live;
+        copy16(dst + r * RowsCfg<HD>::kRow + 16 * c, on ? tile + r * stride + 16 * c : tile, on);
     }
 }
 
 template <int HD, typename T>
 __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
     using Cfg = RowsCfg<HD>;
-    extern __shared__ __align__(16) float sm[];  // merge: [warp][row][HD + 4]
+    extern __shared__ __align__(16) unsigned char smem[];  // rings by warp; at an item's end [row][HD + 4] floats each
     __shared__ float mlm[kWarps][kRows][3];
     asm volatile("griddepcontrol.launch_dependents;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int cta = blockIdx.x, ctas = gridDim.x;
+    unsigned char *ring = smem + warp * Cfg::kStages * Cfg::kStep;
+    const uint32_t ring_s = smem_u32(ring);
+    constexpr int kMerge = Cfg::kStages * Cfg::kStep / 4;  // floats from one warp's merge rows to the next's
     const Place pl = find_place<kThreads>(p.b, p.a, p.c.heads, cta, ctas);
     if (threadIdx.x == 0) p.part.split[cta].nrows = 0;
     Walk wk;
@@ -181,18 +158,20 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
             const int tok = on ? r / p.a.group : 0, h = head * p.a.group + (on ? r - tok * p.a.group : 0);
             const T *src = static_cast<const T *>(p.q) + (static_cast<int64_t>(it.seq.q0) + tok) * p.q_row +
                            h * p.q_head + 16 * t;
-            uint4 raw[HD / 64][2];
+            uint32_t raw[HD / 64][8];
             uint32_t most = 0;
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    raw[c][i] = on ? reinterpret_cast<const uint4 *>(src + 64 * c)[i] : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 v = on ? reinterpret_cast<const uint4 *>(src + 64 * c)[i] : make_uint4(0, 0, 0, 0);
+                    raw[c][4 * i] = v.x, raw[c][4 * i + 1] = v.y, raw[c][4 * i + 2] = v.z, raw[c][4 * i + 3] = v.w;
+                }
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float2 f = two<T>((&raw[c][0].x)[i]);
+                    const float2 f = two<T>(raw[c][i]);
                     most = max(most, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
                 }
 #pragma unroll
@@ -212,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
             for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float2 f = two<T>((&raw[c][0].x)[i]);
+                    const float2 f = two<T>(raw[c][i]);
                     qf[c][i >> 1][i & 1] = pack_h2(f.x * up, f.y * up);
                 }
             // columns 2 t, 2 t + 1 of the accumulators are rows held by lanes 8 t, 8 t + 4
@@ -256,61 +235,66 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                 }
             }
         };
-        KTile<HD> kt[Cfg::kTiles];
-        VTile<HD> vt[Cfg::kTiles];
-        int64_t kp[Cfg::kTiles], vp[Cfg::kTiles];
-        float kss[Cfg::kTiles], lvss[Cfg::kTiles];
         const int steps = (tb - ta + kWarps * Cfg::kTiles - 1) / (kWarps * Cfg::kTiles);
-        auto live_of = [&](int n, int64_t at) { return at < 0 ? 0 : it.hi - tile_at(n) * 16; };
-        auto fetch_k = [&](int n0) {
+        // step n's copies, and its tiles' scales (K; log2 of V) for later: they are shuffled out of the lanes' look-up
+        // window before it moves on
+        float ks_at[Cfg::kStages][Cfg::kTiles], lv_at[Cfg::kStages][Cfg::kTiles];
+        uint32_t there = 0;  // bit kTiles * stage + i: the tile has a place
+        auto fetch = [&](int step, int stage) {
+            if (step < steps) {
+                const int n0 = step * Cfg::kTiles;
+                if ((n0 & 31) == 0) look_up(n0);
 #pragma unroll
-            for (int i = 0; i < Cfg::kTiles; ++i) {
-                kp[i] = __shfl_sync(0xffffffffu, place, (n0 + i) & 31);
-                kss[i] = __shfl_sync(0xffffffffu, ks, (n0 + i) & 31);
-                lvss[i] = __shfl_sync(0xffffffffu, lvs, (n0 + i) & 31);
-                load_k<HD>(kt[i], p.c.k + kp[i], p.c.token_stride, live_of(n0 + i, kp[i]), lane);
+                for (int i = 0; i < Cfg::kTiles; ++i) {
+                    const int64_t at = __shfl_sync(0xffffffffu, place, (n0 + i) & 31);
+                    ks_at[stage][i] = __shfl_sync(0xffffffffu, ks, (n0 + i) & 31);
+                    lv_at[stage][i] = __shfl_sync(0xffffffffu, lvs, (n0 + i) & 31);
+                    const uint32_t bit = 1u << (Cfg::kTiles * stage + i);
+                    there = at >= 0 ? there | bit : there & ~bit;
+                    const int live = at < 0 ? 0 : it.hi - tile_at(n0 + i) * 16;
+                    const int64_t src = at < 0 ? 0 : at;
+                    const uint32_t dst = ring_s + stage * Cfg::kStep + i * 16 * Cfg::kRow;
+                    copy_tile<HD>(dst, p.c.k + src, p.c.token_stride, live, lane);
+                    copy_tile<HD>(dst + Cfg::kTiles * 16 * Cfg::kRow, p.c.v + src, p.c.token_stride, live, lane);
+                }
             }
+            copies_commit();  // an empty group past the end: the count of groups stays that of steps
         };
-        auto fetch_v = [&](int n0) {
 #pragma unroll
-            for (int i = 0; i < Cfg::kTiles; ++i)
-                load_v<HD>(vt[i], p.c.v + vp[i], p.c.token_stride, live_of(n0 + i, vp[i]), lane);
-        };
-        if (steps > 0) {
-            look_up(0);
-            fetch_k(0);
-#pragma unroll
-            for (int i = 0; i < Cfg::kTiles; ++i) vp[i] = kp[i];
-            fetch_v(0);
-        }
-        for (int step = 0; step < steps; ++step) {
+        for (int i = 0; i < Cfg::kStages - 1; ++i) fetch(i, i);
+        auto work = [&](int step, int stage) {
             const int n0 = step * Cfg::kTiles;
+            copies_wait<Cfg::kStages - 1>();
+            __syncwarp();
+            const unsigned char *kt = ring + stage * Cfg::kStep, *vt = kt + Cfg::kTiles * 16 * Cfg::kRow;
             // S^T
             float s[Cfg::kTiles][4];
 #pragma unroll
             for (int i = 0; i < Cfg::kTiles; ++i) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+                // lane's K: tokens g and g + 8, bytes 64 c + 16 t .. + 15
+                const unsigned char *row = kt + (16 * i + g) * Cfg::kRow + 16 * t;
 #pragma unroll
-                for (int c = 0; c < HD / 64; ++c)
+                for (int c = 0; c < HD / 64; ++c) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(row + 64 * c);
+                    const uint4 y = *reinterpret_cast<const uint4 *>(row + 8 * Cfg::kRow + 64 * c);
+                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t a0, a1, a2, a3;
-                        e4m3x4_to_h2x2((&kt[i].w[c][0].x)[j], a0, a2);
-                        e4m3x4_to_h2x2((&kt[i].w[c][1].x)[j], a1, a3);
+                        e4m3x4_to_h2x2(xw[j], a0, a2);
+                        e4m3x4_to_h2x2(yw[j], a1, a3);
                         mma16816(s[i], a0, a1, a2, a3, qf[c][j][0], qf[c][j][1]);
                     }
+                }
             }
-            // masked, scaled scores; the next step's K loads go out once these registers are free
+            // masked, scaled scores
             float sk[Cfg::kTiles], lv[Cfg::kTiles];
             bool seen[Cfg::kTiles];
 #pragma unroll
-            for (int i = 0; i < Cfg::kTiles; ++i) sk[i] = kss[i], lv[i] = lvss[i], seen[i] = kp[i] >= 0;
-            const bool more = step + 1 < steps;
-            if (more) {
-                if (((n0 + Cfg::kTiles) & 31) == 0) look_up(n0 + Cfg::kTiles);
-                fetch_k(n0 + Cfg::kTiles);
-            }
+            for (int i = 0; i < Cfg::kTiles; ++i)
+                sk[i] = ks_at[stage][i], lv[i] = lv_at[stage][i], seen[i] = there >> (Cfg::kTiles * stage + i) & 1u;
             float top[2] = {-kInf, -kInf}, topv[2] = {-kInf, -kInf};
 #pragma unroll
             for (int i = 0; i < Cfg::kTiles; ++i) {
@@ -352,30 +336,48 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                     pr[e] = ex2(s[i][e] + lv[i] - basev[e & 1]);
                 }
                 const uint32_t b0 = transpose8x8(pack_h2(pr[0], pr[1])), b1 = transpose8x8(pack_h2(pr[2], pr[3]));
+                // lane's V: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9, bytes kVB (8 h + g) .. of each
+                const unsigned char *row = vt + (16 * i + 2 * t) * Cfg::kRow + Cfg::kVB * g;
 #pragma unroll
-                for (int h = 0; h < Cfg::kVH; ++h)
+                for (int h = 0; h < Cfg::kVH; ++h) {
+                    uint32_t w[4][Cfg::kVB / 4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const unsigned char *at = row + ((r & 1) + 8 * (r >> 1)) * Cfg::kRow + 8 * Cfg::kVB * h;
+                        if constexpr (Cfg::kVB == 16) {
+                            const uint4 x = *reinterpret_cast<const uint4 *>(at);
+                            w[r][0] = x.x, w[r][1] = x.y, w[r][2] = x.z, w[r][3] = x.w;
+                        } else {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(at);
+                            w[r][0] = x.x, w[r][1] = x.y;
+                        }
+                    }
 #pragma unroll
                     for (int j = 0; j < Cfg::kVB / 4; ++j) {
                         // tokens 2 t and 2 t + 1 (then + 8) of dims 4 j .. 4 j + 3, interleaved
-                        const uint32_t x0 = vt[i].w[h][0][j], x1 = vt[i].w[h][1][j];
-                        const uint32_t y0 = vt[i].w[h][2][j], y1 = vt[i].w[h][3][j];
                         uint32_t a[4], b[4];
-                        e4m3x4_to_h2x2(__byte_perm(x0, x1, 0x5140), a[0], a[1]);
-                        e4m3x4_to_h2x2(__byte_perm(x0, x1, 0x7362), a[2], a[3]);
-                        e4m3x4_to_h2x2(__byte_perm(y0, y1, 0x5140), b[0], b[1]);
-                        e4m3x4_to_h2x2(__byte_perm(y0, y1, 0x7362), b[2], b[3]);
+                        e4m3x4_to_h2x2(__byte_perm(w[0][j], w[1][j], 0x5140), a[0], a[1]);
+                        e4m3x4_to_h2x2(__byte_perm(w[0][j], w[1][j], 0x7362), a[2], a[3]);
+                        e4m3x4_to_h2x2(__byte_perm(w[2][j], w[3][j], 0x5140), b[0], b[1]);
+                        e4m3x4_to_h2x2(__byte_perm(w[2][j], w[3][j], 0x7362), b[2], b[3]);
                         float(&d0)[4] = o[h * (Cfg::kVB / 2) + 2 * j];
                         float(&d1)[4] = o[h * (Cfg::kVB / 2) + 2 * j + 1];
                         mma16816(d0, a[0], a[1], b[0], b[1], b0, b1);
                         mma16816(d1, a[2], a[3], b[2], b[3], b0, b1);
                     }
+                }
             }
-            if (more) {
+            __syncwarp();  // the stage has been read
+        };
+        for (int step0 = 0; step0 < steps; step0 += Cfg::kStages) {
 #pragma unroll
-                for (int i = 0; i < Cfg::kTiles; ++i) vp[i] = kp[i];
-                fetch_v(n0 + Cfg::kTiles);
+            for (int st = 0; st < Cfg::kStages; ++st) {
+                if (step0 + st >= steps) continue;
+                fetch(step0 + st + Cfg::kStages - 1, (st + Cfg::kStages - 1) % Cfg::kStages);
+                work(step0 + st, st);
             }
         }
+        copies_wait<0>();
 
         // ---- merge the warps
 #pragma unroll
@@ -392,7 +394,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
 #pragma unroll
         for (int i = 0; i < Cfg::kM; ++i) {
             const int h = i / (Cfg::kVB / 2), j = i % (Cfg::kVB / 2);
-            float *dst = sm + (warp * kRows + 2 * t) * (HD + 4) + Cfg::kVB * (8 * h + g) + 2 * j;
+            float *dst = reinterpret_cast<float *>(ring) + 2 * t * (HD + 4) + Cfg::kVB * (8 * h + g) + 2 * j;
             *reinterpret_cast<float2 *>(dst) = make_float2(o[i][0], o[i][2]);
             *reinterpret_cast<float2 *>(dst + HD + 4) = make_float2(o[i][1], o[i][3]);
         }
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
             for (int i = 0; i < kWarps; ++i) {
                 ll += mlm[i][r][1] * ex2(mlm[i][r][0] - b);
                 const float f = ex2(mlm[i][r][2] - bv);
-                const float4 v = *reinterpret_cast<const float4 *>(sm + (i * kRows + r) * (HD + 4) + d);
+                const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem) + i * kMerge + r * (HD + 4) + d);
                 acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
             }
             // O is in units of 2^M, l in units of 2^m; a row that saw nothing has l = 0
