@@ -53,6 +53,27 @@ __device__ __forceinline__ Seq load_seq(const Batch &b, int i, bool report) {
     return s;
 }
 
+// ---- launches.  A kernel is launched so that it may be set up while its
+// predecessor on the stream ends (programmatic dependent launch), and waits for
+// the predecessor's results itself, before its first access to memory.  No
+// kernel lets its successor begin before it ends: a combine whose blocks came
+// early cost the attention 1 to 2 us.
+__device__ __forceinline__ void kernel_begins() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ---- e4m3 <-> wider.  Codes convert to fp16 exactly (448 and 2^-9 are both in its range).
 __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t two) {
     uint32_t r;

@@ -2,25 +2,31 @@
 // cache, with the head norm and the position rotation on the way (the QK-norm,
 // RoPE and cache write of layers.mojo:43-61), and the rotated queries.
 //
-// One CTA owns one block of 16 positions of one sequence and kv head: the
-// block's scale is a maximum over its tokens, so the tokens of the call that
-// fall into it, its earlier codes and its scale all belong to one CTA, and the
-// q heads of the same tokens and kv head go along (they share the cos / sin
-// rows).  A head vector is held by head_dim / 8 lanes, lane i with elements
-// 4 i .. 4 i + 3 of each half, so that a rotation's pairs meet in one lane and
-// loads are 4 elements wide.
+// A block's scale is a maximum over its tokens, so the tokens of a call that
+// fall into one block of 16 positions of a sequence and kv head, the block's
+// earlier codes and its scale all belong to one owner, and the q heads of the
+// same tokens and kv head go along (they share the cos / sin rows).  A head
+// vector is held by head_dim / 8 lanes (a group), lane i with elements 4 i ..
+// 4 i + 3 of each half, so that a rotation's pairs meet in one lane and loads
+// are 4 elements wide.  Two forms:
+//  * max_q 1 (a decode step): the owner is a group; nothing crosses groups;
+//  * otherwise the owner is a CTA of 16 groups, one per token of the block.
 //
 // The work is memory traffic: the rows in, the rotated queries and one byte
-// per value out; per element a norm and a rotation are a few operations.
+// per value out; per element a norm and a rotation are a few operations.  What
+// it costs is latency, so a token's K, V, q heads, cos and sin rows are all
+// loaded before the first is used, and the page id and old scales, which only
+// the stores need, are not waited for earlier.
 #include "kv8.cuh"
 
 #include <cstdio>
+#include <type_traits>
 
 namespace mg {
 namespace kv8 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kTokenThreads = 128;  // CTA of the one-token form
 
 struct AppendParams {
     Cache c;
@@ -30,28 +36,24 @@ struct AppendParams {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
     const float *q_norm, *k_norm, *cos_t, *sin_t;
     int group;            // q heads per kv head (0: no queries)
-    int blocks_per_seq;   // > 0: block index = sequence * this + block; 0: by rows, seq_of_block
+    int blocks_per_seq;   // block form: > 0: block index = sequence * this + block; 0: by rows, seq_of_block
 };
 
+// Four elements as they lie in memory, and as floats.
 template <typename T>
-__device__ __forceinline__ void load4(const T *p, float (&x)[4]);
-template <>
-__device__ __forceinline__ void load4<float>(const float *p, float (&x)[4]) {
-    const float4 v = *reinterpret_cast<const float4 *>(p);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-}
-template <>
-__device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16 *p, float (&x)[4]) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
-    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
-}
-template <>
-__device__ __forceinline__ void load4<__half>(const __half *p, float (&x)[4]) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
-    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+using Raw = typename std::conditional<sizeof(T) == 4, float4, uint2>::type;
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T> &v, float *x) {
+    if constexpr (std::is_same<T, float>::value) {
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
+        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    } else {
+        x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+        x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
 }
 __device__ __forceinline__ void store4(float *p, const float *x) {
     *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
@@ -69,47 +71,228 @@ __device__ __forceinline__ void store4(__half *p, const float *x) {
 
 // A head vector's 8 elements of this lane: 0-3 from the first half, 4-7 from the second.
 template <int HD, typename T>
-__device__ __forceinline__ void load_vec(const T *p, int gl, float (&x)[8]) {
-    float a[4], b[4];
-    load4<T>(p + 4 * gl, a);
-    load4<T>(p + HD / 2 + 4 * gl, b);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-}
-// x <- rope(norm(x)) at position pos.
+struct Vec {
+    Raw<T> a, b;
+    __device__ __forceinline__ void load(const T *p, int gl) {
+        a = *reinterpret_cast<const Raw<T> *>(p + 4 * gl);
+        b = *reinterpret_cast<const Raw<T> *>(p + HD / 2 + 4 * gl);
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+        widen<T>(a, x);
+        widen<T>(b, x + 4);
+    }
+};
 template <int HD>
-__device__ __forceinline__ void turn(float (&x)[8], int gl, const float *w, const float *cos_t, const float *sin_t,
-                                     int pos) {
-    constexpr int kLanes = HD / 8;
-    if (w) {
-        float ss = 0.f;
+__device__ __forceinline__ void load_weights(const float *w, int gl, float (&x)[8]) {
+    Vec<HD, float> v;
+    v.load(w, gl);
+    v.floats(x);
+}
+__device__ __forceinline__ void rotate(float (&x)[8], const float4 &c, const float4 &s) {
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rms_inv(ss, 1.0f / HD);
-        float nw[8];
-        load_vec<HD, float>(w, gl, nw);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * (1.0f + nw[i]);
+    for (int i = 0; i < 4; ++i) {
+        const float a = x[i], b = x[4 + i];
+        x[i] = a * cc[i] - b * ss[i];
+        x[4 + i] = b * cc[i] + a * ss[i];
     }
-    if (cos_t) {
-        float c[4], s[4];
-        load4<float>(cos_t + static_cast<int64_t>(pos) * (HD / 2) + 4 * gl, c);
-        load4<float>(sin_t + static_cast<int64_t>(pos) * (HD / 2) + 4 * gl, s);
+}
+template <int HD>
+__device__ __forceinline__ void norm(float (&x)[8], const float (&w)[8]) {
+    float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = x[i], b = x[4 + i];
-            x[i] = a * c[i] - b * s[i];
-            x[4 + i] = b * c[i] + a * s[i];
-        }
-    }
+    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+#pragma unroll
+    for (int o = HD / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rms_inv(ss, 1.0f / HD);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * (1.0f + w[i]);
+}
+// The same for a key, whose values are about to be rounded to 4 bits: the sum and the factor in 64 bits, so that what
+// is left of its error (four roundings to 32 bits) moves hardly more values across a border than one rounding would.
+template <int HD>
+__device__ __forceinline__ void norm_key(float (&x)[8], const float (&w)[8]) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += static_cast<double>(x[i]) * static_cast<double>(x[i]);
+#pragma unroll
+    for (int o = HD / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const double m = ss * (1.0 / HD) + 1e-6;
+    double inv = static_cast<double>(rsqrtf(static_cast<float>(m)));
+    inv = inv * (1.5 - 0.5 * m * inv * inv);  // one Newton step from 2^-22 to 2^-44
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= static_cast<float>(inv * (1.0 + static_cast<double>(w[i])));
+}
+// The largest magnitude of a group's vector, as bits: finite < infinity < NaN.
+template <int HD>
+__device__ __forceinline__ uint32_t most_of(const float (&x)[8]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = HD / 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    return most;
+}
+// Eight codes of the lane at a token's row; `fill`: instead of them.
+template <int HD>
+__device__ __forceinline__ void store_codes(uint8_t *row, int gl, const float (&x)[8], float inv, bool bad, uint32_t fill) {
+    const uint32_t a = to_e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    const uint32_t b = to_e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+    reinterpret_cast<uint32_t *>(row)[gl] = bad ? fill : a;
+    reinterpret_cast<uint32_t *>(row + HD / 2)[gl] = bad ? fill : b;
+}
+// Four codes under a scale that grew: ratio = old / new.
+__device__ __forceinline__ uint32_t requantise(uint32_t four, float ratio) {
+    uint32_t a, b;
+    e4m3x4_to_h2x2(four, a, b);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a));
+    const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+    return to_e4m3x4(f.x * ratio, f.y * ratio, g.x * ratio, g.y * ratio);
 }
 // The exponent of the smallest power of two s >= 2^-100 with amax <= 448 s, for finite amax >= 0 (as bits):
 // 448 = 1.75 * 2^8.
 __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
     const int e = static_cast<int>(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     return max(e, -100);
+}
+__device__ __forceinline__ float scale_of(uint32_t amax_bits) {
+    return __uint_as_float(static_cast<uint32_t>(scale_exponent(amax_bits) + 127) << 23);
+}
+constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr uint32_t kBadKey = 0x7f7f7f7fu;  // four e4m3 NaNs: the key of a token with a non-finite key or value
+
+// Where a block lies: byte offset of its first token, index of its scales.
+struct Spot {
+    int64_t at, scale;
+};
+__device__ __forceinline__ Spot spot_of(const Cache &c, int page, int kvh, int first) {
+    const int slot = first & ((1 << c.page_shift) - 1);
+    return Spot{page * c.page_stride + kvh * c.head_stride + slot * c.token_stride,
+                 ((static_cast<int64_t>(page) * c.heads + kvh) << (c.page_shift - 4)) + slot / kBlock};
+}
+
+// One token's vectors of a group: loaded together, then worked off.
+template <int HD, int kQ, typename T, typename O>  // kQ: q heads in flight
+struct Token {
+    Vec<HD, T> k, v, q[kQ];
+    float4 c, s;
+    const T *qp;
+    O *op;
+    int64_t q_head, out_head;
+    int group;
+    __device__ __forceinline__ void load(const AppendParams &p, int64_t row, int pos, int kvh, int gl) {
+        k.load(static_cast<const T *>(p.k) + row * p.k_row + kvh * p.k_head, gl);
+        v.load(static_cast<const T *>(p.v) + row * p.v_row + kvh * p.v_head, gl);
+        group = p.group;
+        q_head = p.q_head, out_head = p.out_head;
+        qp = static_cast<const T *>(p.q) + row * p.q_row + static_cast<int64_t>(kvh) * group * q_head;
+        op = static_cast<O *>(p.q_out) + row * p.out_row + static_cast<int64_t>(kvh) * group * out_head;
+#pragma unroll
+        for (int i = 0; i < kQ; ++i)
+            if (i < group) q[i].load(qp + i * q_head, gl);
+        c = s = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.cos_t) {
+            c = *reinterpret_cast<const float4 *>(p.cos_t + static_cast<int64_t>(pos) * (HD / 2) + 4 * gl);
+            s = *reinterpret_cast<const float4 *>(p.sin_t + static_cast<int64_t>(pos) * (HD / 2) + 4 * gl);
+        }
+    }
+    __device__ __forceinline__ void key(const AppendParams &p, int gl, float (&x)[8]) const {
+        k.floats(x);
+        if (p.k_norm) {
+            float w[8];
+            load_weights<HD>(p.k_norm, gl, w);
+            norm_key<HD>(x, w);
+        }
+        if (p.cos_t) rotate(x, c, s);
+    }
+    // All lanes of the warp take part; `on`: of this group's token.
+    __device__ __forceinline__ void queries(const AppendParams &p, int gl, bool on) {
+        float w[8];
+        if (p.q_norm) load_weights<HD>(p.q_norm, gl, w);
+        for (int h0 = 0; h0 < group; h0 += kQ) {
+#pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                if (h0 + i >= group) break;
+                float x[8];
+                q[i].floats(x);
+                if (p.q_norm) norm<HD>(x, w);
+                if (p.cos_t) rotate(x, c, s);
+                if (on) {
+                    store4(op + (h0 + i) * out_head + 4 * gl, x);
+                    store4(op + (h0 + i) * out_head + HD / 2 + 4 * gl, x + 4);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kQ; ++i)
+                if (h0 + kQ + i < group) q[i].load(qp + (h0 + kQ + i) * q_head, gl);
+        }
+    }
+};
+
+// max_q 1: a group per (sequence, kv head).
+template <int HD, typename T, typename O>
+__global__ void __launch_bounds__(kTokenThreads) kv8_append_token_kernel(const AppendParams p) {
+    constexpr int kLanes = HD / 8, kGroups = kTokenThreads / kLanes;
+    kernel_begins();
+    const int gl = threadIdx.x % kLanes;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kLanes;
+    const int si = min(static_cast<int>(item / p.c.heads), p.b.batch - 1), kvh = static_cast<int>(item % p.c.heads);
+    const Seq s = load_seq(p.b, si, kvh == 0 && gl == 0);
+    const int pos = s.pos0;
+    const bool on = item < static_cast<int64_t>(p.b.batch) * p.c.heads && s.nq == 1 && pos >= 0;
+    if (!__any_sync(0xffffffffu, on)) return;
+    constexpr int kQ = 4;
+    Token<HD, kQ, T, O> tk;
+    int page = -1;
+    if (on) {
+        page = p.b.table[si * p.b.table_stride + (pos >> p.c.page_shift)];
+        tk.load(p, s.q0, pos, kvh, gl);
+    } else {
+        tk.group = p.group;  // the warp's other groups run along with what the registers hold
+        tk.k = tk.v = Vec<HD, T>{};
+        tk.c = tk.s = make_float4(0.f, 0.f, 0.f, 0.f);
+        tk.qp = static_cast<const T *>(p.q);
+        tk.q_head = 0;
+#pragma unroll
+        for (int i = 0; i < kQ; ++i) tk.q[i] = Vec<HD, T>{};
+    }
+    float k[8], v[8];
+    tk.key(p, gl, k);
+    tk.v.floats(v);
+    const uint32_t mk = most_of<HD>(k), mv = most_of<HD>(v);
+    tk.queries(p, gl, on);
+    if (!on) return;
+    if (page < 0 || page >= p.c.num_pages) {
+        if (gl == 0) set_error(p.b.err, kErrPage);
+        return;
+    }
+    const int t = pos % kBlock;
+    const Spot pl = spot_of(p.c, page, kvh, pos - t);
+    const bool bad = mk >= kInfBits || mv >= kInfBits;
+    float sk = scale_of(bad ? 0u : mk), sv = scale_of(bad ? 0u : mv);
+    uint8_t *kb = p.c.k + pl.at, *vb = p.c.v + pl.at;
+    if (t > 0) {  // the block's earlier tokens follow a scale that grows
+        const float ok = p.c.k_scale[pl.scale], ov = p.c.v_scale[pl.scale];
+        sk = fmaxf(sk, ok);
+        sv = fmaxf(sv, ov);
+        const float rk = ok / sk, rv = ov / sv;
+        if (rk != 1.0f || rv != 1.0f) {
+#pragma unroll 4
+            for (int i = 0; i < 4 * t; ++i) {  // K, then V of a token's two halves
+                uint8_t *row = (i & 1 ? vb : kb) + (i >> 2) * p.c.token_stride + (i & 2 ? HD / 2 : 0);
+                const uint32_t old = reinterpret_cast<uint32_t *>(row)[gl];
+                reinterpret_cast<uint32_t *>(row)[gl] = requantise(old, i & 1 ? rv : rk);
+            }
+        }
+    }
+    store_codes<HD>(kb + t * p.c.token_stride, gl, k, 1.0f / sk, bad, kBadKey);
+    store_codes<HD>(vb + t * p.c.token_stride, gl, v, 1.0f / sv, bad, 0u);
+    const uint32_t lanes = static_cast<uint32_t>((1ull << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes);
+    __syncwarp(lanes);  // every lane of the group has read the old scales
+    if (gl == 0) {
+        p.c.k_scale[pl.scale] = sk;
+        p.c.v_scale[pl.scale] = sv;
+    }
 }
 
 // Blocks by rows: sequence b has the indices [q_start[b] / 16 + 2 b, q_start[b + 1] / 16 + 2 (b + 1)), at least as
@@ -118,7 +301,7 @@ __device__ __forceinline__ int seq_of_block(const Batch &b, int index, int &base
     __shared__ int found;
     if (threadIdx.x == 0) found = -1;
     __syncthreads();
-    for (int i = threadIdx.x; i < b.batch; i += kThreads) {
+    for (int i = threadIdx.x; i < b.batch; i += blockDim.x) {
         const int a = min(max(b.q_start[i], 0), b.total_q), e = min(max(b.q_start[i + 1], a), b.total_q);
         if (index >= a / kBlock + 2 * i && index < e / kBlock + 2 * (i + 1)) atomicMax(&found, i);
     }
@@ -128,13 +311,14 @@ __device__ __forceinline__ int seq_of_block(const Batch &b, int index, int &base
     return i;
 }
 
+// A CTA of 16 groups per (sequence, block, kv head).
 template <int HD, typename T, typename O>
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
-    constexpr int kLanes = HD / 8, kGroups = kThreads / kLanes, kPer = 2 * kBlock / kGroups;
-    static_assert(kPer >= 1 && kPer * kGroups == 2 * kBlock, "32 K / V vectors over the groups");
+__global__ void __launch_bounds__(2 * HD, 512 / HD) kv8_append_block_kernel(const AppendParams p) {
+    constexpr int kLanes = HD / 8, kThreads = kBlock * kLanes;
     __shared__ uint32_t amax_s[2 * kBlock];  // K of tokens 0-15, V of tokens 0-15
+    kernel_begins();
     const int kvh = blockIdx.y, lane = threadIdx.x & 31;
-    const int gi = threadIdx.x / kLanes, gl = threadIdx.x % kLanes;
+    const int t = threadIdx.x / kLanes, gl = threadIdx.x % kLanes;
     int si, j;
     if (p.blocks_per_seq > 0) {
         si = blockIdx.x / p.blocks_per_seq;
@@ -146,128 +330,71 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
         j = blockIdx.x - base;
     }
     const Seq s = load_seq(p.b, si, j == 0 && kvh == 0 && threadIdx.x == 0);
-    const int blk = max(s.pos0, 0) / kBlock + j;
-    const int first = blk * kBlock;
+    const int first = (max(s.pos0, 0) / kBlock + j) * kBlock;
     const int lo = max(max(s.pos0, 0), first), hi = min(s.pos0 + s.nq, first + kBlock);
     if (lo >= hi) return;
-    // the block's place in the cache
-    const int pt = first >> p.c.page_shift;
-    const int page = p.b.table[si * p.b.table_stride + pt];
-    const bool page_ok = page >= 0 && page < p.c.num_pages;
-    if (!page_ok && threadIdx.x == 0) set_error(p.b.err, kErrPage);
-    const int slot = first & ((1 << p.c.page_shift) - 1);
-    const int64_t at = page * p.c.page_stride + kvh * p.c.head_stride + slot * p.c.token_stride;
-    const int64_t sc = ((static_cast<int64_t>(page) * p.c.heads + kvh) << (p.c.page_shift - 4)) + slot / kBlock;
-    const bool had = lo > first;  // the block holds earlier tokens
-    float old_k = 0.f, old_v = 0.f;
-    if (had && page_ok) {
-        old_k = p.c.k_scale[sc];
-        old_v = p.c.v_scale[sc];
+    const int page = p.b.table[si * p.b.table_stride + (first >> p.c.page_shift)];
+    const int pos = first + t;
+    const bool on = pos >= lo && pos < hi;
+    Token<HD, 2, T, O> tk;  // 64 registers: twice the CTAs of 4 heads in flight
+    // a group without a token runs along with the block's first new one
+    const int at_pos = on ? pos : lo;
+    tk.load(p, static_cast<int64_t>(s.q0) + at_pos - s.pos0, at_pos, kvh, gl);
+    float k[8], v[8];
+    tk.key(p, gl, k);
+    tk.v.floats(v);
+    const uint32_t mk = most_of<HD>(k), mv = most_of<HD>(v);
+    if (gl == 0) {
+        amax_s[t] = on ? mk : 0u;
+        amax_s[kBlock + t] = on ? mv : 0u;
     }
-    const int64_t row0 = static_cast<int64_t>(s.q0) - s.pos0;  // row of a position
-
-    // K and V vectors of the block: slot n = token n & 15 of K (n < 16) or V
-    float x[kPer][8];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int n = i * kGroups + gi, pos = first + (n & 15);
-        const bool on = pos >= lo && pos < hi;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-        if (on) {
-            const int64_t row = row0 + pos;
-            if (n < kBlock)
-                load_vec<HD, T>(static_cast<const T *>(p.k) + row * p.k_row + kvh * p.k_head, gl, x[i]);
-            else
-                load_vec<HD, T>(static_cast<const T *>(p.v) + row * p.v_row + kvh * p.v_head, gl, x[i]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int n = i * kGroups + gi, pos = first + (n & 15);
-        const bool on = pos >= lo && pos < hi;
-        uint32_t most = 0;
-        if (__any_sync(0xffffffffu, on)) {
-            // a warp's vectors are all K or all V; absent tokens hold zeros and take a valid position
-            if (n < kBlock) turn<HD>(x[i], gl, p.k_norm, p.cos_t, p.sin_t, on ? pos : lo);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                most = max(most, __float_as_uint(x[i][e]) & 0x7fffffffu);  // finite < infinity < NaN
-#pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        }
-        if (gl == 0) amax_s[n] = on ? most : 0u;
-    }
-    // the q heads of the block's tokens, from the groups' other end: with one token they run beside its K and V
-    const int nq = (hi - lo) * p.group;
-    for (int n0 = 0; n0 < nq; n0 += kGroups) {
-        const int n = n0 + kGroups - 1 - gi;
-        const bool on = n < nq;
-        const int pos = lo + (on ? n / p.group : 0), h = kvh * p.group + (on ? n % p.group : 0);
-        const int64_t row = row0 + pos;
-        float y[8];
-        load_vec<HD, T>(static_cast<const T *>(p.q) + row * p.q_row + h * p.q_head, gl, y);
-        turn<HD>(y, gl, p.q_norm, p.cos_t, p.sin_t, pos);
-        if (on) {
-            O *dst = static_cast<O *>(p.q_out) + row * p.out_row + h * p.out_head;
-            store4(dst + 4 * gl, y);
-            store4(dst + HD / 2 + 4 * gl, y + 4);
-        }
-    }
+    tk.queries(p, gl, on);
     __syncthreads();
-    if (!page_ok) return;
+    if (page < 0 || page >= p.c.num_pages) {
+        if (threadIdx.x == 0) set_error(p.b.err, kErrPage);
+        return;
+    }
+    const Spot pl = spot_of(p.c, page, kvh, first);
     // lane n < 16: K of token n, lane 16 + n: V of it; a token with a non-finite vector counts for neither scale
     const uint32_t mine = amax_s[lane], other = __shfl_xor_sync(0xffffffffu, mine, 16);
-    const bool bad = mine >= 0x7f800000u || other >= 0x7f800000u;
+    const bool bad = mine >= kInfBits || other >= kInfBits;
     const uint32_t bad_tokens = __ballot_sync(0xffffffffu, bad) & 0xffffu;
     uint32_t most = bad ? 0u : mine;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    float sk = __uint_as_float(static_cast<uint32_t>(scale_exponent(__shfl_sync(0xffffffffu, most, 0)) + 127) << 23);
-    float sv = __uint_as_float(static_cast<uint32_t>(scale_exponent(__shfl_sync(0xffffffffu, most, 16)) + 127) << 23);
-    if (had) {
-        // earlier tokens of the block follow a scale that grows; K and V apart
-        const float nk = fmaxf(sk, old_k), nv = fmaxf(sv, old_v);
+    float sk = scale_of(__shfl_sync(0xffffffffu, most, 0)), sv = scale_of(__shfl_sync(0xffffffffu, most, 16));
+    uint8_t *kb = p.c.k + pl.at, *vb = p.c.v + pl.at;
+    if (lo > first) {  // the block's earlier tokens follow a scale that grows
+        const float ok = p.c.k_scale[pl.scale], ov = p.c.v_scale[pl.scale];
+        __syncthreads();  // every thread has read the old scales
+        sk = fmaxf(sk, ok);
+        sv = fmaxf(sv, ov);
         const int words = (lo - first) * (HD / 4);
         for (int w = threadIdx.x; w < 2 * words; w += kThreads) {
             const bool is_k = w < words;
             const int r = is_k ? w : w - words;
-            const float ratio = is_k ? old_k / nk : old_v / nv;
+            const float ratio = is_k ? ok / sk : ov / sv;
             if (ratio == 1.0f) continue;
-            uint32_t *cell = reinterpret_cast<uint32_t *>((is_k ? p.c.k : p.c.v) + at +
-                                                          (r / (HD / 4)) * p.c.token_stride) + r % (HD / 4);
-            uint32_t a, b;
-            e4m3x4_to_h2x2(*cell, a, b);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a));
-            const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&b));
-            *cell = to_e4m3x4(f.x * ratio, f.y * ratio, g.x * ratio, g.y * ratio);
+            uint32_t *cell = reinterpret_cast<uint32_t *>((is_k ? kb : vb) + (r / (HD / 4)) * p.c.token_stride) + r % (HD / 4);
+            *cell = requantise(*cell, ratio);
         }
-        sk = nk;
-        sv = nv;
     }
     if (threadIdx.x == 0) {
-        p.c.k_scale[sc] = sk;
-        p.c.v_scale[sc] = sv;
+        p.c.k_scale[pl.scale] = sk;
+        p.c.v_scale[pl.scale] = sv;
     }
-    const float ik = 1.0f / sk, iv = 1.0f / sv;  // exact for the powers of two that this kernel writes
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int n = i * kGroups + gi, t = n & 15, pos = first + t;
-        if (pos < lo || pos >= hi) continue;
-        const float inv = n < kBlock ? ik : iv;
-        uint32_t a = to_e4m3x4(x[i][0] * inv, x[i][1] * inv, x[i][2] * inv, x[i][3] * inv);
-        uint32_t b = to_e4m3x4(x[i][4] * inv, x[i][5] * inv, x[i][6] * inv, x[i][7] * inv);
-        if (bad_tokens >> t & 1u) a = b = n < kBlock ? 0x7f7f7f7fu : 0u;  // key NaN, value 0
-        uint8_t *dst = (n < kBlock ? p.c.k : p.c.v) + at + t * p.c.token_stride;
-        reinterpret_cast<uint32_t *>(dst)[gl] = a;
-        reinterpret_cast<uint32_t *>(dst + HD / 2)[gl] = b;
-    }
+    if (!on) return;
+    store_codes<HD>(kb + t * p.c.token_stride, gl, k, 1.0f / sk, bad_tokens >> t & 1u, kBadKey);
+    store_codes<HD>(vb + t * p.c.token_stride, gl, v, 1.0f / sv, bad_tokens >> t & 1u, 0u);
 }
 
 template <int HD, typename T, typename O>
 cudaError_t launch(const AppendParams &p, dim3 grid, cudaStream_t s) {
-    kv8_append_kernel<HD, T, O><<<grid, kThreads, 0, s>>>(p);
-    return cudaGetLastError();
+    if (p.b.max_q > 1) return launch_behind(kv8_append_block_kernel<HD, T, O>, grid, 2 * HD, 0, s, p);
+    constexpr int kGroups = kTokenThreads / (HD / 8);
+    const int64_t items = static_cast<int64_t>(p.b.batch) * p.c.heads;
+    return launch_behind(kv8_append_token_kernel<HD, T, O>, dim3(static_cast<unsigned>((items + kGroups - 1) / kGroups)),
+                         kTokenThreads, 0, s, p);
 }
 template <int HD>
 cudaError_t launch_types(const AppendParams &p, dim3 grid, int in, int out, cudaStream_t s) {

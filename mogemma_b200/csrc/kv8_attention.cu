@@ -19,8 +19,8 @@
 // 16-byte copies kStages - 1 steps (8 KB each, hd 64: 4 KB) ahead, and nothing but its own
 // copies to wait for; token rows are padded by 16 bytes, so that the fragments'
 // loads meet no bank twice.  With the codes in registers instead, one step
-// ahead, 64 KB per SM at most were in flight: 4.3 TB/s where the ring reaches
-// RING_RATE.
+// ahead, 64 KB per SM at most were in flight: 4.3 TB/s on 1.37 GB of cache
+// where the ring reaches 5.8.
 //
 // With s = scale log2(e) k_scale <q, k> the state per row is m = max s,
 // l = sum 2^(s - m) and the sum of P V with P = 2^(s + log2 v_scale - M),
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
     using Cfg = RowsCfg<HD>;
     extern __shared__ __align__(16) unsigned char smem[];  // rings by warp; at an item's end [row][HD + 4] floats each
     __shared__ float mlm[kWarps][kRows][3];
-    asm volatile("griddepcontrol.launch_dependents;");
+    kernel_begins();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int cta = blockIdx.x, ctas = gridDim.x;
     unsigned char *ring = smem + warp * Cfg::kStages * Cfg::kStep;
@@ -147,6 +147,56 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
         const int tb = min((it.unit0 + wk.first + wk.take) * (kUnit / 16), (it.hi + 15) / 16);
         const int si = pair / p.a.tiles;
         const int32_t *table = p.b.table + si * p.b.table_stride;
+
+        // ---- the warp's tiles, kTiles neighbours per step: its n-th is ta + ((n / kTiles) kWarps + warp) kTiles + n % kTiles
+        auto tile_at = [&](int n) { return ta + ((n / Cfg::kTiles) * kWarps + warp) * Cfg::kTiles + n % Cfg::kTiles; };
+        // lane i holds the place and scales of tile number base + i (place -1: none), and the scales of the 32 before
+        int64_t place = -1;
+        float ks = 0.f, lvs = 0.f, ks_old = 0.f, lvs_old = 0.f;
+        uint32_t there = 0, there_old = 0;  // bit i: tile number base + i has a place
+        auto look_up = [&](int base) {
+            const int tile = tile_at(base + lane);
+            place = -1;
+            ks_old = ks;
+            lvs_old = lvs;
+            there_old = there;
+            ks = 0.f;
+            lvs = 1.f;
+            if (tile < tb) {
+                const int tok = tile * 16, slot = tok & ((1 << p.c.page_shift) - 1);
+                const int page = table[tok >> p.c.page_shift];
+                if (page >= 0 && page < p.c.num_pages) {
+                    const int64_t sc = ((static_cast<int64_t>(page) * p.c.heads + head) << (p.c.page_shift - 4)) +
+                                       (slot >> 4);
+                    place = page * p.c.page_stride + head * p.c.head_stride + slot * p.c.token_stride;
+                    ks = p.c.k_scale[sc];
+                    lvs = p.c.v_scale[sc];
+                } else {
+                    set_error(p.b.err, kErrPage);
+                }
+            }
+            there = __ballot_sync(0xffffffffu, place >= 0);
+        };
+        const int steps = (tb - ta + kWarps * Cfg::kTiles - 1) / (kWarps * Cfg::kTiles);
+        // A step's copies; the scales, read along with the places, have until the step is worked on to arrive.
+        auto fetch = [&](int step, int stage) {
+            if (step < steps) {
+                const int n0 = step * Cfg::kTiles;
+                if ((n0 & 31) == 0) look_up(n0);
+#pragma unroll
+                for (int i = 0; i < Cfg::kTiles; ++i) {
+                    const int64_t at = __shfl_sync(0xffffffffu, place, (n0 + i) & 31);
+                    const int live = at < 0 ? 0 : it.hi - tile_at(n0 + i) * 16;
+                    const int64_t src = at < 0 ? 0 : at;
+                    const uint32_t dst = ring_s + stage * Cfg::kStep + i * 16 * Cfg::kRow;
+                    copy_tile<HD>(dst, p.c.k + src, p.c.token_stride, live, lane);
+                    copy_tile<HD>(dst + Cfg::kTiles * 16 * Cfg::kRow, p.c.v + src, p.c.token_stride, live, lane);
+                }
+            }
+            copies_commit();  // an empty group past the end: the count of groups stays that of steps
+        };
+#pragma unroll
+        for (int i = 0; i < Cfg::kStages - 1; ++i) fetch(i, i);
 
         // ---- query rows: B fragments, row g, k order as the K fragments
         uint32_t qf[HD / 64][4][2];
@@ -205,63 +255,12 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
             }
         }
 
-        // ---- the warp's tiles, kTiles neighbours per step: its n-th is ta + ((n / kTiles) kWarps + warp) kTiles + n % kTiles
         float o[Cfg::kM][4];
 #pragma unroll
         for (int i = 0; i < Cfg::kM; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
         float m[2] = {-kInf, -kInf}, mv[2] = {-kInf, -kInf}, l[2] = {0.f, 0.f};
-        auto tile_at = [&](int n) { return ta + ((n / Cfg::kTiles) * kWarps + warp) * Cfg::kTiles + n % Cfg::kTiles; };
-        // lane i holds the place and scales of tile number base + i; place -1: none
-        int64_t place = -1;
-        float ks = 0.f, lvs = 0.f;
-        auto look_up = [&](int base) {
-            const int tile = tile_at(base + lane);
-            place = -1;
-            ks = 0.f;
-            lvs = 0.f;
-            if (tile < tb) {
-                const int tok = tile * 16, slot = tok & ((1 << p.c.page_shift) - 1);
-                const int page = table[tok >> p.c.page_shift];
-                if (page >= 0 && page < p.c.num_pages) {
-                    const int64_t sc = ((static_cast<int64_t>(page) * p.c.heads + head) << (p.c.page_shift - 4)) +
-                                       (slot >> 4);
-                    place = page * p.c.page_stride + head * p.c.head_stride + slot * p.c.token_stride;
-                    ks = p.c.k_scale[sc];
-                    lvs = __log2f(p.c.v_scale[sc]);
-                } else {
-                    set_error(p.b.err, kErrPage);
-                }
-            }
-        };
-        const int steps = (tb - ta + kWarps * Cfg::kTiles - 1) / (kWarps * Cfg::kTiles);
-        // step n's copies, and its tiles' scales (K; log2 of V) for later: they are shuffled out of the lanes' look-up
-        // window before it moves on
-        float ks_at[Cfg::kStages][Cfg::kTiles], lv_at[Cfg::kStages][Cfg::kTiles];
-        uint32_t there = 0;  // bit kTiles * stage + i: the tile has a place
-        auto fetch = [&](int step, int stage) {
-            if (step < steps) {
-                const int n0 = step * Cfg::kTiles;
-                if ((n0 & 31) == 0) look_up(n0);
-#pragma unroll
-                for (int i = 0; i < Cfg::kTiles; ++i) {
-                    const int64_t at = __shfl_sync(0xffffffffu, place, (n0 + i) & 31);
-                    ks_at[stage][i] = __shfl_sync(0xffffffffu, ks, (n0 + i) & 31);
-                    lv_at[stage][i] = __shfl_sync(0xffffffffu, lvs, (n0 + i) & 31);
-                    const uint32_t bit = 1u << (Cfg::kTiles * stage + i);
-                    there = at >= 0 ? there | bit : there & ~bit;
-                    const int live = at < 0 ? 0 : it.hi - tile_at(n0 + i) * 16;
-                    const int64_t src = at < 0 ? 0 : at;
-                    const uint32_t dst = ring_s + stage * Cfg::kStep + i * 16 * Cfg::kRow;
-                    copy_tile<HD>(dst, p.c.k + src, p.c.token_stride, live, lane);
-                    copy_tile<HD>(dst + Cfg::kTiles * 16 * Cfg::kRow, p.c.v + src, p.c.token_stride, live, lane);
-                }
-            }
-            copies_commit();  // an empty group past the end: the count of groups stays that of steps
-        };
-#pragma unroll
-        for (int i = 0; i < Cfg::kStages - 1; ++i) fetch(i, i);
         auto work = [&](int step, int stage) {
             const int n0 = step * Cfg::kTiles;
             copies_wait<Cfg::kStages - 1>();
@@ -293,8 +292,13 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
             float sk[Cfg::kTiles], lv[Cfg::kTiles];
             bool seen[Cfg::kTiles];
 #pragma unroll
-            for (int i = 0; i < Cfg::kTiles; ++i)
-                sk[i] = ks_at[stage][i], lv[i] = lv_at[stage][i], seen[i] = there >> (Cfg::kTiles * stage + i) & 1u;
+            for (int i = 0; i < Cfg::kTiles; ++i) {
+                const int n = n0 + i;  // the copies are up to kStages - 1 steps ahead: perhaps in the next window
+                const bool old = n / 32 != min(step + Cfg::kStages - 1, steps - 1) * Cfg::kTiles / 32;
+                sk[i] = __shfl_sync(0xffffffffu, old ? ks_old : ks, n & 31);
+                lv[i] = __log2f(__shfl_sync(0xffffffffu, old ? lvs_old : lvs, n & 31));
+                seen[i] = (old ? there_old : there) >> (n & 31) & 1u;
+            }
             float top[2] = {-kInf, -kInf}, topv[2] = {-kInf, -kInf};
 #pragma unroll
             for (int i = 0; i < Cfg::kTiles; ++i) {
@@ -435,12 +439,11 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
 }
 
 // Joins the partial answers of the items that several CTAs share: their
-// weights are l 2^(m - max m).  16 lanes hold 64 dims of a row; the CTA's 16
-// such groups take a row each where an item has few parts (prompts: 2 or 3),
-// or share one row's parts where it has many (one long context: hundreds), so
-// that the loads of all parts are in flight at once.  Tasks (item, rows, 64
-// dims) are dealt over a fixed grid; the sums run in the order of the CTAs, the
-// same every time.
+// weights are l 2^(m - max m).  An item of few parts (prompts: 2 or 3) has a
+// row per 16 lanes; the parts of one of many (a long context: hundreds) are
+// spread over the CTA, so that the loads of all of them are in flight at once.
+// Tasks (item, rows, dims) are dealt over a fixed grid; the order of the sums
+// is that of the CTAs, the same every time.
 constexpr int kCombThreads = 256;
 constexpr int kFewParts = 8;
 constexpr int kCombPerSm = 4;
@@ -462,18 +465,18 @@ template <typename T>
 __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArgs p, int hd, int ctas) {
     extern __shared__ int sm_i[];  // [ctas] tasks of the entries before this one
     __shared__ int warp_n[kCombThreads / 32];
-    __shared__ float4 acc_s[16][16];
-    __shared__ float2 ml_s[16];
+    __shared__ float4 acc_s[kCombThreads / 32][4];
+    __shared__ float2 ml_s[kCombThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid >> 4, gl = tid & 15;
-    const int chunks = hd / 64;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int chunks = hd / 64, fine = hd / 16;
+    kernel_begins();
     int tasks = 0;
     for (int i0 = 0; i0 < ctas; i0 += kCombThreads) {
         const int i = i0 + tid;
         int mine = 0;
         if (i < ctas) {
             const Split sp = p.part.split[i];
-            if (sp.nrows > 0) mine = (sp.last_cta - i < kFewParts ? (sp.nrows + 15) / 16 : sp.nrows) * chunks;
+            if (sp.nrows > 0) mine = sp.last_cta - i < kFewParts ? (sp.nrows + 15) / 16 * chunks : sp.nrows * fine;
         }
         int upto = mine;
 #pragma unroll
@@ -502,10 +505,12 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
         const Split sp = p.part.split[first];
         const int sub = task - sm_i[first], n = sp.last_cta - first + 1;
         const bool few = n <= kFewParts;
-        const int r = few ? 16 * (sub / chunks) + grp : sub / chunks, d = 64 * (sub % chunks) + 4 * gl;
+        // few parts: 16 lanes hold 64 dims, a row per 16 lanes; many: 4 lanes hold 16 dims, every 64th part per 4 lanes
+        const int r = few ? 16 * (sub / chunks) + grp : sub / fine;
+        const int d = few ? 64 * (sub % chunks) + 4 * gl : 16 * (sub % fine) + 4 * (tid & 3);
         Joined j;
         if (r < sp.nrows) {
-            const int i0 = few ? 0 : grp, step = few ? 1 : 16;
+            const int i0 = few ? 0 : tid >> 2, step = few ? 1 : kCombThreads / 4;
 #pragma unroll 4
             for (int i = i0; i < n; i += step) {
                 const int64_t at = static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r;
@@ -513,27 +518,42 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
                 j.add(ml.x, ml.y, *reinterpret_cast<const float4 *>(p.part.o + at * hd + d));
             }
         }
-        if (!few) {  // join the groups
-            acc_s[grp][gl] = j.acc;
-            if (gl == 0) ml_s[grp] = make_float2(j.m, j.l);
+        if (!few) {  // join the warp's 8 groups, then the warps
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                const float om = __shfl_xor_sync(0xffffffffu, j.m, o), ol = __shfl_xor_sync(0xffffffffu, j.l, o);
+                float4 v;
+                v.x = __shfl_xor_sync(0xffffffffu, j.acc.x, o), v.y = __shfl_xor_sync(0xffffffffu, j.acc.y, o);
+                v.z = __shfl_xor_sync(0xffffffffu, j.acc.z, o), v.w = __shfl_xor_sync(0xffffffffu, j.acc.w, o);
+                const float top = fmaxf(j.m, om), b = top == -kInf ? 0.f : top;
+                const float fa = ex2(j.m - b), fb = ex2(om - b);
+                j.acc.x = j.acc.x * fa + v.x * fb, j.acc.y = j.acc.y * fa + v.y * fb;
+                j.acc.z = j.acc.z * fa + v.z * fb, j.acc.w = j.acc.w * fa + v.w * fb;
+                j.l = j.l * fa + ol * fb;
+                j.m = top;
+            }
+            if (lane < 4) {
+                acc_s[warp][lane] = j.acc;
+                if (lane == 0) ml_s[warp] = make_float2(j.m, j.l);
+            }
             __syncthreads();
-            if (grp == 0) {
+            if (tid < 4) {
                 j = Joined();
                 float top = -kInf;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, ml_s[i].x);
+                for (int i = 0; i < kCombThreads / 32; ++i) top = fmaxf(top, ml_s[i].x);
                 const float b = top == -kInf ? 0.f : top;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < kCombThreads / 32; ++i) {
                     const float f = ex2(ml_s[i].x - b);
-                    const float4 v = acc_s[i][gl];
+                    const float4 v = acc_s[i][tid];
                     j.acc.x += v.x * f, j.acc.y += v.y * f, j.acc.z += v.z * f, j.acc.w += v.w * f;
                     j.l += ml_s[i].y * f;
                 }
             }
             __syncthreads();
         }
-        if (r < sp.nrows && (few || grp == 0)) {
+        if (r < sp.nrows && (few || tid < 4)) {
             const float f = j.l == 0.f ? 0.f : 1.0f / j.l;
             const int si = sp.pair / p.a.tiles, row = (sp.pair - si * p.a.tiles) * p.a.rows + r;
             const int tok = row / p.a.group, hq = sp.head * p.a.group + row - tok * p.a.group;
@@ -556,27 +576,14 @@ cudaError_t sm_count(int *sms) {
 template <int HD, typename T>
 cudaError_t launch_rows(const AttnArgs &p, int ctas, cudaStream_t s) {
     const size_t smem = RowsCfg<HD>::kSmem;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv8_rows_kernel<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
-    }
-    kv8_rows_kernel<HD, T><<<ctas, kThreads, smem, s>>>(p);
-    return cudaGetLastError();
+    const cudaError_t e = cudaFuncSetAttribute(kv8_rows_kernel<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    return e != cudaSuccess ? e : launch_behind(kv8_rows_kernel<HD, T>, dim3(ctas), kThreads, smem, s, p);
 }
 template <typename T>
 cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kCombPerSm * sms);
-    cfg.blockDim = dim3(kCombThreads);
-    cfg.dynamicSmemBytes = sizeof(int) * static_cast<size_t>(ctas);
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv8_combine_kernel<T>, p, hd, ctas);
+    return launch_behind(kv8_combine_kernel<T>, dim3(kCombPerSm * sms), kCombThreads,
+                         sizeof(int) * static_cast<size_t>(ctas), s, p, hd, ctas);
 }
 template <typename T>
 cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {

@@ -261,7 +261,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     __shared__ int stop_s;
     volatile int *stop = &stop_s;
     uint32_t *err = p.b.err;
-    asm volatile("griddepcontrol.launch_dependents;");
     const uintptr_t base = (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023);
     unsigned char *gen = reinterpret_cast<unsigned char *>(base);
     const uint32_t sq = smem_u32(gen), sk = sq + C::kQBytes, sv = sk + kSt * C::kTileBytes;
@@ -300,6 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    kernel_begins();
     const Place pl = find_place<kThreads>(p.b, p.a, p.c.heads, cta, gridDim.x);
     tc::tc_fence_before();
     __syncthreads();
@@ -857,9 +857,7 @@ template <int HD, typename T>
 cudaError_t launch(const AttnArgs &p, int ctas, cudaStream_t s) {
     const cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(Cfg<HD>::kSmem));
-    if (e != cudaSuccess) return e;
-    kv8_prompt_kernel<HD, T><<<ctas, kThreads, Cfg<HD>::kSmem, s>>>(p);
-    return cudaGetLastError();
+    return e != cudaSuccess ? e : launch_behind(kv8_prompt_kernel<HD, T>, dim3(ctas), kThreads, Cfg<HD>::kSmem, s, p);
 }
 }  // namespace
 
