@@ -264,7 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     const uintptr_t base = (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023);
     unsigned char *gen = reinterpret_cast<unsigned char *>(base);
     const uint32_t sq = smem_u32(gen), sk = sq + C::kQBytes, sv = sk + kSt * C::kTileBytes;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // broadcast, so that what depends on the warp alone is warp-uniform to the compiler (the MMAs' operands)
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int cta = blockIdx.x;
 
     if (threadIdx.x == 0) {
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     // The i-th item; null at the end of the share, or (stop set) when a wait ran out.
     auto item = [&](uint32_t i) -> const Desc * {
         const bool ok = wait(&item_full[i % kItems], (i / kItems) & 1u, stop, err);
@@ -339,8 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             bool begun = false;
             auto sees = [&](int j) { return d->sees(g, d->token(j)); };
             // S of unit u, the item's j-th
-            auto s_of = [&](uint32_t u, int j) -> bool {
-                const uint32_t st = u % kSt, ss = u % kSS;
+            auto s_at = [&](auto parity, uint32_t u, int j) -> bool {
+                constexpr uint32_t st = decltype(parity)::value % kSt, ss = decltype(parity)::value % kSS;
                 if (!warp_wait(&k_full[st], (u / kSt) & 1u)) return false;
                 tc::tc_fence_after();
                 if (sees(j)) {
@@ -358,8 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                 return true;
             };
             // P V of unit n, the item's j-th
-            auto pv_of = [&](int j) -> bool {
-                const uint32_t st = n % kSt, ss = n % kSS;
+            auto pv_at = [&](auto parity, int j) -> bool {
+                constexpr uint32_t st = decltype(parity)::value % kSt, ss = decltype(parity)::value % kSS;
                 if (!warp_wait(&v_full[st], (n / kSt) & 1u)) return false;
                 if (sees(j)) {
                     if (!warp_wait(&p_full[g][ss], uses >> ss & 1u)) return false;
@@ -381,6 +382,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                 commit(&v_empty[st]);
                 return true;
             };
+            using Even = std::integral_constant<uint32_t, 0>;  // stages are constants to the MMAs
+            using Odd = std::integral_constant<uint32_t, 1>;
+            auto s_of = [&](uint32_t u, int j) { return u & 1 ? s_at(Odd(), u, j) : s_at(Even(), u, j); };
+            auto pv_of = [&](int j) { return n & 1 ? pv_at(Odd(), j) : pv_at(Even(), j); };
             if (d->sees(g, d->tok0, take)) ok = warp_wait(&q_full[g], acts++ & 1u);
             ok = ok && s_of(n, 0);
             for (int j = 0; ok && j < take; ++j, ++n) {
@@ -542,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         const uint32_t t_o = tmem + tg * HD + lane_off, t_s0 = tmem + C::kS + kSS * tg * kN + lane_off;
         uint32_t n = 0, acts = 0;         // units of the share; items in which this tile sees something
         uint32_t uses = 0;                // bit st: parity of the tile's uses of S stage st
+        uint32_t met = 0;                 // bit st: parity of this warp's exchanges with its other half
         bool ok = true;
         for (uint32_t i_at = 0;; ++i_at) {
             const Desc *d = warp_item(i_at);
@@ -770,8 +776,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         xch[st][wg][r] = make_float2(mn, vn);
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&pair_bar[warp & 3][st]);
-                        ok = warp_wait(&pair_bar[warp & 3][st], ph);
+                        ok = warp_wait(&pair_bar[warp & 3][st], met >> st & 1u);
                         if (!ok) break;
+                        met ^= 1u << st;  // not `uses`: a warp without rows in an item exchanges nothing
                         const float2 o = xch[st][wg ^ 1][r];
                         ok = move_to(fmaxf(mn, o.x), fmaxf(vn, o.y), 0);
                         if (!ok) break;

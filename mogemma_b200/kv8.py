@@ -33,6 +33,11 @@ BLOCK = 16  # tokens per scale (MG_KV8_BLOCK)
 _TYPES = {torch.float32: _core.MG_F32, torch.bfloat16: _core.MG_BF16, torch.float16: _core.MG_F16}
 
 
+# The current stream's handle without making a torch.cuda.Stream of it (3 us a call).
+_raw_stream: Callable[[int], int] = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (  # noqa: SLF001
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
@@ -81,9 +86,9 @@ class KV8Call:
         dev = self._device.index
         if torch.cuda.current_device() != dev:
             with torch.cuda.device(dev):
-                status = self._fn(*self._refs, torch.cuda.current_stream().cuda_stream)
+                status = self._fn(*self._refs, _raw_stream(dev))
         else:
-            status = self._fn(*self._refs, torch.cuda.current_stream().cuda_stream)
+            status = self._fn(*self._refs, _raw_stream(dev))
         if status:
             _core._check(status)  # noqa: SLF001
 

@@ -455,3 +455,20 @@ def test_bad_tensors_are_refused() -> None:
     wide = KV8Batch(b.q_start, b.ctx_len, b.page_table, max_q=2, max_ctx=10**6)
     with pytest.raises(ValueError, match="page table"):
         c.attention(wide, q)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("seed", range(4))
+def test_attention_of_items_of_many_sizes(dim, seed) -> None:
+    """Sequences whose rows fill one warp, several or all of a row tile, in every order within a CTA's share: what a
+    warp skips in one item must not put it out of step in the next."""
+    r = random.Random(seed * 3 + dim)
+    lens = []
+    for _ in range(60):
+        n = r.choice([1, 2, 9, 16, 17, 33, 40, 64, 65, 100])
+        lens.append((n, n + r.choice([0, 1, 30, 127, 128, 300, 900])))
+    w = World(lens, kv_heads=8, dim=dim, page=32, seed=seed)
+    q = w.rand(w.rows, 16, dim, dtype=BF16)
+    window = r.choice([0, 0, 40, 200])
+    out = w.cache.attention(w.batch, q, window=window)
+    _check_attention(w, q, out, scale=dim**-0.5, window=window)
