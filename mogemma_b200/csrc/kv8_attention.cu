@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
         int mine = 0;
         if (i < ctas) {
             const Split sp = p.part.split[i];
-            if (sp.nrows > 0) mine = sp.last_cta - i < kFewParts ? (sp.nrows + 15) / 16 * chunks : sp.nrows * fine;
+            if (sp.nrows > 0) mine = sp.last_cta - i < kFewParts ? (sp.nrows + 15) / 16 : sp.nrows * fine;
         }
         int upto = mine;
 #pragma unroll
@@ -495,6 +495,12 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
         if (i < ctas) sm_i[i] = before;
         __syncthreads();
     }
+    auto out_at = [&](const Split &sp, int r) {  // row r of the item
+        const int si = sp.pair / p.a.tiles, row = (sp.pair - si * p.a.tiles) * p.a.rows + r;
+        const int tok = row / p.a.group, hq = sp.head * p.a.group + row - tok * p.a.group;
+        return static_cast<T *>(p.out) + (static_cast<int64_t>(load_seq(p.b, si, false).q0) + tok) * p.out_row +
+               hq * p.out_head;
+    };
     for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
         int first = 0, end = ctas;  // the last entry with sm_i <= task: the one that has it, as empty ones follow it
         while (end - first > 1) {
@@ -504,63 +510,74 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
         }
         const Split sp = p.part.split[first];
         const int sub = task - sm_i[first], n = sp.last_cta - first + 1;
-        const bool few = n <= kFewParts;
-        // few parts: 16 lanes hold 64 dims, a row per 16 lanes; many: 4 lanes hold 16 dims, every 64th part per 4 lanes
-        const int r = few ? 16 * (sub / chunks) + grp : sub / fine;
-        const int d = few ? 64 * (sub % chunks) + 4 * gl : 16 * (sub % fine) + 4 * (tid & 3);
-        Joined j;
-        if (r < sp.nrows) {
-            const int i0 = few ? 0 : tid >> 2, step = few ? 1 : kCombThreads / 4;
-#pragma unroll 4
-            for (int i = i0; i < n; i += step) {
+        if (n <= kFewParts) {  // 16 lanes hold a row, lane gl dims 64 c + 4 gl ..
+            const int r = 16 * sub + grp;
+            if (r >= sp.nrows) continue;
+            Joined j[4];
+#pragma unroll 2
+            for (int i = 0; i < n; ++i) {
                 const int64_t at = static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r;
                 const float2 ml = *reinterpret_cast<const float2 *>(p.part.ml + 2 * at);
-                j.add(ml.x, ml.y, *reinterpret_cast<const float4 *>(p.part.o + at * hd + d));
+                float4 v[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < chunks) v[c] = *reinterpret_cast<const float4 *>(p.part.o + at * hd + 64 * c + 4 * gl);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < chunks) j[c].add(ml.x, ml.y, v[c]);
             }
+            T *dst = out_at(sp, r) + 4 * gl;
+            const float f = j[0].l == 0.f ? 0.f : 1.0f / j[0].l;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (c < chunks) store_out4(dst + 64 * c, j[c].acc.x * f, j[c].acc.y * f, j[c].acc.z * f, j[c].acc.w * f);
+            continue;
         }
-        if (!few) {  // join the warp's 8 groups, then the warps
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-                const float om = __shfl_xor_sync(0xffffffffu, j.m, o), ol = __shfl_xor_sync(0xffffffffu, j.l, o);
-                float4 v;
-                v.x = __shfl_xor_sync(0xffffffffu, j.acc.x, o), v.y = __shfl_xor_sync(0xffffffffu, j.acc.y, o);
-                v.z = __shfl_xor_sync(0xffffffffu, j.acc.z, o), v.w = __shfl_xor_sync(0xffffffffu, j.acc.w, o);
-                const float top = fmaxf(j.m, om), b = top == -kInf ? 0.f : top;
-                const float fa = ex2(j.m - b), fb = ex2(om - b);
-                j.acc.x = j.acc.x * fa + v.x * fb, j.acc.y = j.acc.y * fa + v.y * fb;
-                j.acc.z = j.acc.z * fa + v.z * fb, j.acc.w = j.acc.w * fa + v.w * fb;
-                j.l = j.l * fa + ol * fb;
-                j.m = top;
-            }
-            if (lane < 4) {
-                acc_s[warp][lane] = j.acc;
-                if (lane == 0) ml_s[warp] = make_float2(j.m, j.l);
-            }
-            __syncthreads();
-            if (tid < 4) {
-                j = Joined();
-                float top = -kInf;
-#pragma unroll
-                for (int i = 0; i < kCombThreads / 32; ++i) top = fmaxf(top, ml_s[i].x);
-                const float b = top == -kInf ? 0.f : top;
-#pragma unroll
-                for (int i = 0; i < kCombThreads / 32; ++i) {
-                    const float f = ex2(ml_s[i].x - b);
-                    const float4 v = acc_s[i][tid];
-                    j.acc.x += v.x * f, j.acc.y += v.y * f, j.acc.z += v.z * f, j.acc.w += v.w * f;
-                    j.l += ml_s[i].y * f;
-                }
-            }
-            __syncthreads();
+        // 4 lanes hold 16 dims of the row, every 64th part per 4 lanes
+        const int r = sub / fine, d = 16 * (sub % fine) + 4 * (tid & 3);
+        Joined j;
+#pragma unroll 4
+        for (int i = tid >> 2; i < n; i += kCombThreads / 4) {
+            const int64_t at = static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r;
+            const float2 ml = *reinterpret_cast<const float2 *>(p.part.ml + 2 * at);
+            j.add(ml.x, ml.y, *reinterpret_cast<const float4 *>(p.part.o + at * hd + d));
         }
-        if (r < sp.nrows && (few || tid < 4)) {
+        // join the warp's 8 groups, then the warps
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, j.m, o), ol = __shfl_xor_sync(0xffffffffu, j.l, o);
+            float4 v;
+            v.x = __shfl_xor_sync(0xffffffffu, j.acc.x, o), v.y = __shfl_xor_sync(0xffffffffu, j.acc.y, o);
+            v.z = __shfl_xor_sync(0xffffffffu, j.acc.z, o), v.w = __shfl_xor_sync(0xffffffffu, j.acc.w, o);
+            const float top = fmaxf(j.m, om), b = top == -kInf ? 0.f : top;
+            const float fa = ex2(j.m - b), fb = ex2(om - b);
+            j.acc.x = j.acc.x * fa + v.x * fb, j.acc.y = j.acc.y * fa + v.y * fb;
+            j.acc.z = j.acc.z * fa + v.z * fb, j.acc.w = j.acc.w * fa + v.w * fb;
+            j.l = j.l * fa + ol * fb;
+            j.m = top;
+        }
+        if (lane < 4) {
+            acc_s[warp][lane] = j.acc;
+            if (lane == 0) ml_s[warp] = make_float2(j.m, j.l);
+        }
+        __syncthreads();
+        if (tid < 4) {
+            j = Joined();
+            float top = -kInf;
+#pragma unroll
+            for (int i = 0; i < kCombThreads / 32; ++i) top = fmaxf(top, ml_s[i].x);
+            const float b = top == -kInf ? 0.f : top;
+#pragma unroll
+            for (int i = 0; i < kCombThreads / 32; ++i) {
+                const float f = ex2(ml_s[i].x - b);
+                const float4 v = acc_s[i][tid];
+                j.acc.x += v.x * f, j.acc.y += v.y * f, j.acc.z += v.z * f, j.acc.w += v.w * f;
+                j.l += ml_s[i].y * f;
+            }
             const float f = j.l == 0.f ? 0.f : 1.0f / j.l;
-            const int si = sp.pair / p.a.tiles, row = (sp.pair - si * p.a.tiles) * p.a.rows + r;
-            const int tok = row / p.a.group, hq = sp.head * p.a.group + row - tok * p.a.group;
-            T *dst = static_cast<T *>(p.out) + (static_cast<int64_t>(load_seq(p.b, si, false).q0) + tok) * p.out_row +
-                     hq * p.out_head + d;
-            store_out4(dst, j.acc.x * f, j.acc.y * f, j.acc.z * f, j.acc.w * f);
+            store_out4(out_at(sp, r) + d, j.acc.x * f, j.acc.y * f, j.acc.z * f, j.acc.w * f);
         }
+        __syncthreads();
     }
 }
 
