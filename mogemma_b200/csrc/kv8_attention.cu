@@ -2,8 +2,8 @@
 // (the attention of layers.mojo:63-94), for few query rows per kv head; the
 // combine of partial answers; and the entry points.
 //
-// kv8_rows_kernel takes items of up to 8 query rows.  It is bound by reading
-// the cache: one code byte feeds 8 rows' products, so the legacy warp-level
+// kv8_rows_kernel takes items of up to 8 or 16 query rows.  It is bound by reading
+// the cache: one code byte feeds few rows' products, so the legacy warp-level
 // MMA is fast enough.  A warp takes 16 tokens (one scale block) at a time and
 // computes transposed products, tokens and head dims on the MMA's 16 rows, the
 // query rows on its 8 columns:
@@ -43,7 +43,7 @@ int prompt_rows(int hd);
 cudaError_t launch_prompt(const AttnArgs &p, int hd, bool f16, int ctas, cudaStream_t s);
 
 namespace {
-constexpr int kRows = 8;       // query rows of an item
+constexpr int kRows = 8;       // query rows of an MMA; an item has 8 or 16
 constexpr int kUnit = 64;      // tokens of a unit of the schedule
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
@@ -100,7 +100,7 @@ struct RowsCfg {
     static constexpr int kStep = 2 * kTiles * 16 * kRow;  // K rows, then V rows
     static constexpr int kStages = HD == 64 ? 5 : 3;    // 100 to 110 KB for four warps: two CTAs per SM
     static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kStages * kStep;
-    static_assert(sizeof(float) * kRows * (HD + 4) <= kStages * kStep, "the merge takes the place of a warp's ring");
+    static_assert(sizeof(float) * 2 * kRows * (HD + 4) <= kStages * kStep, "the merge takes the place of a warp's ring");
 };
 
 // 16 bytes to shared memory, asynchronously; zeros where !on.
@@ -124,11 +124,11 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t *tile, int
     }
 }
 
-template <int HD, typename T>
+template <int HD, int NT, typename T>  // NT: 8-row tiles of an item
 __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
     using Cfg = RowsCfg<HD>;
     extern __shared__ __align__(16) unsigned char smem[];  // rings by warp; at an item's end [row][HD + 4] floats each
-    __shared__ float mlm[kWarps][kRows][3];
+    __shared__ float mlm[kWarps][NT * kRows][3];
     kernel_begins();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int cta = blockIdx.x, ctas = gridDim.x;
@@ -199,12 +199,13 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
         for (int i = 0; i < Cfg::kStages - 1; ++i) fetch(i, i);
 
         // ---- query rows: B fragments, row g, k order as the K fragments
-        uint32_t qf[HD / 64][4][2];
-        float factor[2];
-        int lo[2], hi[2];
-        {
-            const int r = it.row0 + g;
-            const bool on = g < it.nrows;
+        uint32_t qf[NT][HD / 64][4][2];
+        float factor[NT][2];
+        int lo[NT][2], hi[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = it.row0 + nt * kRows + g;
+            const bool on = nt * kRows + g < it.nrows;
             const int tok = on ? r / p.a.group : 0, h = head * p.a.group + (on ? r - tok * p.a.group : 0);
             const T *src = static_cast<const T *>(p.q) + (static_cast<int64_t>(it.seq.q0) + tok) * p.q_row +
                            h * p.q_head + 16 * t;
@@ -242,36 +243,40 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float2 f = two<T>(raw[c][i]);
-                    qf[c][i >> 1][i & 1] = pack_h2(f.x * up, f.y * up);
+                    qf[nt][c][i >> 1][i & 1] = pack_h2(f.x * up, f.y * up);
                 }
             // columns 2 t, 2 t + 1 of the accumulators are rows held by lanes 8 t, 8 t + 4
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                factor[i] = p.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t + 4 * i);
-                const int ri = 2 * t + i;
+                factor[nt][i] = p.scale_log2 * __shfl_sync(0xffffffffu, down, 8 * t + 4 * i);
+                const int ri = nt * kRows + 2 * t + i;
                 const int pos = it.seq.pos0 + (it.row0 + ri) / p.a.group;
-                hi[i] = ri < it.nrows ? pos + 1 : 0;
-                lo[i] = p.a.window > 0 ? pos - p.a.window + 1 : 0;
+                hi[nt][i] = ri < it.nrows ? pos + 1 : 0;
+                lo[nt][i] = p.a.window > 0 ? pos - p.a.window + 1 : 0;
             }
         }
 
-        float o[Cfg::kM][4];
+        float o[NT][Cfg::kM][4], m[NT][2], mv[NT][2], l[NT][2];
 #pragma unroll
-        for (int i = 0; i < Cfg::kM; ++i)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-        float m[2] = {-kInf, -kInf}, mv[2] = {-kInf, -kInf}, l[2] = {0.f, 0.f};
+            for (int i = 0; i < Cfg::kM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+            m[nt][0] = m[nt][1] = mv[nt][0] = mv[nt][1] = -kInf;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
         auto work = [&](int step, int stage) {
             const int n0 = step * Cfg::kTiles;
             copies_wait<Cfg::kStages - 1>();
             __syncwarp();
             const unsigned char *kt = ring + stage * Cfg::kStep, *vt = kt + Cfg::kTiles * 16 * Cfg::kRow;
             // S^T
-            float s[Cfg::kTiles][4];
+            float s[Cfg::kTiles][NT][4];
 #pragma unroll
             for (int i = 0; i < Cfg::kTiles; ++i) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+                for (int e = 0; e < 4 * NT; ++e) s[i][e / 4][e % 4] = 0.f;
                 // lane's K: tokens g and g + 8, bytes 64 c + 16 t .. + 15
                 const unsigned char *row = kt + (16 * i + g) * Cfg::kRow + 16 * t;
 #pragma unroll
@@ -284,7 +289,9 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                         uint32_t a0, a1, a2, a3;
                         e4m3x4_to_h2x2(xw[j], a0, a2);
                         e4m3x4_to_h2x2(yw[j], a1, a3);
-                        mma16816(s[i], a0, a1, a2, a3, qf[c][j][0], qf[c][j][1]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma16816(s[i][nt], a0, a1, a2, a3, qf[nt][c][j][0], qf[nt][c][j][1]);
                     }
                 }
             }
@@ -299,47 +306,57 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                 lv[i] = __log2f(__shfl_sync(0xffffffffu, old ? lvs_old : lvs, n & 31));
                 seen[i] = (old ? there_old : there) >> (n & 31) & 1u;
             }
-            float top[2] = {-kInf, -kInf}, topv[2] = {-kInf, -kInf};
+            float base[NT][2], basev[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float top[2] = {-kInf, -kInf}, topv[2] = {-kInf, -kInf};
+#pragma unroll
+                for (int i = 0; i < Cfg::kTiles; ++i) {
+                    const int tok = tile_at(n0 + i) * 16 + g;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int c = e & 1, at = tok + 8 * (e >> 1);
+                        float &x = s[i][nt][e];
+                        x = seen[i] && at >= lo[nt][c] && at < hi[nt][c] ? x * (factor[nt][c] * sk[i]) : -kInf;
+                        top[c] = fmaxf(top[c], x);
+                        topv[c] = fmaxf(topv[c], x + lv[i]);
+                    }
+                }
+                bool moved = false;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float mn = fmaxf(m[nt][c], max_over_rows(top[c]));
+                    const float vn = fmaxf(mv[nt][c], max_over_rows(topv[c]));
+                    base[nt][c] = mn == -kInf ? 0.f : mn;
+                    basev[nt][c] = vn == -kInf ? 0.f : vn;
+                    l[nt][c] *= ex2(m[nt][c] - base[nt][c]);
+                    moved |= vn != mv[nt][c];
+                    top[c] = ex2(mv[nt][c] - basev[nt][c]);  // O's factor
+                    m[nt][c] = mn;
+                    mv[nt][c] = vn;
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int i = 0; i < Cfg::kM; ++i) {
+                        o[nt][i][0] *= top[0], o[nt][i][2] *= top[0];
+                        o[nt][i][1] *= top[1], o[nt][i][3] *= top[1];
+                    }
+                }
+            }
 #pragma unroll
             for (int i = 0; i < Cfg::kTiles; ++i) {
-                const int tok = tile_at(n0 + i) * 16 + g;
+                uint32_t b0[NT], b1[NT];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int c = e & 1, at = tok + 8 * (e >> 1);
-                    s[i][e] = seen[i] && at >= lo[c] && at < hi[c] ? s[i][e] * (factor[c] * sk[i]) : -kInf;
-                    top[c] = fmaxf(top[c], s[i][e]);
-                    topv[c] = fmaxf(topv[c], s[i][e] + lv[i]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    float pr[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        l[nt][e & 1] += ex2(s[i][nt][e] - base[nt][e & 1]);
+                        pr[e] = ex2(s[i][nt][e] + lv[i] - basev[nt][e & 1]);
+                    }
+                    b0[nt] = transpose8x8(pack_h2(pr[0], pr[1]));
+                    b1[nt] = transpose8x8(pack_h2(pr[2], pr[3]));
                 }
-            }
-            float base[2], basev[2];
-            bool moved = false;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float mn = fmaxf(m[c], max_over_rows(top[c])), vn = fmaxf(mv[c], max_over_rows(topv[c]));
-                base[c] = mn == -kInf ? 0.f : mn;
-                basev[c] = vn == -kInf ? 0.f : vn;
-                l[c] *= ex2(m[c] - base[c]);
-                moved |= vn != mv[c];
-                top[c] = ex2(mv[c] - basev[c]);  // O's factor
-                m[c] = mn;
-                mv[c] = vn;
-            }
-            if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                for (int i = 0; i < Cfg::kM; ++i) {
-                    o[i][0] *= top[0], o[i][2] *= top[0];
-                    o[i][1] *= top[1], o[i][3] *= top[1];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < Cfg::kTiles; ++i) {
-                float pr[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    l[e & 1] += ex2(s[i][e] - base[e & 1]);
-                    pr[e] = ex2(s[i][e] + lv[i] - basev[e & 1]);
-                }
-                const uint32_t b0 = transpose8x8(pack_h2(pr[0], pr[1])), b1 = transpose8x8(pack_h2(pr[2], pr[3]));
                 // lane's V: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9, bytes kVB (8 h + g) .. of each
                 const unsigned char *row = vt + (16 * i + 2 * t) * Cfg::kRow + Cfg::kVB * g;
 #pragma unroll
@@ -364,10 +381,12 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                         e4m3x4_to_h2x2(__byte_perm(w[0][j], w[1][j], 0x7362), a[2], a[3]);
                         e4m3x4_to_h2x2(__byte_perm(w[2][j], w[3][j], 0x5140), b[0], b[1]);
                         e4m3x4_to_h2x2(__byte_perm(w[2][j], w[3][j], 0x7362), b[2], b[3]);
-                        float(&d0)[4] = o[h * (Cfg::kVB / 2) + 2 * j];
-                        float(&d1)[4] = o[h * (Cfg::kVB / 2) + 2 * j + 1];
-                        mma16816(d0, a[0], a[1], b[0], b[1], b0, b1);
-                        mma16816(d1, a[2], a[3], b[2], b[3], b0, b1);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const int d = h * (Cfg::kVB / 2) + 2 * j;
+                            mma16816(o[nt][d], a[0], a[1], b[0], b[1], b0[nt], b1[nt]);
+                            mma16816(o[nt][d + 1], a[2], a[3], b[2], b[3], b0[nt], b1[nt]);
+                        }
                     }
                 }
             }
@@ -385,22 +404,24 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
 
         // ---- merge the warps
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) l[c] += __shfl_xor_sync(0xffffffffu, l[c], x);
-            if (g == 0) {
-                mlm[warp][2 * t + c][0] = m[c];
-                mlm[warp][2 * t + c][1] = l[c];
-                mlm[warp][2 * t + c][2] = mv[c];
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+                if (g == 0) {
+                    float *row = mlm[warp][nt * kRows + 2 * t + c];
+                    row[0] = m[nt][c], row[1] = l[nt][c], row[2] = mv[nt][c];
+                }
             }
-        }
-        // o[..][e]: dim kVB (8 h + g) + 2 j + (e >> 1), row 2 t + (e & 1), for MMA h kVB / 2 + j
+            // o[..][e]: dim kVB (8 h + g) + 2 j + (e >> 1), row 2 t + (e & 1), for MMA h kVB / 2 + j
 #pragma unroll
-        for (int i = 0; i < Cfg::kM; ++i) {
-            const int h = i / (Cfg::kVB / 2), j = i % (Cfg::kVB / 2);
-            float *dst = reinterpret_cast<float *>(ring) + 2 * t * (HD + 4) + Cfg::kVB * (8 * h + g) + 2 * j;
-            *reinterpret_cast<float2 *>(dst) = make_float2(o[i][0], o[i][2]);
-            *reinterpret_cast<float2 *>(dst + HD + 4) = make_float2(o[i][1], o[i][3]);
+            for (int i = 0; i < Cfg::kM; ++i) {
+                const int h = i / (Cfg::kVB / 2), j = i % (Cfg::kVB / 2);
+                float *dst = reinterpret_cast<float *>(ring) + (nt * kRows + 2 * t) * (HD + 4) + Cfg::kVB * (8 * h + g) + 2 * j;
+                *reinterpret_cast<float2 *>(dst) = make_float2(o[nt][i][0], o[nt][i][2]);
+                *reinterpret_cast<float2 *>(dst + HD + 4) = make_float2(o[nt][i][1], o[nt][i][3]);
+            }
         }
         __syncthreads();
         const int slot = wk.slot(cta);
@@ -427,7 +448,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                          hq * p.out_head + d;
                 store_out4(dst, acc.x, acc.y, acc.z, acc.w);
             } else {
-                const int64_t at = static_cast<int64_t>(slot) * kRows + r;
+                const int64_t at = static_cast<int64_t>(slot) * NT * kRows + r;
                 *reinterpret_cast<float4 *>(p.part.o + at * HD + d) = acc;
                 if (d == 0) *reinterpret_cast<float2 *>(p.part.ml + 2 * at) = make_float2(mm, ll);
             }
@@ -581,9 +602,11 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
     }
 }
 
-// Rows of a sequence and kv head up to which the rows kernel is taken (its tiles of 8 read the cache again, from L2).
-// Measured against the prompt kernel on five shapes of 20 to 160 MB of cache: at 16 rows 31 to 45 us against 42 to 78,
-// at 32 rows 38 to 60 against 43 to 80, at 48 rows 47 to 82 against 44 to 79, at 64 rows 56 to 99 against 45 to 81.
+// Rows of a sequence and kv head up to which the rows kernel is taken (its further tiles read the cache again, from
+// L2).  Measured against the prompt kernel on five shapes of 20 to 160 MB of cache: at 16 rows 29 to 39 us against 42
+// to 78, at 32 rows 38 to 54 against 43 to 80, at 48 rows 47 to 71 against 39 to 68, at 64 rows 56 to 81 against 40 to 69.
+// Tiles of 16 rows instead of 8 (head dims 64 and 128; at 256 their sums spill: 52 us against 37): at 16 rows 29 to 39 us
+// against 31 to 45.
 constexpr int kRowsMost = 32;
 // CTAs per SM of the rows kernel: registers allow two of 128 threads.
 constexpr int kRowsPerSm = 2;
@@ -594,12 +617,18 @@ cudaError_t sm_count(int *sms) {
     return e != cudaSuccess ? e : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
 }
 
+template <int HD, int NT, typename T>
+cudaError_t launch_tiles(const AttnArgs &p, int ctas, cudaStream_t s) {
+    const size_t smem = RowsCfg<HD>::kSmem;
+    const cudaError_t e = cudaFuncSetAttribute(kv8_rows_kernel<HD, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    return e != cudaSuccess ? e : launch_behind(kv8_rows_kernel<HD, NT, T>, dim3(ctas), kThreads, smem, s, p);
+}
 template <int HD, typename T>
 cudaError_t launch_rows(const AttnArgs &p, int ctas, cudaStream_t s) {
-    const size_t smem = RowsCfg<HD>::kSmem;
-    const cudaError_t e = cudaFuncSetAttribute(kv8_rows_kernel<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
-    return e != cudaSuccess ? e : launch_behind(kv8_rows_kernel<HD, T>, dim3(ctas), kThreads, smem, s, p);
+    if constexpr (HD <= 128)
+        if (p.a.rows == 2 * kRows) return launch_tiles<HD, 2, T>(p, ctas, s);
+    return launch_tiles<HD, 1, T>(p, ctas, s);
 }
 template <typename T>
 cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {
@@ -608,7 +637,7 @@ cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, int sms, cudaStr
 }
 template <typename T>
 cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {
-    const cudaError_t e = p.a.rows != kRows
+    const cudaError_t e = p.a.rows > 2 * kRows
                               ? launch_prompt(p, hd, std::is_same<T, __half>::value, ctas, s)
                           : hd == 64  ? launch_rows<64, T>(p, ctas, s)
                           : hd == 128 ? launch_rows<128, T>(p, ctas, s)
@@ -627,7 +656,8 @@ cudaError_t plan_of(int hd, int group, int max_q, Plan *pl) {
     if (e != cudaSuccess) return e;
     const bool prompt = static_cast<int64_t>(max_q) * group > kRowsMost;
     pl->sms = sms;
-    pl->rows = prompt ? prompt_rows(hd) : kRows;
+    const bool two = hd <= 128 && static_cast<int64_t>(max_q) * group > kRows;  // the sums of 16 rows of 256 dims spill
+    pl->rows = prompt ? prompt_rows(hd) : two ? 2 * kRows : kRows;
     pl->unit = prompt ? kPromptUnit : kUnit;
     pl->extra = prompt ? kPromptExtra : 0;
     pl->ctas = prompt ? sms : sms * kRowsPerSm;
