@@ -281,13 +281,18 @@ mg_status mg_tp_disconnect(mg_model *m);
  * All of it is read on the device when the kernels run, so a captured call may
  * be replayed with new lengths, tables and rows within those bounds.
  *
- * err_dev is a device word that receives a nonzero code (the first one stays)
- * when a length breaks the bounds or a page id is outside [0, num_pages): the
- * tokens concerned are then neither stored nor seen; nothing outside the
- * tensors is touched.
+ * err_dev is a device word that receives a nonzero code (the first one stays):
+ * MG_KV8_ERR_LENGTHS when a length breaks the bounds (the sequence's tokens are
+ * not stored and its queries answer 0), MG_KV8_ERR_PAGE when a page id that is
+ * needed is outside [0, num_pages) (its tokens are neither stored nor seen);
+ * nothing outside the tensors is touched.  MG_KV8_ERR_WAIT: a bounded wait
+ * inside a kernel expired and the call's answers are not complete.
  * Both calls run on `stream` (a cudaStream_t of the current device; NULL: the
  * legacy default stream) without allocating or synchronising. */
 #define MG_KV8_BLOCK 16
+#define MG_KV8_ERR_LENGTHS 0x70000u
+#define MG_KV8_ERR_PAGE 0x80000u
+#define MG_KV8_ERR_WAIT 0x90000u
 typedef struct mg_kv8_cache {
     int32_t struct_size; /* sizeof(mg_kv8_cache) */
     int32_t num_pages, page_size, num_kv_heads, head_dim;
@@ -343,7 +348,7 @@ mg_status mg_kv8_append(const mg_kv8_cache *cache, const mg_kv8_batch *batch, co
  * multiple of num_kv_heads, at most 128 per kv head; rows as above with strides
  * in multiples of 8 elements and 16-byte aligned data.
  * V codes must be finite (the append writes no others); the cache's content
- * behind ctx_len is never used.
+ * behind ctx_len is never used, nor are pages that lie before every window.
  * The workspace (16-byte aligned, mg_kv8_attention_workspace bytes on this
  * device for these cache dimensions and bounds) needs no initial value and
  * keeps nothing between calls: calls that may overlap need one each. */

@@ -19,7 +19,7 @@ mg_status report_error(mg_status st, const char *msg);
 namespace kv8 {
 
 constexpr int kBlock = MG_KV8_BLOCK;  // tokens per scale
-constexpr uint32_t kErrLens = 0x70000u, kErrPage = 0x80000u;  // err_dev codes: bad lengths, bad page id
+constexpr uint32_t kErrLens = MG_KV8_ERR_LENGTHS, kErrPage = MG_KV8_ERR_PAGE, kErrWait = MG_KV8_ERR_WAIT;
 
 // The cache and the batch as the kernels see them.
 struct Cache {

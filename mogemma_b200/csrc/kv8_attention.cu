@@ -2,9 +2,9 @@
 // (the attention of layers.mojo:63-94), for few query rows per kv head; the
 // combine of partial answers; and the entry points.
 //
-// kv8_rows_kernel takes items of up to 8 or 16 query rows.  It is bound by reading
-// the cache: one code byte feeds few rows' products, so the legacy warp-level
-// MMA is fast enough.  A warp takes 16 tokens (one scale block) at a time and
+// kv8_rows_kernel takes items of up to 8 or 16 query rows.  It is bound by
+// reading the cache: one code byte feeds few rows' products, so the legacy
+// warp-level MMA is fast enough.  A warp takes 16 tokens (one scale block) at a time and
 // computes transposed products, tokens and head dims on the MMA's 16 rows, the
 // query rows on its 8 columns:
 //   S^T[16 tokens][8 rows] = K . Q^T     A = K codes, widened to fp16 (exact)
@@ -16,8 +16,8 @@
 // S^T's accumulator layout transposes into P^T's operand layout by movmatrix.
 //
 // Every warp has a ring of its own in shared memory, filled by asynchronous
-// 16-byte copies kStages - 1 steps (8 KB each, hd 64: 4 KB) ahead, and nothing but its own
-// copies to wait for; token rows are padded by 16 bytes, so that the fragments'
+// 16-byte copies kStages - 1 steps (8 KB each, hd 64: 4 KB) ahead, and nothing
+// but its own copies to wait for; token rows are padded by 16 bytes, so that the fragments'
 // loads meet no bank twice.  With the codes in registers instead, one step
 // ahead, 64 KB per SM at most were in flight: 4.3 TB/s on 1.37 GB of cache
 // where the ring reaches 5.8.
@@ -466,7 +466,6 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
 // Tasks (item, rows, dims) are dealt over a fixed grid; the order of the sums
 // is that of the CTAs, the same every time.
 constexpr int kCombThreads = 256;
-constexpr int kFewParts = 8;
 constexpr int kCombPerSm = 4;
 
 struct Joined {  // a running join of parts
@@ -483,7 +482,7 @@ struct Joined {  // a running join of parts
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArgs p, int hd, int ctas) {
+__global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArgs p, int hd, int ctas, int few) {
     extern __shared__ int sm_i[];  // [ctas] tasks of the entries before this one
     __shared__ int warp_n[kCombThreads / 32];
     __shared__ float4 acc_s[kCombThreads / 32][4];
@@ -497,7 +496,7 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
         int mine = 0;
         if (i < ctas) {
             const Split sp = p.part.split[i];
-            if (sp.nrows > 0) mine = sp.last_cta - i < kFewParts ? (sp.nrows + 15) / 16 : sp.nrows * fine;
+            if (sp.nrows > 0) mine = sp.last_cta - i < few ? (sp.nrows + 15) / 16 : sp.nrows * fine;
         }
         int upto = mine;
 #pragma unroll
@@ -531,7 +530,7 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
         }
         const Split sp = p.part.split[first];
         const int sub = task - sm_i[first], n = sp.last_cta - first + 1;
-        if (n <= kFewParts) {  // 16 lanes hold a row, lane gl dims 64 c + 4 gl ..
+        if (n <= few) {  // 16 lanes hold a row, lane gl dims 64 c + 4 gl ..
             const int r = 16 * sub + grp;
             if (r >= sp.nrows) continue;
             Joined j[4];
@@ -632,8 +631,11 @@ cudaError_t launch_rows(const AttnArgs &p, int ctas, cudaStream_t s) {
 }
 template <typename T>
 cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {
+    // parts up to which an item is joined by rows: more where there are many items to fill the grid with (48 items of 6
+    // to 9 parts: 40 us -> 37 with 16; one item of 10 parts: 2 us slower with 16 than with 8)
+    const int few = static_cast<int64_t>(p.b.batch) * p.a.tiles * p.c.heads >= 32 ? 16 : 8;
     return launch_behind(kv8_combine_kernel<T>, dim3(kCombPerSm * sms), kCombThreads,
-                         sizeof(int) * static_cast<size_t>(ctas), s, p, hd, ctas);
+                         sizeof(int) * static_cast<size_t>(ctas), s, p, hd, ctas, few);
 }
 template <typename T>
 cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {
@@ -734,7 +736,9 @@ extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_ba
     AttnArgs p;
     p.c = cache_of(cache);
     p.b = batch_of(batch);
-    p.a = AttnShape{group, pl.rows, pl.tiles, args->window, pl.unit, pl.extra};
+    // a window that reaches every position is none (and no position less it underflows)
+    const int window = args->window >= batch->max_ctx ? 0 : args->window;
+    p.a = AttnShape{group, pl.rows, pl.tiles, window, pl.unit, pl.extra};
     p.part = partials_at(args->workspace_dev, pl.ctas, pl.rows);
     p.q = args->q_dev, p.out = args->out_dev;
     p.q_row = args->q_row_stride, p.q_head = args->q_head_stride;

@@ -38,8 +38,8 @@
 // the S it was made from; the tensor pipe runs one thread's MMAs in order, so
 // the next S on a stage lands after P V has read P.  K and V have two stages
 // each (hd 256: one; S and P V alternate, and either is reloaded under the
-// other).  O is rescaled only when M grows by more than 8 (P stays below 2^8,
-// within fp16's range).  A row tile takes no part in units that none of its
+// other).  O is rescaled only when m or M grows by more than 15 (P stays below
+// 2^15, within fp16's range).  A row tile takes no part in units that none of its
 // rows see.
 //
 // Units of 64 tokens were the first form: N = 64 reads Q from shared memory for
@@ -60,7 +60,6 @@ namespace {
 constexpr int kM = 128;   // rows of a tile
 constexpr int kN = 128;   // tokens of a unit
 constexpr int kThreads = 640;
-constexpr uint32_t kErrWait = 0x90000u;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kRescale = 15.0f;  // P stays below 2^15, within fp16
 constexpr int kRing = 4;  // units whose scales are at hand

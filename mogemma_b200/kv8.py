@@ -30,6 +30,9 @@ import torch
 from . import _core
 
 BLOCK = 16  # tokens per scale (MG_KV8_BLOCK)
+# MG_KV8_ERR_*
+_ERRORS = {0x70000: "lengths out of bounds", 0x80000: "page id out of range",
+           0x90000: "a device wait ran out; the answers are not complete"}
 _TYPES = {torch.float32: _core.MG_F32, torch.bfloat16: _core.MG_BF16, torch.float16: _core.MG_F16}
 
 
@@ -119,8 +122,7 @@ class KV8Batch:
         code = int(self.err.item())
         if code:
             self.err.zero_()
-            msg = "page id out of range" if code == 0x80000 else f"lengths out of bounds (0x{code:x})"
-            raise RuntimeError(f"8-bit cache: {msg}")
+            raise RuntimeError(f"8-bit cache: {_ERRORS.get(code, f'error word 0x{code:x}')}")
 
     def _desc(self, total_q: int) -> _core.KV8BatchDesc:
         # a single row may report any stride

@@ -472,3 +472,39 @@ def test_attention_of_items_of_many_sizes(dim, seed) -> None:
     window = r.choice([0, 0, 40, 200])
     out = w.cache.attention(w.batch, q, window=window)
     _check_attention(w, q, out, scale=dim**-0.5, window=window)
+
+
+@pytest.mark.parametrize("n", [1, 9, 40])
+def test_pages_before_the_window_may_be_gone(n) -> None:
+    w = World([(n, 700), (n, 333)], kv_heads=2, dim=128, page=16)
+    q = w.rand(w.rows, 4, 128, dtype=BF16)
+    window = 100
+    want = w.cache.attention(w.batch, q, window=window)
+    for b, (_, ctx) in enumerate(w.lens):
+        w.batch.page_table[b, : (ctx - n + 1 - window) // 16] = -1
+    out = w.cache.attention(w.batch, q, window=window)
+    w.batch.check()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("n", [1, 9, 40])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_negative_and_zero_scales(n, scale) -> None:
+    w = World([(n, 200), (n, 77)], kv_heads=2, dim=64, page=32)
+    q = w.rand(w.rows, 6, 64, dtype=F16)
+    out = w.cache.attention(w.batch, q, scale=scale)
+    _check_attention(w, q, out, scale=scale, window=0)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_windows_as_long_as_can_be(n) -> None:
+    """A window of 2^31 - 1 is none, also for a sequence whose lengths are refused."""
+    w = World([(n, 200), (n, 77)], kv_heads=1, dim=64, page=32)
+    q = w.rand(w.rows, 2, 64, dtype=F16)
+    want = w.cache.attention(w.batch, q)
+    assert torch.equal(w.cache.attention(w.batch, q, window=2**31 - 1), want)
+    w.batch.ctx_len[1] = n - 1
+    out = w.cache.attention(w.batch, q, window=2**31 - 1)
+    with pytest.raises(RuntimeError, match="lengths"):
+        w.batch.check()
+    assert torch.equal(out[:n], want[:n]) and bool((out[n:] == 0).all())
