@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[kRing], q_full[2], pair_bar[4][2], q_pair[4];
     __shared__ __align__(8) uint64_t item_full[kItems], item_empty[kItems];
     __shared__ __align__(8) uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [tile][S stage]
+    __shared__ __align__(8) uint64_t drained[2];  // a tile's MMAs have all run
     __shared__ Desc items_s[kItems];
     __shared__ __align__(16) float sc_k[kRing][8], sc_v[kRing][8];  // scales of a unit's eight blocks: K, log2 of V
     __shared__ __align__(8) uint8_t sc_ok[kRing][8];
@@ -279,6 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                 mbar_init(&p_full[g][i], C::kTwo ? 4 : 8);
                 mbar_init(&pv_done[g][i], 1);
             }
+            mbar_init(&drained[i], 1);
         }
         for (int i = 0; i < kRing; ++i) mbar_init(&sc_full[i], 8);
         for (int i = 0; i < kItems; ++i) {
@@ -394,6 +396,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             __syncwarp();
             if (lane == 0) mbar_arrive(&item_empty[i % kItems]);
         }
+        commit(&drained[g]);  // after a wait that ran out MMAs may be in flight: TMEM and shared memory are held for them
+        volatile int never = 0;
+        wait(&drained[g], 0, &never, err);
     } else if (warp == 18) {  // ---- walker
         if (lane == 0) {
             Walk wk;
