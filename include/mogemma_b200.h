@@ -323,7 +323,8 @@ typedef struct mg_kv8_batch {
  * stored as a key of NaN and a value of zero: every query that sees it answers
  * NaN, and no other query or token is affected.
  * q (num_heads of them, a multiple of num_kv_heads) may be absent: num_heads 0.
- * q_out may be q itself.  Two tokens of one call must not share a cache slot,
+ * q_out may be q itself (with its dtype and strides); else it overlaps no other
+ * tensor of the call.  Two tokens of one call must not share a cache slot,
  * nor two sequences a block that the call writes.  Rows: element (row, head, d)
  * at row * row_stride + head * head_stride + d (in elements, multiples of 4;
  * data aligned to 4 elements).  dtype: MG_F32, MG_BF16 or MG_F16; out_dtype
@@ -347,6 +348,7 @@ mg_status mg_kv8_append(const mg_kv8_cache *cache, const mg_kv8_batch *batch, co
  * nothing answers 0.  dtype of q and out: MG_BF16 or MG_F16; num_heads a
  * multiple of num_kv_heads, at most 128 per kv head; rows as above with strides
  * in multiples of 8 elements and 16-byte aligned data.
+ * out overlaps no other tensor of the call, q neither.
  * V codes must be finite (the append writes no others); the cache's content
  * behind ctx_len is never used, nor are pages that lie before every window.
  * The workspace (16-byte aligned, mg_kv8_attention_workspace bytes on this

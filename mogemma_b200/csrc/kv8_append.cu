@@ -493,6 +493,10 @@ extern "C" mg_status mg_kv8_append(const mg_kv8_cache *cache, const mg_kv8_batch
     if (in % in_align != 0 || out % out_align != 0 || strides % 4 != 0 || tables % 16 != 0)
         return report_error(MG_ERR_INVALID, "mg_kv8_append: rows must be aligned to 4 elements and their strides "
                                             "multiples of 4; norms and cos / sin aligned to 16 bytes");
+    if (args->num_heads > 0 && args->q_out_dev == args->q_dev &&
+        (args->out_dtype != args->dtype || args->out_row_stride != args->q_row_stride ||
+         args->out_head_stride != args->q_head_stride))
+        return report_error(MG_ERR_INVALID, "mg_kv8_append: q_out may be q only with its dtype and strides");
     AppendParams p;
     p.c = cache_of(cache);
     p.b = batch_of(batch);

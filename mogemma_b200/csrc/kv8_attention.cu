@@ -725,6 +725,8 @@ extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_ba
         ((args->q_row_stride | args->q_head_stride | args->out_row_stride | args->out_head_stride) % 8) != 0)
         return report_error(MG_ERR_INVALID,
                             "mg_kv8_attention: q and out must be 16-byte aligned with strides in multiples of 8");
+    // a part of an item may read a row that another part has answered already
+    if (args->q_dev == args->out_dev) return report_error(MG_ERR_INVALID, "mg_kv8_attention: out must not be q");
     const int group = args->num_heads / cache->num_kv_heads;
     Plan pl;
     cudaError_t e = plan_of(cache->head_dim, group, batch->max_q, &pl);

@@ -15,8 +15,9 @@ object they return launches the call each time it is called (on torch's current
 stream of the cache's device), so a decode loop that keeps its buffers pays for
 the checks once.  A bound call reads the tensors' contents anew every time: new
 rows, lengths and tables are written into the same tensors.  It may be captured
-into a CUDA graph.  An attention call has a workspace of its own unless one is
-given; calls that may run at the same time must not share one.
+into a CUDA graph; the call object then has to live as long as the graph.  An
+attention call has a workspace of its own unless one is given; calls that may
+run at the same time must not share one.
 """
 
 from __future__ import annotations
@@ -44,6 +45,11 @@ _raw_stream: Callable[[int], int] = getattr(torch._C, "_cuda_getCurrentRawStream
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+def _i32(x: int) -> int:
+    """An int32 field's value; what it cannot hold becomes its nearest end, not the low bits."""
+    return min(max(int(x), -(2**31)), 2**31 - 1)
 
 
 def _rows(name: str, x: torch.Tensor, device: torch.device, dim: int) -> torch.Tensor:
@@ -113,7 +119,7 @@ class KV8Batch:
         _need(q_start.shape[0] == n + 1 and page_table.shape[0] == n,
               "q_start has batch + 1 entries, page_table one row per sequence")
         self.q_start, self.ctx_len, self.page_table = q_start, ctx_len, page_table
-        self.max_q, self.max_ctx = int(max_q), int(max_ctx)
+        self.max_q, self.max_ctx = _i32(max_q), _i32(max_ctx)
         self.device = q_start.device
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
 
@@ -128,8 +134,7 @@ class KV8Batch:
         # a single row may report any stride
         width = self.page_table.shape[1] if self.ctx_len.shape[0] == 1 else self.page_table.stride(0)
         return _core.KV8BatchDesc(
-            ctypes.sizeof(_core.KV8BatchDesc), self.ctx_len.shape[0], total_q, self.max_q,
-            min(self.max_ctx, 2**31 - 1), 0, self.q_start.data_ptr(), self.ctx_len.data_ptr(),
+            ctypes.sizeof(_core.KV8BatchDesc), self.ctx_len.shape[0], _i32(total_q), self.max_q, self.max_ctx, 0, self.q_start.data_ptr(), self.ctx_len.data_ptr(),
             self.page_table.data_ptr(), width, self.err.data_ptr())
 
 
@@ -198,6 +203,8 @@ class KV8Cache:
             _need(q.dtype == k.dtype and q.shape == q_out.shape and q.shape[0] == k.shape[0],
                   "q must have the rows and type of k, and q_out the shape of q")
             _written("q_out", q_out)
+            _need(q_out.data_ptr() != q.data_ptr() or (q_out.dtype == q.dtype and _strides(q_out) == _strides(q)),
+                  "q_out may be q only with its dtype and strides")
             heads, out_dtype = q.shape[1], q_out.dtype
         length = 0
         if cos is not None:
@@ -235,13 +242,14 @@ class KV8Cache:
         _rows("out", out, self.device, d)
         _need(q.shape == out.shape and q.dtype == out.dtype, "out must have the shape and type of q")
         _written("out", out)
+        _need(q.data_ptr() != out.data_ptr(), "out must not be q")
         size = self.workspace_bytes(batch, q.shape[1])
         if workspace is None:
             workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
         _need(workspace.dtype == torch.uint8 and workspace.device == self.device and workspace.is_contiguous(),
               f"workspace must be a contiguous uint8 tensor on {self.device}")
         args = _core.KV8AttentionArgs(
-            ctypes.sizeof(_core.KV8AttentionArgs), _TYPES[q.dtype], q.shape[1], int(window),
+            ctypes.sizeof(_core.KV8AttentionArgs), _TYPES[q.dtype], q.shape[1], _i32(window),
             d ** -0.5 if scale is None else float(scale), 0, q.data_ptr(), out.data_ptr(), *_strides(q),
             *_strides(out), workspace.data_ptr(), workspace.numel())
         return KV8Call(_core.lib().mg_kv8_attention, self.device, (self._c, self._batch(batch, q.shape[0]), args),

@@ -441,6 +441,7 @@ def test_bad_tensors_are_refused() -> None:
             (lambda: c.append(b, k, v, q=q, q_out=torch.empty(3, 1, 64, dtype=BF16, device="cuda").expand(3, 4, 64)),
              "overlap"),
             (lambda: c.attention(b, q, q.half()), "shape and type"),
+            (lambda: c.attention(b, q, q), "must not be q"),
             (lambda: c.attention(b, q.float()), "dtype"),
             (lambda: c.attention(b, q[:, :3]), "multiple"),
             (lambda: c.attention(b, q.transpose(1, 2)), "contiguous"),

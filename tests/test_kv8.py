@@ -126,6 +126,14 @@ def test_bad_attentions_are_refused(more, status, text) -> None:
     _refused(LIB.mg_kv8_attention, _cache(), _batch(), _attention(**more), status, text)
 
 
+def test_answers_over_the_queries_are_refused() -> None:
+    """Attention answers a row while other CTAs may still read it; the append may, but only element for element."""
+    _refused(LIB.mg_kv8_attention, _cache(), _batch(), _attention(), INVALID, "out must not be q")
+    text = "q_out may be q only"
+    _refused(LIB.mg_kv8_append, _cache(), _batch(), _append(out_row_stride=128), INVALID, text)
+    _refused(LIB.mg_kv8_append, _cache(), _batch(), _append(dtype=_core.MG_F32), INVALID, text)
+
+
 def test_null_arguments_are_refused() -> None:
     c, b = ctypes.byref(_cache()), ctypes.byref(_batch())
     assert LIB.mg_kv8_append(None, b, ctypes.byref(_append()), None) == INVALID
