@@ -313,7 +313,8 @@ typedef struct mg_kv8_batch {
 /* Appends the batch's new keys and values, rotating on the way:
  *   q_out = rope(norm(q)),  K <- rope(norm(k)),  V <- v   (fp32 arithmetic)
  * norm(x) = x * rsqrt(mean(x^2) + 1e-6) * (1 + w) with q_norm / k_norm as w
- * ([head_dim]; NULL: no norm); rope turns the pairs (i, i + head_dim / 2) by the
+ * ([head_dim]; NULL: no norm; a head whose mean square passes fp32's range
+ * becomes 0, as the formula in fp32 has it); rope turns the pairs (i, i + head_dim / 2) by the
  * position's row of cos / sin ([rope_len][head_dim / 2]; both NULL: no rotation;
  * rope_len >= max_ctx).
  * A block's scale becomes the smallest power of two (at least 2^-100) that

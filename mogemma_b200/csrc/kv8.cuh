@@ -274,9 +274,5 @@ struct AttnArgs {
     int64_t q_row, q_head, out_row, out_head;
     float scale_log2;  // scale * log2(e)
 };
-
-
-
-
 }  // namespace kv8
 }  // namespace mg

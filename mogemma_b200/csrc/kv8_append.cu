@@ -17,6 +17,13 @@
 // it costs is latency, so a token's K, V, q heads, cos and sin rows are all
 // loaded before the first is used, and the page id and old scales, which only
 // the stores need, are not waited for earlier.
+//
+// Measured (launches in a graph; a plain copy on this GPU reaches 6.46 TB/s):
+// one token of 4 q and 1 kv heads of 256, 3.5 us, bound by the launch (4.8 in
+// the block form); 128 tokens of 32 and 16 heads of 128 in fp16, 3.8 us (12.6
+// in the block form); 7500 fp32 prompt tokens of 8 and 4 heads of 256, 32 us,
+// 4.1 TB/s; one prompt of 16384 bf16 tokens of 32 and 16 heads of 128, 96 us,
+// 5.0 TB/s (43 and 133 us while a token's rows were loaded one after another).
 #include "kv8.cuh"
 
 #include <cstdio>

@@ -22,6 +22,12 @@
 // ahead, 64 KB per SM at most were in flight: 4.3 TB/s on 1.37 GB of cache
 // where the ring reaches 5.8.
 //
+// Measured (in a graph, with the combine): 32 tokens over 16384 positions each,
+// 32 / 16 heads of 128, 235 us, 5.8 TB/s; one token over 131072 positions, 4 / 1
+// heads of 256, 24 us, 2.8 TB/s; one over 640 positions, 9.7 us, which is
+// latency alone: two launches, the scan for a CTA's place, the page look-up, two
+// steps and the join.
+//
 // With s = scale log2(e) k_scale <q, k> the state per row is m = max s,
 // l = sum 2^(s - m) and the sum of P V with P = 2^(s + log2 v_scale - M),
 // M = max(s + log2 v_scale): the value scale rides in the exponent, so that P
