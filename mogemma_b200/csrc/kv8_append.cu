@@ -309,6 +309,7 @@ __device__ __forceinline__ int seq_of_block(const Batch &b, int index, int &base
     if (threadIdx.x == 0) found = -1;
     __syncthreads();
     for (int i = threadIdx.x; i < b.batch; i += blockDim.x) {
+        if (index == 0) load_seq(b, i, true);  // starts that fall back may leave their sequence no index to be seen at
         const int a = min(max(b.q_start[i], 0), b.total_q), e = min(max(b.q_start[i + 1], a), b.total_q);
         if (index >= a / kBlock + 2 * i && index < e / kBlock + 2 * (i + 1)) atomicMax(&found, i);
     }

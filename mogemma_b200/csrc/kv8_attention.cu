@@ -31,7 +31,7 @@
 // With s = scale log2(e) k_scale <q, k> the state per row is m = max s,
 // l = sum 2^(s - m) and the sum of P V with P = 2^(s + log2 v_scale - M),
 // M = max(s + log2 v_scale): the value scale rides in the exponent, so that P
-// is at most 1 whatever the scales, and fp16 holds it to 2^-12.
+// is at most 1 whatever the scales, and fp16 holds it to 2^-11.
 #include <cstdio>
 #include <type_traits>
 

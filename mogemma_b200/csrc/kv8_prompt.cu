@@ -13,7 +13,7 @@
 // block scales of K multiply the score columns, those of V ride in P's
 // exponent: with s = scale log2(e) k_scale <q, k>, m = max s and
 // M = max(s + log2 v_scale), P = 2^(s + log2 v_scale - M) and l = sum 2^(s - m),
-// so P is bounded whatever the scales and fp16 holds it to 2^-12.
+// so P is bounded whatever the scales and fp16 holds it to 2^-11.
 //
 // Warps of a CTA (640 threads, one CTA per SM):
 //  * warps 0-7: softmax.  Two row tiles: warpgroup g has tile g, a row per

@@ -509,3 +509,13 @@ def test_windows_as_long_as_can_be(n) -> None:
     with pytest.raises(RuntimeError, match="lengths"):
         w.batch.check()
     assert torch.equal(out[:n], want[:n]) and bool((out[n:] == 0).all())
+
+
+def test_append_reports_starts_that_fall_back() -> None:
+    """The second sequence starts behind its end, in rows that the third one claims; blocks are found by rows."""
+    w = World([(60, 60), (50, 50), (60, 60)], kv_heads=1, dim=64, page=64, max_q=1000)
+    w.batch.q_start.copy_(_ints([0, 100, 50, 120]))
+    k, v = (w.rand(w.rows, 1, 64) for _ in range(2))
+    w.cache.append(w.batch, k, v)
+    with pytest.raises(RuntimeError, match="lengths"):
+        w.batch.check()
