@@ -277,7 +277,9 @@ mg_status mg_tp_disconnect(mg_model *m);
  * i-th new token is at position ctx_len[b] - q_len[b] + i.  Position p lives in
  * page page_table[b * table_stride + p / page_size].  max_q and max_ctx bound
  * every q_len and ctx_len (host values: the device arrays are not read on the
- * host); max_ctx <= table_stride * page_size.
+ * host); max_ctx <= table_width * page_size, where table_width counts the page ids that
+ * may be read of a sequence (0: table_stride; less where the table's rows are
+ * part of wider ones).
  * All of it is read on the device when the kernels run, so a captured call may
  * be replayed with new lengths, tables and rows within those bounds.
  *
@@ -304,9 +306,9 @@ typedef struct mg_kv8_cache {
 typedef struct mg_kv8_batch {
     int32_t struct_size; /* sizeof(mg_kv8_batch) */
     int32_t batch, total_q, max_q, max_ctx;
-    int32_t reserved0;
+    int32_t table_width; /* page ids of a sequence; 0: table_stride */
     const int32_t *q_start_dev, *ctx_len_dev, *page_table_dev;
-    int64_t table_stride; /* page ids per sequence */
+    int64_t table_stride; /* page ids from a sequence's first to the next one's */
     uint32_t *err_dev;
 } mg_kv8_batch;
 

@@ -126,7 +126,7 @@ class KV8BatchDesc(ctypes.Structure):
     """``mg_kv8_batch``."""
 
     _fields_ = [(n, ctypes.c_int32) for n in (
-        "struct_size", "batch", "total_q", "max_q", "max_ctx", "reserved0")] + [
+        "struct_size", "batch", "total_q", "max_q", "max_ctx", "table_width")] + [
         (n, ctypes.c_void_p) for n in ("q_start_dev", "ctx_len_dev", "page_table_dev")] + [
         ("table_stride", ctypes.c_int64), ("err_dev", ctypes.c_void_p)]
 

@@ -446,8 +446,9 @@ mg_status check_cache_batch(const char *who, const mg_kv8_cache *c, const mg_kv8
         return bad(MG_ERR_INVALID, "need batch, total_q, max_q, max_ctx and table_stride > 0");
     if (b->batch > (1 << 20) || b->total_q > (1 << 28) || b->max_q > (1 << 22) || b->max_ctx > (1 << 28))
         return bad(MG_ERR_UNSUPPORTED, "batch, total_q, max_q or max_ctx too large");
-    if (b->max_ctx > b->table_stride * c->page_size)
-        return bad(MG_ERR_INVALID, "max_ctx exceeds the page table (table_stride * page_size)");
+    if (b->table_width < 0) return bad(MG_ERR_INVALID, "need table_width >= 0");
+    if (b->max_ctx > (b->table_width > 0 ? b->table_width : b->table_stride) * c->page_size)
+        return bad(MG_ERR_INVALID, "max_ctx exceeds the page table (its width * page_size)");
     if (!b->q_start_dev || !b->ctx_len_dev || !b->page_table_dev || !b->err_dev)
         return bad(MG_ERR_INVALID, "null batch pointer");
     return MG_OK;

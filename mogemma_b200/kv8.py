@@ -131,11 +131,12 @@ class KV8Batch:
             raise RuntimeError(f"8-bit cache: {_ERRORS.get(code, f'error word 0x{code:x}')}")
 
     def _desc(self, total_q: int) -> _core.KV8BatchDesc:
-        # a single row may report any stride
-        width = self.page_table.shape[1] if self.ctx_len.shape[0] == 1 else self.page_table.stride(0)
+        # the table may be some columns of a wider one; a single row may report any stride
+        n, width = self.page_table.shape
         return _core.KV8BatchDesc(
-            ctypes.sizeof(_core.KV8BatchDesc), self.ctx_len.shape[0], _i32(total_q), self.max_q, self.max_ctx, 0, self.q_start.data_ptr(), self.ctx_len.data_ptr(),
-            self.page_table.data_ptr(), width, self.err.data_ptr())
+            ctypes.sizeof(_core.KV8BatchDesc), n, _i32(total_q), self.max_q, self.max_ctx, _i32(width),
+            self.q_start.data_ptr(), self.ctx_len.data_ptr(), self.page_table.data_ptr(),
+            width if n == 1 else self.page_table.stride(0), self.err.data_ptr())
 
 
 class KV8Cache:

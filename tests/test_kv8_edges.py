@@ -1,0 +1,45 @@
+"""Edges of the 8-bit paged cache's entry points, without a GPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+from test_kv8 import INVALID, LIB, P, _append, _attention, _batch, _cache, _refused
+
+torch = pytest.importorskip("torch")
+
+from mogemma_b200.kv8 import KV8Batch  # noqa: E402
+
+
+@pytest.mark.parametrize(("more", "ok"), [
+    ({"table_stride": 100, "table_width": 2}, False),  # 2 pages of 32 hold 64 of the 96 positions
+    ({"table_stride": 100, "table_width": 3}, True),
+    ({"table_stride": 3, "table_width": 0}, True),
+    ({"table_stride": 100, "table_width": -1}, False),
+])
+def test_max_ctx_is_held_to_the_tables_width(more, ok) -> None:
+    """Of a table that is some columns of a wider one, the pitch says nothing about the ids that belong to a sequence."""
+    n = ctypes.c_int64()
+    if ok:  # past the batch's checks: refused for its heads
+        _refused(LIB.mg_kv8_attention, _cache(), _batch(**more), _attention(num_heads=5), INVALID, "num_heads")
+        return
+    text = "table_width" if more["table_width"] < 0 else "page table"
+    _refused(LIB.mg_kv8_append, _cache(), _batch(**more), _append(), INVALID, text)
+    _refused(LIB.mg_kv8_attention, _cache(), _batch(**more), _attention(), INVALID, text)
+    assert LIB.mg_kv8_attention_workspace(ctypes.byref(_cache()), ctypes.byref(_batch(**more)), 4,
+                                          ctypes.byref(n)) == INVALID
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+def test_a_column_slice_of_a_table_gives_its_own_width(rows) -> None:
+    wide = torch.zeros(rows, 50, dtype=torch.int32)
+    batch = KV8Batch.__new__(KV8Batch)  # its constructor wants CUDA tensors; the description reads no contents
+    batch.q_start, batch.ctx_len = torch.zeros(rows + 1, dtype=torch.int32), torch.zeros(rows, dtype=torch.int32)
+    batch.err, batch.max_q, batch.max_ctx = torch.zeros(1, dtype=torch.int32), 4, 65
+    batch.page_table = wide[:, 8:10]
+    desc = batch._desc(7)
+    assert desc.table_width == 2 and desc.table_stride == (50 if rows > 1 else 2)
+    _refused(LIB.mg_kv8_append, _cache(), desc, _append(), INVALID, "page table")  # 65 positions, 2 pages of 32
+    batch.page_table = wide[:, 8:11]
+    _refused(LIB.mg_kv8_append, _cache(), batch._desc(7), _append(k_dev=P + 4), INVALID, "aligned")
