@@ -29,9 +29,13 @@
 // steps and the join.
 //
 // With s = scale log2(e) k_scale <q, k> the state per row is m = max s,
-// l = sum 2^(s - m) and the sum of P V with P = 2^(s + log2 v_scale - M),
+// l = sum 2^(s - m) and the sum of P V with P = 2^(s + log2 v_scale - M + 15),
 // M = max(s + log2 v_scale): the value scale rides in the exponent, so that P
-// is at most 1 whatever the scales, and fp16 holds it to 2^-11.
+// is at most 2^15 whatever the scales.  P is fp16 because it is an MMA operand:
+// held to 2^-11 of itself down to 2^-29 of the row's largest, below that to
+// 2^-40 of the largest, where a term also ends.  (With a largest P of 1 a long
+// tail of weights at 2^-25 of one token's, 0.4 % of a softmax over 131072
+// positions, was lost from the sum of P V while l counted it.)
 #include <cstdio>
 #include <type_traits>
 
@@ -54,6 +58,7 @@ constexpr int kUnit = 64;      // tokens of a unit of the schedule
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kInf = __builtin_huge_valf();
+constexpr float kLift = 15.0f;  // log2 of a row's largest P: 2^15 is the largest power of two in fp16
 
 // D += A . B, 16 x 8 x 16, fp16 operands, fp32 accumulators.
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -358,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         l[nt][e & 1] += ex2(s[i][nt][e] - base[nt][e & 1]);
-                        pr[e] = ex2(s[i][nt][e] + lv[i] - basev[nt][e & 1]);
+                        pr[e] = ex2(s[i][nt][e] + (lv[i] + kLift) - basev[nt][e & 1]);
                     }
                     b0[nt] = transpose8x8(pack_h2(pr[0], pr[1]));
                     b1[nt] = transpose8x8(pack_h2(pr[2], pr[3]));
@@ -445,8 +450,8 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                 const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem) + i * kMerge + r * (HD + 4) + d);
                 acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
             }
-            // O is in units of 2^M, l in units of 2^m; a row that saw nothing has l = 0
-            const float f = ll == 0.f ? 0.f : ex2(bv - b) / ll;
+            // O is in units of 2^(M - kLift), l in units of 2^m; a row that saw nothing has l = 0
+            const float f = ll == 0.f ? 0.f : ex2(bv - b - kLift) / ll;
             acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
             if (whole) {
                 const int row = it.row0 + r, tok = row / p.a.group, hq = head * p.a.group + row - tok * p.a.group;

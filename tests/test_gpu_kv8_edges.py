@@ -6,6 +6,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import kv8_reference as ref  # noqa: E402
+
 from mogemma_b200.kv8 import KV8Batch  # noqa: E402
 from test_gpu_kv8 import BF16, F16, F32, World, _check_append, _check_attention, _ints, _snapshot  # noqa: E402, F401
 
@@ -35,3 +37,54 @@ def test_a_column_slice_of_a_page_table(n) -> None:
     with pytest.raises(RuntimeError, match="lengths"):
         batch.check()
     assert bool((out[n:2 * n] == 0).all()) and torch.equal(out[:n], want[:n])
+
+
+# ---------------------------------------------------------------- weights far below a row's largest
+def _one_hot_world(lens, *, dim, page, codes, kv_heads=1, seed=0):
+    """Keys whose score is their first code alone: codes [positions] (shared by sequences), the rest 0; scales of 1."""
+    w = World(lens, kv_heads=kv_heads, dim=dim, page=page, seed=seed)
+    c = w.cache
+    c.k_scale.fill_(1.0)
+    c.v_scale.fill_(1.0)
+    c.k.view(torch.uint8).zero_()
+    for b, (_, ctx) in enumerate(lens):
+        for p0 in range(0, ctx, page):
+            m = min(page, ctx - p0)
+            c.k[w.table[b][p0 // page], :, :m, 0] = codes[p0:p0 + m, None].T.to(c.k.dtype).expand(kv_heads, m)
+    return w
+
+
+def _set_values(w, b, at, row):
+    """Sequence b's value at position `at` of every head becomes row."""
+    w.cache.v[w.table[b][at // w.page], :, at % w.page] = row.to(w.cache.v.dtype)
+
+
+# P is rounded to fp16 as 2^lift times its ratio to the row's largest so far
+@pytest.mark.parametrize(("n", "dim", "group", "lift"), [(1, 256, 4, 15), (1, 64, 1, 15), (6, 128, 2, 15)])
+@pytest.mark.parametrize("depth", [18.0, 25.2, 30.0])
+def test_a_long_tail_of_small_weights_counts(n, dim, group, lift, depth) -> None:
+    """One token whose weight is 2^depth of every other's and whose value is 0, before 100000 equal ones; 600 streams over
+    the same pages, so that every CTA meets whole contexts (parts of a context have maxima of their own)."""
+    ctx, streams = 100_000, 600
+    codes = torch.full((ctx,), -8.0, device="cuda")
+    codes[3] = 8.0
+    w = _one_hot_world([(n, ctx)], dim=dim, page=256, codes=codes)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w.cache.v.copy_(torch.randint(64, 448, (w.cache.v.shape[0], 1, 1, dim), device="cuda", generator=g)
+                    .expand(w.cache.v.shape))  # all of a sign: the tail does not cancel
+    _set_values(w, 0, 3, torch.zeros(dim, device="cuda"))
+    batch = KV8Batch(_ints(range(0, streams * n + 1, n)), _ints([ctx] * streams), _ints(w.table * streams), max_q=n,
+                     max_ctx=ctx)
+    q = torch.zeros(streams * n, group, dim, dtype=BF16, device="cuda")
+    q[..., 0] = 1.0
+    scale = depth / 16 / 1.4426950408889634
+    out = w.cache.attention(batch, q, scale=scale).view(streams, n, group, dim)
+    batch.check()
+    k, v = (ref.gather(x, s, w.table[0], ctx) for x, s in ((w.cache.k, w.cache.k_scale), (w.cache.v, w.cache.v_scale)))
+    o, size, most = ref.attention(q[:n], k, v, ctx - n, scale, 0)
+    delta = 2 * 2.0**-23 * (dim + 8) * most + 2.0**-20
+    # below fp16's normal range a half step is 2^-25, relative to the 2^lift that the largest P was at its time
+    tol = (torch.finfo(BF16).eps / 2 * o.abs() + size * (2.0**-11 + 2 * delta)
+           + ctx * 2.0**(-25 - lift) * float(v.abs().max()) + 2.0**-126)
+    worst = float(((out.double() - o).abs() / tol).max())
+    assert worst <= 1.0, worst
