@@ -12,8 +12,11 @@
 // shared memory; q is brought into fp16's range by a power of two per row.  The
 // block scales of K multiply the score columns, those of V ride in P's
 // exponent: with s = scale log2(e) k_scale <q, k>, m = max s and
-// M = max(s + log2 v_scale), P = 2^(s + log2 v_scale - M) and l = sum 2^(s - m),
-// so P is bounded whatever the scales and fp16 holds it to 2^-11.
+// M = max(s + log2 v_scale), P = 2^(s + log2 v_scale - M + 8) and l = sum
+// 2^(s - m), so P is bounded whatever the scales.  fp16, the MMA operand's type,
+// holds P to 2^-11 of itself down to 2^-22 of the row's largest, below that to
+// 2^-33 of the largest, where a term also ends; m and M may lag (kRescale),
+// which only widens that.
 //
 // Warps of a CTA (640 threads, one CTA per SM):
 //  * warps 0-7: softmax.  Two row tiles: warpgroup g has tile g, a row per
@@ -38,8 +41,8 @@
 // the S it was made from; the tensor pipe runs one thread's MMAs in order, so
 // the next S on a stage lands after P V has read P.  K and V have two stages
 // each (hd 256: one; S and P V alternate, and either is reloaded under the
-// other).  O is rescaled only when m or M grows by more than 15 (P stays below
-// 2^15, within fp16's range).  A row tile takes no part in units that none of its
+// other).  O is rescaled only when m or M grows by more than 7.9 (P stays within
+// fp16's range).  A row tile takes no part in units that none of its
 // rows see.
 //
 // Units of 64 tokens were the first form: N = 64 reads Q from shared memory for
@@ -71,7 +74,12 @@ constexpr int kM = 128;   // rows of a tile
 constexpr int kN = 128;   // tokens of a unit
 constexpr int kThreads = 640;
 constexpr float kInf = __builtin_huge_valf();
-constexpr float kRescale = 15.0f;  // P stays below 2^15, within fp16
+// log2 of P at a row's reference M, and how far the maximum may grow past M before O is rescaled: P stays below
+// 2^15.9, within fp16.  A higher lift keeps more of the weights far below the row's largest (down to 2^(-24 - kLift)) and
+// rescales more often: lift 0, 6, 8, 13 take 261, 266, 272, 284 us for the 27B prompt below, whose key scales lie 8
+// times apart, and 259 us each where they are alike.
+constexpr float kLift = 8.0f;
+constexpr float kRescale = 15.9f - kLift;
 constexpr int kRing = 4;  // units whose scales are at hand
 
 template <int HD>
@@ -703,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         uint32_t pk[kCh / 2];
 #pragma unroll
                         for (int b = 0; b < kB; ++b) {
-                            const float wv = ex2(fminf(lv[b] + mb - rb, 126.f));
+                            const float wv = ex2(fminf(lv[b] + mb - rb + kLift, 126.f));
                             const F2 w2 = f2(wv, wv), c2 = f2(cf[b], cf[b]);
                             sum[b] = f2(0.f, 0.f);
 #pragma unroll
@@ -828,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             if (any_rows) {
                 const int slot = d->slot;
                 const bool whole = slot < 0;
-                const float f = l == 0.f || !begun ? 0.f : ex2(finite_or_0(mref) - finite_or_0(m)) / l;
+                const float f = l == 0.f || !begun ? 0.f : ex2(finite_or_0(mref) - finite_or_0(m) - kLift) / l;
                 const int row = d->row0 + tg * kM + r, tok = row / p.a.group, hq = d->head * p.a.group + row - tok * p.a.group;
                 T *dst = static_cast<T *>(p.out) + (static_cast<int64_t>(d->q0) + tok) * p.out_row + hq * p.out_head;
                 const int64_t at = static_cast<int64_t>(slot) * C::kRows + tg * kM + r;

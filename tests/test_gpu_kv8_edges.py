@@ -60,7 +60,7 @@ def _set_values(w, b, at, row):
 
 
 # P is rounded to fp16 as 2^lift times its ratio to the row's largest so far
-@pytest.mark.parametrize(("n", "dim", "group", "lift"), [(1, 256, 4, 15), (1, 64, 1, 15), (6, 128, 2, 15)])
+@pytest.mark.parametrize(("n", "dim", "group", "lift"), [(1, 256, 4, 15), (1, 64, 1, 15), (6, 128, 2, 15), (40, 64, 1, 8), (70, 128, 2, 8), (20, 256, 4, 8)])
 @pytest.mark.parametrize("depth", [18.0, 25.2, 30.0])
 def test_a_long_tail_of_small_weights_counts(n, dim, group, lift, depth) -> None:
     """One token whose weight is 2^depth of every other's and whose value is 0, before 100000 equal ones; 600 streams over
