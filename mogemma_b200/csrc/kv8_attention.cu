@@ -238,14 +238,14 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                 }
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-            // a power of two that brings the row's maximum to [2^7, 2^8): fp16 then holds every bf16 value down
-            // to 2^-21 of it exactly.  A row with an infinity or NaN answers NaN.
+            // a power of two that brings the row's maximum to [2^15, 2^16), fp16's last binade: fp16 values then stay
+            // as they are, bf16 values down to 2^-32 of it.  A row with an infinity or NaN answers NaN.
             const int e = static_cast<int>(most >> 23);
             float up = 1.0f, down = 1.0f;
             if (e >= 255) {
                 down = __int_as_float(0x7fc00000);
             } else if (e > 0) {
-                const int sh = min(134 - e, 126);  // exponent of `up`; |sh| <= 126 keeps both normal
+                const int sh = min(142 - e, 126);  // exponent of `up`; |sh| <= 126 keeps both normal
                 up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
                 down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
             }

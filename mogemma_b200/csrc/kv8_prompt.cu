@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             const int t_rows = d->t_rows[tg], take = d->take;
             const bool active = d->sees(tg, d->tok0, take);
             if (active) {
-                // Q: a warp brings kQR rows, kBatch at a time, 4 lanes to a row; a row's largest becomes 2^7 .. 2^8
+                // Q: a warp brings kQR rows, 8 kB at a time, 4 lanes to a row; a row's largest becomes 2^15 .. 2^16
                 constexpr int kQR = C::kTwo ? 32 : 16, kCh = HD / 32;  // 16-byte chunks of a lane: 4 i + lane % 4
                 constexpr int kB = kCh >= 8 ? 1 : 8 / kCh < kQR / 8 ? 8 / kCh : kQR / 8;  // rows of a lane: 32 registers
                 const int nrows = d->nrows, sub = lane & 3;
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         if (e >= 255) {  // a row with an infinity or NaN answers NaN
                             down = __int_as_float(0x7fc00000);
                         } else if (e > 0) {
-                            const int sh = min(134 - e, 126);
+                            const int sh = min(142 - e, 126);
                             up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
                             down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
                         }

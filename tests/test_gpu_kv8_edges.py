@@ -88,3 +88,20 @@ def test_a_long_tail_of_small_weights_counts(n, dim, group, lift, depth) -> None
            + ctx * 2.0**(-25 - lift) * float(v.abs().max()) + 2.0**-126)
     worst = float(((out.double() - o).abs() / tol).max())
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize(("n", "dim", "group"), [(1, 64, 2), (4, 128, 3), (2, 256, 8), (50, 64, 2), (50, 128, 1), (20, 256, 3)])
+def test_query_elements_far_below_their_rows_largest(n, dim, group, dtype) -> None:
+    """The largest elements meet keys of zero, and the scores come from elements 2^-15 to 2^-31 of them."""
+    w = World([(n, 300), (n, 65)], kv_heads=2, dim=dim, page=32, seed=dim)
+    w.cache.k.view(torch.uint8)[..., ::4] = 0
+    q = w.rand(w.rows, 2 * group, dim)
+    bf16 = dtype == BF16
+    low = torch.randint(24, 31, q.shape, device="cuda", generator=w.g) if bf16 else torch.full(q.shape, 15, device="cuda")
+    q = (q.clamp(-3.9, 3.9).abs().clamp(min=1.0).copysign(q) * torch.exp2(-low.float()))  # bits down to 2^-38 of 1
+    q[..., ::4] = 1.5 if bf16 else 60000.0
+    q = q.to(dtype)
+    scale = 2.0**25 if bf16 else 2.0**14
+    out = w.cache.attention(w.batch, q, scale=scale)
+    _check_attention(w, q, out, scale=scale, window=0)
