@@ -218,6 +218,14 @@ mg_status mg_encode(mg_model *m, const int32_t *token_ids_host, const int32_t *l
  * model's positions restored and the model usable.  Production callers leave
  * both unset. */
 mg_status mg_set_debug(mg_model *m, uint64_t wait_budget_ns, int32_t stall_phase);
+/* The same for the bounded waits inside mg_kv8_attention's kernel for many query
+ * rows, in the calling thread's later calls: their budget (0: 2 s), and a
+ * hand-off that one CTA withholds (-1: none; 0 items, 1 items done, 2 keys,
+ * 3 keys done, 4 values, 5 values done, 6 queries, 7 scores, 8 weights,
+ * 9 answers, 10 scales, 11 the halves of a row (head dim 256), 12 the end).  The
+ * waits on it run out, the call's err_dev receives MG_KV8_ERR_WAIT, and the
+ * kernel ends; calls after the hook is cleared run as before. */
+mg_status mg_kv8_set_debug(uint64_t wait_budget_ns, int32_t stall);
 
 /* ---- inspection (tests) ---- */
 mg_status mg_read_kv(const mg_model *m, int32_t layer, int32_t row, int32_t pos, float *k_host, float *v_host);

@@ -200,10 +200,12 @@ _lib.mg_kv8_attention.argtypes = [ctypes.POINTER(KV8CacheDesc), ctypes.POINTER(K
                                   ctypes.POINTER(KV8AttentionArgs), _P]
 _lib.mg_kv8_attention_workspace.argtypes = [ctypes.POINTER(KV8CacheDesc), ctypes.POINTER(KV8BatchDesc),
                                             ctypes.c_int32, ctypes.POINTER(ctypes.c_int64)]
+_lib.mg_kv8_set_debug.argtypes = [ctypes.c_uint64, ctypes.c_int32]
 for _f in ("mg_model_create", "mg_model_info_get", "mg_model_destroy", "mg_set_pos", "mg_get_pos", "mg_step",
            "mg_prefill", "mg_generate", "mg_set_tokens", "mg_sample", "mg_embed", "mg_read_kv",
            "mg_tp_ipc_handle", "mg_tp_connect", "mg_tp_disconnect", "mg_encode", "mg_trace_enable", "mg_trace_read",
-           "mg_set_debug", "mg_kv8_append", "mg_kv8_attention", "mg_kv8_attention_workspace"):
+           "mg_set_debug", "mg_kv8_append", "mg_kv8_attention", "mg_kv8_attention_workspace",
+           "mg_kv8_set_debug"):
     getattr(_lib, _f).restype = ctypes.c_int
 
 

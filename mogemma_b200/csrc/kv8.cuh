@@ -273,6 +273,13 @@ struct AttnArgs {
     void *out;
     int64_t q_row, q_head, out_row, out_head;
     float scale_log2;  // scale * log2(e)
+    uint64_t wait_ns;  // budget of a wait inside the prompt kernel
+    int stall;         // mg_kv8_set_debug: the hand-off that CTA 0 withholds; -1: none
+};
+// Hand-offs of the prompt kernel, as mg_kv8_set_debug counts them.
+enum Handoff : int {
+    kItemFull, kItemEmpty, kKFull, kKEmpty, kVFull, kVEmpty, kQFull, kSFull, kPFull, kPvDone, kScales, kPair, kDrained,
+    kHandoffs
 };
 }  // namespace kv8
 }  // namespace mg

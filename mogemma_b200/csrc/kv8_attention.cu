@@ -658,6 +658,12 @@ cudaError_t launch_attention(const AttnArgs &p, int hd, int ctas, int sms, cudaS
     return e != cudaSuccess ? e : launch_combine<T>(p, hd, ctas, sms, s);
 }
 
+struct Debug {  // mg_kv8_set_debug, of the calling thread
+    uint64_t wait_ns = kWaitBudgetNs;
+    int stall = -1;
+};
+thread_local Debug debug;
+
 struct Plan {
     int rows, unit, extra, tiles, ctas, sms;
     size_t bytes;
@@ -757,8 +763,22 @@ extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_ba
     p.q_row = args->q_row_stride, p.q_head = args->q_head_stride;
     p.out_row = args->out_row_stride, p.out_head = args->out_head_stride;
     p.scale_log2 = args->scale * 1.4426950408889634f;
+    p.wait_ns = debug.wait_ns;
+    p.stall = debug.stall;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     e = args->dtype == MG_BF16 ? launch_attention<__nv_bfloat16>(p, cache->head_dim, pl.ctas, pl.sms, s)
                                : launch_attention<__half>(p, cache->head_dim, pl.ctas, pl.sms, s);
     return e == cudaSuccess ? MG_OK : cuda_error(who, e);
+}
+
+extern "C" mg_status mg_kv8_set_debug(uint64_t wait_budget_ns, int32_t stall) {
+    using namespace kv8;
+    if (stall < -1 || stall >= kHandoffs) {
+        char buf[100];
+        snprintf(buf, sizeof buf, "mg_kv8_set_debug: stall %d outside [-1, %d)", stall, static_cast<int>(kHandoffs));
+        return report_error(MG_ERR_INVALID, buf);
+    }
+    debug.wait_ns = wait_budget_ns ? wait_budget_ns : kWaitBudgetNs;
+    debug.stall = stall;
+    return MG_OK;
 }

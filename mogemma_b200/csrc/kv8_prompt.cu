@@ -181,14 +181,14 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
 }
 
 // Bounded wait.  err_dev may hold a bad page's code already, so a stop is announced in shared memory.
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err) {
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err, uint64_t budget) {
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t n = 1;; ++n) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((n & 15u) == 0u) {
             if (*stop) return false;
-            if (globaltimer_ns() - t0 > kWaitBudgetNs) {
+            if (globaltimer_ns() - t0 > budget) {
                 *stop = 1;
                 set_error(err, kErrWait);
                 return false;
@@ -287,28 +287,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     const int cta = blockIdx.x;
 
     if (threadIdx.x == 0) {
+        // one arrival more than there will be withholds a hand-off (a test of the bounded waits)
+        auto init = [&](uint64_t *bar, int arrivals, Handoff h) {
+            mbar_init(bar, arrivals + (cta == 0 && p.stall == h ? 1 : 0));
+        };
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 4);
-            mbar_init(&k_empty[i], kTiles);
-            mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], kTiles);
-            mbar_init(&q_full[i], C::kTwo ? 4 : 8);
+            init(&k_full[i], 4, kKFull);
+            init(&k_empty[i], kTiles, kKEmpty);
+            init(&v_full[i], 4, kVFull);
+            init(&v_empty[i], kTiles, kVEmpty);
+            init(&q_full[i], C::kTwo ? 4 : 8, kQFull);
             for (int g = 0; g < 2; ++g) {
-                mbar_init(&s_full[g][i], 1);
-                mbar_init(&p_full[g][i], C::kTwo ? 4 : 8);
-                mbar_init(&pv_done[g][i], 1);
+                init(&s_full[g][i], 1, kSFull);
+                init(&p_full[g][i], C::kTwo ? 4 : 8, kPFull);
+                init(&pv_done[g][i], 1, kPvDone);
             }
-            mbar_init(&drained[i], 1);
+            init(&drained[i], 1, kDrained);
         }
-        for (int i = 0; i < kRing; ++i) mbar_init(&sc_full[i], 8);
+        for (int i = 0; i < kRing; ++i) init(&sc_full[i], 8, kScales);
         for (int i = 0; i < kItems; ++i) {
-            mbar_init(&item_full[i], 1);
-            mbar_init(&item_empty[i], 16 + kTiles);  // 8 softmax warps, 8 loaders, the MMA issuers
+            init(&item_full[i], 1, kItemFull);
+            init(&item_empty[i], 16 + kTiles, kItemEmpty);  // 8 softmax warps, 8 loaders, the MMA issuers
         }
         for (int i = 0; i < 4; ++i) {
-            mbar_init(&pair_bar[i][0], 2);
-            mbar_init(&pair_bar[i][1], 2);
-            mbar_init(&q_pair[i], 2);
+            init(&pair_bar[i][0], 2, kPair);
+            init(&pair_bar[i][1], 2, kPair);
+            init(&q_pair[i], 2, kPair);
         }
         stop_s = 0;
         fence_barrier_init();
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     // The i-th item; null at the end of the share, or (stop set) when a wait ran out.
     auto item = [&](uint32_t i) -> const Desc * {
-        const bool ok = wait(&item_full[i % kItems], (i / kItems) & 1u, stop, err);
+        const bool ok = wait(&item_full[i % kItems], (i / kItems) & 1u, stop, err, p.wait_ns);
         return ok && items_s[i % kItems].take > 0 ? &items_s[i % kItems] : nullptr;
     };
     // The same, and a wait, for a whole warp.
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         return __all_sync(0xffffffffu, x != nullptr) ? x : nullptr;
     };
     auto warp_wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-        return __all_sync(0xffffffffu, wait(bar, parity, stop, err));
+        return __all_sync(0xffffffffu, wait(bar, parity, stop, err, p.wait_ns));
     };
 
     if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));
@@ -416,14 +420,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         }
         commit(&drained[g]);  // after a wait that ran out MMAs may be in flight: TMEM and shared memory are held for them
         volatile int never = 0;
-        wait(&drained[g], 0, &never, err);
+        wait(&drained[g], 0, &never, err, p.wait_ns);
     } else if (warp == 18) {  // ---- walker
         if (lane == 0) {
             Walk wk;
             p.part.split[cta].nrows = 0;
             bool more = wk.start(p.b, p.a, pl);
             for (uint32_t i = 0;; ++i) {
-                if (i >= kItems && !wait(&item_empty[i % kItems], (i / kItems - 1) & 1u, stop, err)) break;
+                if (i >= kItems && !wait(&item_empty[i % kItems], (i / kItems - 1) & 1u, stop, err, p.wait_ns)) break;
                 Desc &d = items_s[i % kItems];
                 d.take = more ? wk.take : 0;
                 if (more) {

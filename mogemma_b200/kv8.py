@@ -81,6 +81,12 @@ def _vector(name: str, x: torch.Tensor | None, device: torch.device, shape: tupl
     return x.data_ptr()
 
 
+def set_debug(wait_budget_ns: int = 0, stall: int = -1) -> None:
+    """Failure-detection test hook (``mg_kv8_set_debug``): budget of the waits inside this thread's later attention calls,
+    and a hand-off that one CTA withholds."""
+    _core._check(_core.lib().mg_kv8_set_debug(int(wait_budget_ns), int(stall)))  # noqa: SLF001
+
+
 class KV8Call:
     """A checked call with its tensors; launches on torch's current stream each time it is called."""
 

@@ -2,13 +2,15 @@
 
 from __future__ import annotations
 
+import time
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 import kv8_reference as ref  # noqa: E402
 
-from mogemma_b200.kv8 import KV8Batch  # noqa: E402
+from mogemma_b200.kv8 import KV8Batch, set_debug  # noqa: E402
 from test_gpu_kv8 import BF16, F16, F32, World, _check_append, _check_attention, _ints, _snapshot  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
@@ -105,3 +107,34 @@ def test_query_elements_far_below_their_rows_largest(n, dim, group, dtype) -> No
     scale = 2.0**25 if bf16 else 2.0**14
     out = w.cache.attention(w.batch, q, scale=scale)
     _check_attention(w, q, out, scale=scale, window=0)
+
+
+# ---------------------------------------------------------------- bounded waits
+@pytest.fixture
+def hook():
+    yield set_debug
+    set_debug()
+
+
+HANDOFFS = ["items", "items done", "keys", "keys done", "values", "values done", "queries", "scores", "weights",
+            "answers", "scales", "halves", "end"]
+
+
+@pytest.mark.parametrize(("dim", "handoff"), [  # with two row tiles a row is one thread's: no halves
+    (dim, h) for dim in (64, 128, 256) for h in HANDOFFS if h != "halves" or dim == 256])
+def test_a_wait_that_runs_out_ends_the_call(dim, handoff, hook) -> None:
+    """A hand-off of the prompt kernel that never comes: the call ends within its budget and says so, and the next one
+    answers as before.  Items of one unit, six or more to a CTA, so that every hand-off is waited for."""
+    w = World([(40, 100)] * 450, kv_heads=2, dim=dim, page=32, seed=7)
+    q = w.rand(w.rows, 8, dim, dtype=BF16)
+    want = w.cache.attention(w.batch, q)
+    w.batch.check()
+    hook(20_000_000, HANDOFFS.index(handoff))
+    t0 = time.perf_counter()
+    w.cache.attention(w.batch, q)
+    with pytest.raises(RuntimeError, match="wait ran out"):
+        w.batch.check()
+    assert time.perf_counter() - t0 < 1.0  # the 20 ms budget, not the default's 2 s, ended the waits
+    hook()
+    assert torch.equal(w.cache.attention(w.batch, q), want)
+    w.batch.check()

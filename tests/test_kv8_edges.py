@@ -9,7 +9,7 @@ from test_kv8 import INVALID, LIB, P, _append, _attention, _batch, _cache, _refu
 
 torch = pytest.importorskip("torch")
 
-from mogemma_b200.kv8 import KV8Batch  # noqa: E402
+from mogemma_b200.kv8 import KV8Batch, set_debug  # noqa: E402
 
 
 @pytest.mark.parametrize(("more", "ok"), [
@@ -43,3 +43,11 @@ def test_a_column_slice_of_a_table_gives_its_own_width(rows) -> None:
     _refused(LIB.mg_kv8_append, _cache(), desc, _append(), INVALID, "page table")  # 65 positions, 2 pages of 32
     batch.page_table = wide[:, 8:11]
     _refused(LIB.mg_kv8_append, _cache(), batch._desc(7), _append(k_dev=P + 4), INVALID, "aligned")
+
+
+def test_the_debug_hook_refuses_unknown_handoffs() -> None:
+    for stall in (-2, 13, 1 << 20):
+        with pytest.raises(ValueError, match="stall"):
+            set_debug(0, stall)
+    set_debug(5, 12)
+    set_debug()
