@@ -141,11 +141,17 @@ __device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, in
     return it;
 }
 
+// The pair to go on to: behind a tile without rows its sequence has no more.  (max_q may be far above most lengths:
+// one visit per tile kept the prompt kernel's roles waiting for the next item, 4 million tiles beyond 20 ms.)
+__device__ __forceinline__ int pair_after(const AttnShape &a, int pair, const Item &it) {
+    return it.cost > 0 ? pair + 1 : (pair / a.tiles + 1) * a.tiles;
+}
+
 // Where CTA `cta` of `ctas` starts: its range [w0, w1) of the whole cost, and
 // the item (head, pair) and the place within it of w0.  All threads of the CTA
 // call it; THREADS a multiple of 32.
 struct Place {
-    int64_t total, per_head;  // cost of all heads, of one
+    int64_t total;  // cost of all heads
     int64_t w0, w1;
     int ctas;  // CTAs that have a share
     int head, pair, skip;
@@ -159,7 +165,11 @@ __device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, 
     const int pairs = b.batch * a.tiles, chunk = (pairs + THREADS - 1) / THREADS;
     const int p0 = min(pairs, tid * chunk), p1 = min(pairs, p0 + chunk);
     int64_t mine = 0;
-    for (int p = p0; p < p1; ++p) mine += load_item(b, a, p, cta == 0).cost;
+    for (int p = p0; p < p1;) {
+        const Item it = load_item(b, a, p, cta == 0);
+        mine += it.cost;
+        p = pair_after(a, p, it);
+    }
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -176,7 +186,6 @@ __device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, 
         all += warp_sum_s[w];
     }
     Place pl;
-    pl.per_head = all;
     pl.total = all * heads;
     pl.ctas = static_cast<int>(min(pl.total, static_cast<int64_t>(ctas)));
     pl.w0 = cta < pl.ctas ? pl.total * cta / pl.ctas : 0;
@@ -186,10 +195,12 @@ __device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, 
     if (mine > 0 && upto - mine <= in_head && in_head < upto) {
         int64_t left = in_head - (upto - mine);
         int p = p0;
-        for (; p < p1 - 1; ++p) {
-            const int u = load_item(b, a, p, false).cost;
-            if (left < u) break;
-            left -= u;
+        for (;;) {
+            const Item it = load_item(b, a, p, false);
+            const int next = pair_after(a, p, it);
+            if (left < it.cost || next >= p1) break;
+            left -= it.cost;
+            p = next;
         }
         found_pair = p;
         found_skip = static_cast<int>(left);
@@ -225,7 +236,8 @@ struct Walk {
     __device__ __forceinline__ void step(const Batch &b, const AttnShape &a) {
         w += it.cost > 0 ? it.cost - skip : 0;
         skip = 0;
-        if (++pair == b.batch * a.tiles) pair = 0, ++head;
+        pair = pair_after(a, pair, it);
+        if (pair >= b.batch * a.tiles) pair = 0, ++head;
     }
     __device__ __forceinline__ bool start(const Batch &b, const AttnShape &a, const Place &pl) {
         w = pl.w0, w1 = pl.w1, head = pl.head, pair = pl.pair, skip = pl.skip;

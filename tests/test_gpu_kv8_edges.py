@@ -138,3 +138,16 @@ def test_a_wait_that_runs_out_ends_the_call(dim, handoff, hook) -> None:
     hook()
     assert torch.equal(w.cache.attention(w.batch, q), want)
     w.batch.check()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_sequences_without_tokens_do_not_hold_up_the_rest(dim, hook) -> None:
+    """Two sequences around thousands without tokens, under a bound of many tiles each: going from one to the other
+    takes nobody's wait budget."""
+    rows = 256 if dim <= 128 else 128
+    empty, max_q = 8190, 131_000 * rows // 256
+    w = World([(40, 100), *[(0, 0)] * empty, (40, 77)], kv_heads=64, dim=dim, page=16, max_q=max_q)
+    q = w.rand(w.rows, 64, dim, dtype=BF16)
+    hook(20_000_000)
+    out = w.cache.attention(w.batch, q)
+    _check_attention(w, q, out, scale=dim**-0.5, window=0)
