@@ -181,14 +181,15 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
 }
 
 // Bounded wait.  err_dev may hold a bad page's code already, so a stop is announced in shared memory.
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err, uint64_t budget) {
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err,
+                                     const volatile uint64_t *budget) {
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t n = 1;; ++n) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((n & 15u) == 0u) {
             if (*stop) return false;
-            if (globaltimer_ns() - t0 > budget) {
+            if (globaltimer_ns() - t0 > *budget) {
                 *stop = 1;
                 set_error(err, kErrWait);
                 return false;
@@ -277,7 +278,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     __shared__ float2 xch[2][2][kM];  // one row tile: the two halves' maxima (by S stage)
     __shared__ uint32_t tmem_slot;
     __shared__ int stop_s;
+    __shared__ uint64_t budget_s;  // of a wait; in shared memory, read by a wait that lasts, it takes no registers
     volatile int *stop = &stop_s;
+    const volatile uint64_t *budget = &budget_s;
     uint32_t *err = p.b.err;
     const uintptr_t base = (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023);
     unsigned char *gen = reinterpret_cast<unsigned char *>(base);
@@ -315,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             init(&q_pair[i], 2, kPair);
         }
         stop_s = 0;
+        budget_s = p.wait_ns;
         fence_barrier_init();
     }
     if (warp == 16) {
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     // The i-th item; null at the end of the share, or (stop set) when a wait ran out.
     auto item = [&](uint32_t i) -> const Desc * {
-        const bool ok = wait(&item_full[i % kItems], (i / kItems) & 1u, stop, err, p.wait_ns);
+        const bool ok = wait(&item_full[i % kItems], (i / kItems) & 1u, stop, err, budget);
         return ok && items_s[i % kItems].take > 0 ? &items_s[i % kItems] : nullptr;
     };
     // The same, and a wait, for a whole warp.
@@ -340,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         return __all_sync(0xffffffffu, x != nullptr) ? x : nullptr;
     };
     auto warp_wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-        return __all_sync(0xffffffffu, wait(bar, parity, stop, err, p.wait_ns));
+        return __all_sync(0xffffffffu, wait(bar, parity, stop, err, budget));
     };
 
     if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));
@@ -420,14 +424,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         }
         commit(&drained[g]);  // after a wait that ran out MMAs may be in flight: TMEM and shared memory are held for them
         volatile int never = 0;
-        wait(&drained[g], 0, &never, err, p.wait_ns);
+        wait(&drained[g], 0, &never, err, budget);
     } else if (warp == 18) {  // ---- walker
         if (lane == 0) {
             Walk wk;
             p.part.split[cta].nrows = 0;
             bool more = wk.start(p.b, p.a, pl);
             for (uint32_t i = 0;; ++i) {
-                if (i >= kItems && !wait(&item_empty[i % kItems], (i / kItems - 1) & 1u, stop, err, p.wait_ns)) break;
+                if (i >= kItems && !wait(&item_empty[i % kItems], (i / kItems - 1) & 1u, stop, err, budget)) break;
                 Desc &d = items_s[i % kItems];
                 d.take = more ? wk.take : 0;
                 if (more) {
