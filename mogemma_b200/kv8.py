@@ -130,10 +130,13 @@ class KV8Batch:
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     def check(self) -> None:
-        """Raises if a call since the last check met lengths or page ids out of bounds (synchronises)."""
+        """Raises if a call since the last check met lengths or page ids out of bounds.  Waits for the whole device: the
+        calls may have gone to any of its streams."""
+        torch.cuda.synchronize(self.device)
         code = int(self.err.item())
         if code:
             self.err.zero_()
+            torch.cuda.synchronize(self.device)  # before a later call on another stream
             raise RuntimeError(f"8-bit cache: {_ERRORS.get(code, f'error word 0x{code:x}')}")
 
     def _desc(self, total_q: int) -> _core.KV8BatchDesc:

@@ -151,3 +151,21 @@ def test_sequences_without_tokens_do_not_hold_up_the_rest(dim, hook) -> None:
     hook(20_000_000)
     out = w.cache.attention(w.batch, q)
     _check_attention(w, q, out, scale=dim**-0.5, window=0)
+
+
+# ---------------------------------------------------------------- streams
+def test_check_sees_calls_on_every_stream() -> None:
+    """A call that waits on another stream while check() is made, and one that follows it there at once."""
+    w = World([(1, 100), (1, 100)], kv_heads=1, dim=64, page=16, max_ctx=100)
+    q = w.rand(w.rows, 2, 64, dtype=F16)
+    w.batch.ctx_len[1] = 101
+    call = w.cache.attention_call(w.batch, q, torch.zeros_like(q))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+            call()
+        with pytest.raises(RuntimeError, match="lengths"):
+            w.batch.check()
+    w.batch.check()
