@@ -12,7 +12,8 @@ bounds and error rules are those of ``include/mogemma_b200.h``.
 
 ``append_call`` / ``attention_call`` check and bind the same arguments once; the
 object they return launches the call each time it is called (on torch's current
-stream of the cache's device), so a decode loop that keeps its buffers pays for
+stream of the cache's device; the caller orders its own tensors between streams,
+the call its workspace and error word), so a decode loop that keeps its buffers pays for
 the checks once.  A bound call reads the tensors' contents anew every time: new
 rows, lengths and tables are written into the same tensors.  It may be captured
 into a CUDA graph; the call object then has to live as long as the graph.  An
@@ -90,22 +91,40 @@ def set_debug(wait_budget_ns: int = 0, stall: int = -1) -> None:
 class KV8Call:
     """A checked call with its tensors; launches on torch's current stream each time it is called."""
 
-    def __init__(self, fn: Callable[..., int], device: torch.device, structs: tuple[Any, ...], keep: tuple[Any, ...]) -> None:
+    def __init__(self, fn: Callable[..., int], batch: KV8Batch, structs: tuple[Any, ...], keep: tuple[Any, ...],
+                 own: tuple[torch.Tensor, ...] = ()) -> None:
         self._fn = fn
-        self._device = device
+        self._device = batch.device
         self._structs = structs
         self._refs = tuple(ctypes.byref(s) for s in structs)
-        self._keep = keep
+        self._keep = (batch, *keep)
+        self._own = (batch.err, *own)  # the tensors that the caller does not see
+        self._homes = {batch.stream, _raw_stream(self._device.index)}  # streams they were made on
+        self._met = set(self._homes) if len(self._homes) == 1 else set()
+
+    def _meet(self, stream: int) -> None:
+        """On another stream: behind what made the call's own tensors, which then live until this stream is done."""
+        if torch.cuda.is_current_stream_capturing():  # a capture begins with a wait for the device; the graph's owner keeps the call
+            return
+        here = torch.cuda.current_stream()
+        for home in self._homes - {stream}:
+            here.wait_stream(torch.cuda.ExternalStream(home) if home else torch.cuda.default_stream())
+        for x in self._own:
+            x.record_stream(here)
+        self._met.add(stream)
 
     def __call__(self) -> None:
         dev = self._device.index
         if torch.cuda.current_device() != dev:
             with torch.cuda.device(dev):
-                status = self._fn(*self._refs, _raw_stream(dev))
-        else:
-            status = self._fn(*self._refs, _raw_stream(dev))
+                return self()
+        stream = _raw_stream(dev)
+        if stream not in self._met:
+            self._meet(stream)
+        status = self._fn(*self._refs, stream)
         if status:
             _core._check(status)  # noqa: SLF001
+        return None
 
 
 class KV8Batch:
@@ -128,6 +147,7 @@ class KV8Batch:
         self.max_q, self.max_ctx = _i32(max_q), _i32(max_ctx)
         self.device = q_start.device
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.stream = _raw_stream(self.device.index)  # that the error word was made on
 
     def check(self) -> None:
         """Raises if a call since the last check met lengths or page ids out of bounds.  Waits for the whole device: the
@@ -227,8 +247,8 @@ class KV8Cache:
             *(_strides(q_out) if heads else (0, 0)),
             _vector("q_norm", q_norm, self.device, (d,)), _vector("k_norm", k_norm, self.device, (d,)),
             _vector("cos", cos, self.device, (length, d // 2)), _vector("sin", sin, self.device, (length, d // 2)))
-        return KV8Call(_core.lib().mg_kv8_append, self.device, (self._c, self._batch(batch, k.shape[0]), args),
-                       (self, batch, q, k, v, q_out, q_norm, k_norm, cos, sin))
+        return KV8Call(_core.lib().mg_kv8_append, batch, (self._c, self._batch(batch, k.shape[0]), args),
+                       (self, q, k, v, q_out, q_norm, k_norm, cos, sin))
 
     def append(self, batch: KV8Batch, k: torch.Tensor, v: torch.Tensor, **more: Any) -> None:
         """``append_call`` with the same arguments, launched once."""
@@ -254,16 +274,18 @@ class KV8Cache:
         _written("out", out)
         _need(q.data_ptr() != out.data_ptr(), "out must not be q")
         size = self.workspace_bytes(batch, q.shape[1])
+        own: tuple[torch.Tensor, ...] = ()
         if workspace is None:
             workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
+            own = (workspace,)
         _need(workspace.dtype == torch.uint8 and workspace.device == self.device and workspace.is_contiguous(),
               f"workspace must be a contiguous uint8 tensor on {self.device}")
         args = _core.KV8AttentionArgs(
             ctypes.sizeof(_core.KV8AttentionArgs), _TYPES[q.dtype], q.shape[1], _i32(window),
             d ** -0.5 if scale is None else float(scale), 0, q.data_ptr(), out.data_ptr(), *_strides(q),
             *_strides(out), workspace.data_ptr(), workspace.numel())
-        return KV8Call(_core.lib().mg_kv8_attention, self.device, (self._c, self._batch(batch, q.shape[0]), args),
-                       (self, batch, q, out, workspace))
+        return KV8Call(_core.lib().mg_kv8_attention, batch, (self._c, self._batch(batch, q.shape[0]), args),
+                       (self, q, out, workspace), own)
 
     def attention(self, batch: KV8Batch, q: torch.Tensor, out: torch.Tensor | None = None, **more: Any) -> torch.Tensor:
         """``attention_call`` with the same arguments, launched once; returns out (a new tensor if none is given)."""

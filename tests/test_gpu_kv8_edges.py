@@ -169,3 +169,66 @@ def test_check_sees_calls_on_every_stream() -> None:
         with pytest.raises(RuntimeError, match="lengths"):
             w.batch.check()
     w.batch.check()
+
+
+def _load_kernels(w, q) -> None:
+    """A kernel's first launch may wait for the device: everything that a test launches has run before."""
+    torch.cuda._sleep(1000)
+    torch.full((4096,), 255, dtype=torch.uint8, device="cuda")
+    with torch.cuda.stream(torch.cuda.Stream()):
+        w.cache.attention(KV8Batch(w.batch.q_start, w.batch.ctx_len, w.batch.page_table, max_q=1, max_ctx=16), q)
+    torch.cuda.synchronize()
+
+
+def test_an_error_word_made_on_a_busy_stream() -> None:
+    """The batch is made behind work on one stream, and a call on another stream reports before that work is done."""
+    w = World([(1, 100), (1, 100)], kv_heads=1, dim=64, page=16, max_ctx=100)
+    q = w.rand(w.rows, 2, 64, dtype=F16)
+    out, side = torch.zeros_like(q), torch.cuda.Stream()
+    _load_kernels(w, q)
+    w.batch.ctx_len[1] = 101
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    batch = KV8Batch(w.batch.q_start, w.batch.ctx_len, w.batch.page_table, max_q=1, max_ctx=100)
+    call = w.cache.attention_call(batch, q, out)
+    with torch.cuda.stream(side):
+        call()
+    with pytest.raises(RuntimeError, match="lengths"):
+        batch.check()
+
+
+def test_a_workspace_outlives_its_call_on_another_stream() -> None:
+    """The call object goes while its launch on another stream still waits: its workspace is not handed out again."""
+    w = World([(1, 3000)], kv_heads=2, dim=128, page=16)
+    q = w.rand(w.rows, 4, 128, dtype=BF16)
+    want, out, side = w.cache.attention(w.batch, q), torch.zeros_like(q), torch.cuda.Stream()
+    call = w.cache.attention_call(w.batch, q, out)
+    size, places = w.cache.workspace_bytes(w.batch, 4), {call._keep[-1].data_ptr()}
+    _load_kernels(w, q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        call()
+    del call
+    again = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    assert not places & {x.data_ptr() for x in again}
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_a_call_bound_on_one_stream_and_captured_on_another() -> None:
+    w = World([(1, 3000)], kv_heads=2, dim=128, page=16)
+    q = w.rand(w.rows, 4, 128, dtype=BF16)
+    want, out = w.cache.attention(w.batch, q), torch.zeros_like(q)
+    call = w.cache.attention_call(w.batch, q, out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        call()
+    for side in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out.zero_()
+            graph.replay()
+            call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
