@@ -168,14 +168,20 @@ class KV8Batch:
             width if n == 1 else self.page_table.stride(0), self.err.data_ptr())
 
 
+def _check_sizes(pages: int, heads: int, size: int, dim: int) -> None:
+    """What mg_kv8_append and mg_kv8_attention take: a cache of other sizes would be refused by every call."""
+    _need(pages > 0 and 0 < heads <= 65535, "need num_pages > 0 and kv_heads in 1..65535")
+    _need(size in (16, 32, 64, 128, 256), "page_size must be a power of two in 16..256")
+    _need(dim in (64, 128, 256), "head_dim must be 64, 128 or 256")
+
+
 class KV8Cache:
     """One layer's pages of e4m3 codes ``[pages, kv heads, page size, head dim]`` and their scales
     ``[pages, kv heads, page size / 16]``."""
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
                  device: torch.device | str = "cuda") -> None:
-        _need(num_pages > 0 and page_size >= BLOCK and page_size % BLOCK == 0 and kv_heads > 0 and head_dim > 0,
-              "need num_pages, kv_heads, head_dim > 0 and page_size a multiple of 16")
+        _check_sizes(num_pages, kv_heads, page_size, head_dim)
         shape = (num_pages, kv_heads, page_size, head_dim)
         scales = (num_pages, kv_heads, page_size // BLOCK)
         self._bind(*(torch.zeros(shape, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)),
@@ -196,7 +202,7 @@ class KV8Cache:
         _need(k.shape == v.shape and k.stride() == v.stride() and k.device == v.device,
               "k and v must have the same shape, strides and device")
         pages, heads, size, dim = k.shape
-        _need(k.numel() > 0 and size % BLOCK == 0, "the cache must not be empty; page_size a multiple of 16")
+        _check_sizes(pages, heads, size, dim)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
         self.device = k.device

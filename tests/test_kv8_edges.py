@@ -9,7 +9,7 @@ from test_kv8 import INVALID, LIB, P, _append, _attention, _batch, _cache, _refu
 
 torch = pytest.importorskip("torch")
 
-from mogemma_b200.kv8 import KV8Batch, set_debug  # noqa: E402
+from mogemma_b200.kv8 import KV8Batch, KV8Cache, set_debug  # noqa: E402
 
 
 @pytest.mark.parametrize(("more", "ok"), [
@@ -51,3 +51,12 @@ def test_the_debug_hook_refuses_unknown_handoffs() -> None:
             set_debug(0, stall)
     set_debug(5, 12)
     set_debug()
+
+
+@pytest.mark.parametrize(("sizes", "text"), [
+    ((0, 16, 1, 64), "num_pages"), ((4, 16, 0, 64), "kv_heads"), ((4, 16, 65536, 64), "kv_heads"),
+    ((4, 8, 1, 64), "page_size"), ((4, 48, 1, 64), "page_size"), ((4, 512, 1, 64), "page_size"),
+    ((4, 16, 1, 32), "head_dim"), ((4, 16, 1, 96), "head_dim"), ((4, 16, 1, 512), "head_dim")])
+def test_a_cache_that_every_call_would_refuse_is_not_made(sizes, text) -> None:
+    with pytest.raises(ValueError, match=text):
+        KV8Cache(*sizes, device="cpu")  # its codes would be refused for that, but no memory is taken
