@@ -36,6 +36,8 @@
 // 2^-40 of the largest, where a term also ends.  (With a largest P of 1 a long
 // tail of weights at 2^-25 of one token's, 0.4 % of a softmax over 131072
 // positions, was lost from the sum of P V while l counted it.)
+#include <cfloat>
+#include <cmath>
 #include <cstdio>
 #include <type_traits>
 
@@ -735,8 +737,9 @@ extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_ba
     if (st != MG_OK) return st;
     if (args->dtype != MG_BF16 && args->dtype != MG_F16)
         return report_error(MG_ERR_UNSUPPORTED, "mg_kv8_attention: dtype must be MG_BF16 or MG_F16");
-    if (args->window < 0 || !(args->scale >= -3.0e38f && args->scale <= 3.0e38f))
-        return report_error(MG_ERR_INVALID, "mg_kv8_attention: need window >= 0 and a finite scale");
+    const float scale_log2 = args->scale * 1.4426950408889634f;
+    if (args->window < 0 || !(fabsf(scale_log2) <= FLT_MAX))
+        return report_error(MG_ERR_INVALID, "mg_kv8_attention: need window >= 0 and a finite scale (scale * log2(e) too)");
     if (!args->q_dev || !args->out_dev) return report_error(MG_ERR_INVALID, "mg_kv8_attention: null q or out");
     if (((reinterpret_cast<uintptr_t>(args->q_dev) | reinterpret_cast<uintptr_t>(args->out_dev)) % 16) != 0 ||
         ((args->q_row_stride | args->q_head_stride | args->out_row_stride | args->out_head_stride) % 8) != 0)
@@ -762,7 +765,7 @@ extern "C" mg_status mg_kv8_attention(const mg_kv8_cache *cache, const mg_kv8_ba
     p.q = args->q_dev, p.out = args->out_dev;
     p.q_row = args->q_row_stride, p.q_head = args->q_head_stride;
     p.out_row = args->out_row_stride, p.out_head = args->out_head_stride;
-    p.scale_log2 = args->scale * 1.4426950408889634f;
+    p.scale_log2 = scale_log2;
     p.wait_ns = debug.wait_ns;
     p.stall = debug.stall;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

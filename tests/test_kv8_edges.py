@@ -60,3 +60,9 @@ def test_the_debug_hook_refuses_unknown_handoffs() -> None:
 def test_a_cache_that_every_call_would_refuse_is_not_made(sizes, text) -> None:
     with pytest.raises(ValueError, match=text):
         KV8Cache(*sizes, device="cpu")  # its codes would be refused for that, but no memory is taken
+
+
+@pytest.mark.parametrize("scale", [3.0e38, -3.0e38, 2.4e38])
+def test_a_scale_whose_product_with_log2_e_overflows_is_refused(scale) -> None:
+    """The kernels work in powers of two: an infinite factor would turn scores of zero into NaN."""
+    _refused(LIB.mg_kv8_attention, _cache(), _batch(), _attention(scale=scale), INVALID, "finite scale")
