@@ -10,19 +10,12 @@ from typing import TYPE_CHECKING
 if TYPE_CHECKING:
     from .config import EmbeddingConfig, GenerationConfig
     from .hub import HubManager
-    from .kv8 import KV8Batch, KV8Cache
+    from .kv8 import KV8Batch as KV8Batch
+    from .kv8 import KV8Cache as KV8Cache
     from .model import AsyncGemmaModel, EmbeddingModel, SyncGemmaModel
 
-__all__ = [
-    "AsyncGemmaModel",
-    "EmbeddingConfig",
-    "EmbeddingModel",
-    "GenerationConfig",
-    "HubManager",
-    "KV8Batch",
-    "KV8Cache",
-    "SyncGemmaModel",
-]
+# KV8Batch and KV8Cache are imported by name: they need torch, which nothing else here does.
+__all__ = ["AsyncGemmaModel", "EmbeddingConfig", "EmbeddingModel", "GenerationConfig", "HubManager", "SyncGemmaModel"]
 
 _WHERE = {
     "AsyncGemmaModel": ".model",

@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
 
 import pytest
 from test_kv8 import INVALID, LIB, P, _append, _attention, _batch, _cache, _refused
@@ -66,3 +68,13 @@ def test_a_cache_that_every_call_would_refuse_is_not_made(sizes, text) -> None:
 def test_a_scale_whose_product_with_log2_e_overflows_is_refused(scale) -> None:
     """The kernels work in powers of two: an infinite factor would turn scores of zero into NaN."""
     _refused(LIB.mg_kv8_attention, _cache(), _batch(), _attention(scale=scale), INVALID, "finite scale")
+
+
+def test_a_star_import_needs_no_torch() -> None:
+    code = ("import sys; sys.modules['torch'] = None\nfrom mogemma_b200 import *\n"
+            "assert SyncGemmaModel and AsyncGemmaModel and EmbeddingModel and GenerationConfig\n")
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, check=False)
+    assert run.returncode == 0, run.stderr
+    from mogemma_b200 import KV8Batch as by_name
+
+    assert by_name is KV8Batch
