@@ -203,6 +203,12 @@ class KV8Cache:
               "k and v must have the same shape, strides and device")
         pages, heads, size, dim = k.shape
         _check_sizes(pages, heads, size, dim)
+        reach = 1  # bytes that the dimensions of smaller strides span
+        for stride, n in sorted((s, n) for s, n in zip(k.stride(), k.shape) if n > 1):
+            _need(stride >= reach, "pages, heads and tokens of the cache must not overlap")
+            reach += stride * (n - 1)
+        _need(k.data_ptr() != v.data_ptr() and k_scale.data_ptr() != v_scale.data_ptr(),
+              "k and v must not be the same memory, nor their scales")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, size, dim
         self.device = k.device

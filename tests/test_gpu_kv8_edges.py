@@ -10,7 +10,7 @@ torch = pytest.importorskip("torch")
 
 import kv8_reference as ref  # noqa: E402
 
-from mogemma_b200.kv8 import KV8Batch, set_debug  # noqa: E402
+from mogemma_b200.kv8 import KV8Batch, KV8Cache, set_debug  # noqa: E402
 from test_gpu_kv8 import BF16, F16, F32, World, _check_append, _check_attention, _ints, _snapshot  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
@@ -232,3 +232,17 @@ def test_a_call_bound_on_one_stream_and_captured_on_another() -> None:
             call()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_caches_whose_vectors_share_memory_are_refused() -> None:
+    codes, scales = torch.zeros(40_000, dtype=torch.uint8, device="cuda"), [torch.ones(3, 2, 2, device="cuda") for _ in range(2)]
+    shape = (3, 2, 32, 64)
+    k, v = (codes[i:].as_strided(shape, (6144, 3072, 96, 1)) for i in (0, 18_448))
+    for strides in ((4096, 2048, 64), (4096, 64, 128), (2048, 6144, 64), (6144, 3072, 96)):
+        KV8Cache.wrap(*(x.as_strided(shape, (*strides, 1), x.storage_offset()) for x in (k, v)), *scales)
+    for strides in ((64, 2048, 64), (4096, 2048, 48), (4096, 64, 64), (4096, 1024, 64), (4096, 0, 64), (0, 2048, 64)):
+        with pytest.raises(ValueError, match="must not overlap"):
+            KV8Cache.wrap(*(x.as_strided(shape, (*strides, 1), x.storage_offset()) for x in (k, v)), *scales)
+    for args in ((k, k, *scales), (k, v, scales[0], scales[0])):
+        with pytest.raises(ValueError, match="same memory"):
+            KV8Cache.wrap(*args)
