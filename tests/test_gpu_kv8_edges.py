@@ -246,3 +246,132 @@ def test_caches_whose_vectors_share_memory_are_refused() -> None:
     for args in ((k, k, *scales), (k, v, scales[0], scales[0])):
         with pytest.raises(ValueError, match="same memory"):
             KV8Cache.wrap(*args)
+
+
+# ---------------------------------------------------------------- bad pages and lengths
+def _check_rows(w, b, q, out, hidden=()) -> None:
+    """Sequence b's answers, query by query, without the positions of the pages in `hidden`."""
+    n, ctx = w.lens[b]
+    dim = w.cache.head_dim
+    table = [w.table[b][0] if i in hidden else p for i, p in enumerate(w.table[b])]
+    k, v = (ref.gather(x, s, table, ctx) for x, s in ((w.cache.k, w.cache.k_scale), (w.cache.v, w.cache.v_scale)))
+    for i in range(n):
+        row, pos = w.start[b] + i, ctx - n + i
+        keep = [t for t in range(pos + 1) if t // w.page not in hidden]
+        if not keep:
+            assert bool((out[row] == 0).all())
+            continue
+        o, size, most = ref.attention(q[row:row + 1], k[:, keep], v[:, keep], len(keep) - 1, dim**-0.5, 0)
+        tol = ref.attention_tolerance(o, size, most, float(v.abs().max()), len(keep), dim, out.dtype)
+        assert bool(((out[row:row + 1].double() - o).abs() <= tol).all()), i
+
+
+@pytest.mark.parametrize(("dim", "page"), [(64, 16), (128, 32), (256, 128)])
+@pytest.mark.parametrize("n", [1, 9, 60])
+@pytest.mark.parametrize("ids", [(-1, 10**6), (-2**31, 2**31 - 1)])
+def test_attention_sees_none_of_a_bad_page(n, dim, page, ids) -> None:
+    """One sequence's first and third page are out of range, another's all."""
+    w = World([(n, 300), (n, 260), (n, 60), (n, 300)], kv_heads=2, dim=dim, page=page)
+    q = w.rand(w.rows, 4, dim, dtype=F16)
+    good = w.cache.attention(w.batch, q)
+    w.batch.check()
+    w.batch.page_table[1, 0], w.batch.page_table[1, 2] = ids
+    w.batch.page_table[2] = w.cache.num_pages
+    out = w.cache.attention(w.batch, q)
+    with pytest.raises(RuntimeError, match="page id"):
+        w.batch.check()
+    assert torch.equal(out[:n], good[:n]) and torch.equal(out[3 * n:], good[3 * n:])
+    _check_rows(w, 1, q, out, hidden=(0, 2))
+    assert bool((out[2 * n:3 * n] == 0).all())
+
+
+def _append_args(w, group, dtype=F32):
+    kv, d = w.cache.kv_heads, w.cache.head_dim
+    q, k, v = (w.rand(w.rows, h, d, dtype=dtype) for h in (kv * group, kv, kv))
+    cos, sin = ref.rope_tables(320, d, "cuda")
+    return k, v, {"q": q, "q_out": torch.full_like(q, 7.0), "cos": cos, "sin": sin}
+
+
+def _restore(w, was) -> None:
+    for x, old in zip((w.cache.k, w.cache.v, w.cache.k_scale, w.cache.v_scale), was):
+        x.copy_(old)
+
+
+# max_q chooses the form: a group per token, blocks by sequence, blocks by rows
+@pytest.mark.parametrize(("n", "max_q"), [(1, 1), (1, 40), (40, 40), (40, 4000)])
+@pytest.mark.parametrize("bad", [-1, -2**31, "num_pages", 2**31 - 1])
+def test_append_writes_nothing_for_a_bad_page(n, max_q, bad) -> None:
+    w = World([(n, 100), (n, 100), (n, 77)], kv_heads=2, dim=64, page=16, max_q=max_q)
+    k, v, more = _append_args(w, 2)
+    before = _snapshot(w)
+    w.cache.append(w.batch, k, v, **more)
+    w.batch.check()
+    good, q_out = _snapshot(w), more["q_out"].clone()
+    _restore(w, before)
+    last = w.table[1][99 // 16]  # the page of the second sequence's last token
+    w.batch.page_table[1, 99 // 16] = w.cache.num_pages if bad == "num_pages" else bad
+    w.cache.append(w.batch, k, v, **more)
+    with pytest.raises(RuntimeError, match="page id"):
+        w.batch.check()
+    for got, want, old in zip(_snapshot(w), good, before):
+        want[last] = old[last]
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+    assert torch.equal(more["q_out"], q_out)  # the queries need no page
+
+
+@pytest.mark.parametrize(("n", "max_q"), [(1, 1), (1, 40), (40, 40), (40, 4000)])
+@pytest.mark.parametrize("ctx", [-5, -2**31, 0, "short", "long", 2**31 - 1])
+def test_append_leaves_a_sequence_of_bad_lengths_alone(n, max_q, ctx) -> None:
+    w = World([(n, 100), (n, 100), (n, 77)], kv_heads=2, dim=64, page=16, max_q=max_q, max_ctx=100)
+    k, v, more = _append_args(w, 2)
+    before = _snapshot(w)
+    w.cache.append(w.batch, k, v, **more)
+    w.batch.check()
+    good, q_out = _snapshot(w), more["q_out"].clone()
+    _restore(w, before)
+    more["q_out"].fill_(7.0)
+    w.batch.ctx_len[1] = {"short": n - 1, "long": 101}.get(ctx, ctx)
+    w.cache.append(w.batch, k, v, **more)
+    with pytest.raises(RuntimeError, match="lengths"):
+        w.batch.check()
+    mine = w.table[1][:7]
+    for got, want, old in zip(_snapshot(w), good, before):
+        want[mine] = old[mine]
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+    q_out[n:2 * n] = 7.0
+    assert torch.equal(more["q_out"], q_out)
+
+
+@pytest.mark.parametrize("start", [[0, 30, 71, 90], [0, 30, 60, 91], [-1, 30, 60, 90]])
+@pytest.mark.parametrize("max_q", [40, 4000])
+def test_starts_out_of_bounds_hide_their_own_sequence(start, max_q) -> None:
+    """A sequence longer than max_q, one that ends behind the rows, one that starts before them: reported, and the
+    sequences before and behind are stored and answered."""
+    lens = [(b - a, 100) for a, b in zip(start, start[1:])]
+    w = World([(30, 100)] * 3, kv_heads=2, dim=64, page=16, max_q=max_q, max_ctx=100)
+    if start[2] == 71:
+        w.batch.max_q = 40
+    k, v, more = _append_args(w, 2, F16)
+    before = _snapshot(w)
+    w.batch.q_start.copy_(_ints(start))
+    bad = next(i for i, (a, b) in enumerate(zip(start, start[1:])) if a < 0 or b > 90 or b - a > 40)
+    w.cache.append(w.batch, k, v, **more)
+    with pytest.raises(RuntimeError, match="lengths"):
+        w.batch.check()
+    out = w.cache.attention(w.batch, more["q_out"])
+    with pytest.raises(RuntimeError, match="lengths"):
+        w.batch.check()
+    for x, old in zip((w.cache.k, w.cache.v, w.cache.k_scale, w.cache.v_scale), before):
+        assert torch.equal(x.view(torch.uint8)[w.table[bad][:7]], old.view(torch.uint8)[w.table[bad][:7]])
+    w.lens, w.start = lens, start
+    for b in range(3):
+        if b == bad:
+            rows = slice(max(start[b], 0), min(start[b + 1], 90, max(start[b], 0) + w.batch.max_q))
+            assert bool((out[rows] == 0).all()) and bool((more["q_out"][rows] == 7.0).all())
+        else:
+            _check_rows(w, b, more["q_out"], out)
+            pos = torch.arange(100 - lens[b][0], 100, device="cuda")
+            rows = slice(start[b], start[b + 1])
+            got = ref.gather(w.cache.v, w.cache.v_scale, w.table[b], 100)[:, pos].transpose(0, 1)
+            near = ref.E4M3_HALF_STEP * v[rows].double().abs() + 2.0**-15  # scales of 2^-5 at most
+            assert bool(((got - v[rows].double()).abs() <= near).all()) and bool((more["q_out"][rows] != 7.0).any())
