@@ -375,3 +375,49 @@ def test_starts_out_of_bounds_hide_their_own_sequence(start, max_q) -> None:
             got = ref.gather(w.cache.v, w.cache.v_scale, w.table[b], 100)[:, pos].transpose(0, 1)
             near = ref.E4M3_HALF_STEP * v[rows].double().abs() + 2.0**-15  # scales of 2^-5 at most
             assert bool(((got - v[rows].double()).abs() <= near).all()) and bool((more["q_out"][rows] != 7.0).any())
+
+
+# ---------------------------------------------------------------- far apart
+@pytest.mark.parametrize(("n", "dim", "group", "window"), [
+    (1, 64, 1, 0), (1, 256, 4, 0), (3, 128, 3, 0), (40, 64, 2, 0), (20, 256, 2, 0), (1, 128, 2, 70_001), (33, 128, 1, 70_001)])
+def test_attention_over_300000_positions(n, dim, group, window) -> None:
+    w = World([(n, 300_001), (n, 131_072)], kv_heads=1, dim=dim, page=128, seed=2)
+    q = w.rand(w.rows, group, dim, dtype=BF16)
+    out = w.cache.attention(w.batch, q, window=window)
+    _check_attention(w, q, out, scale=dim**-0.5, window=window)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_offsets_beyond_32_bits(n) -> None:
+    """Pages behind 2^32 bytes of codes, and rows 2^31 elements apart."""
+    dim, kv_heads, heads, page, pages = 256, 4, 8, 256, 20_000
+    w = World([(n, 700), (n, 900)], kv_heads=kv_heads, dim=dim, page=page)
+    far = [torch.empty(pages, kv_heads, page, dim, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.empty(pages, kv_heads, page // 16, device="cuda") for _ in range(2)]
+    move = pages - w.cache.num_pages
+    for new, old in zip((*far, *scales), (w.cache.k, w.cache.v, w.cache.k_scale, w.cache.v_scale)):
+        new[move:] = old
+    w.table = [[p + move if p >= 0 else p for p in t] for t in w.table]
+    w.batch.page_table.copy_(_ints(w.table))
+    w.cache = KV8Cache.wrap(*far, *scales)
+    before = [x[move:].clone() for x in (*far, *scales)]
+    # two rows at the ends of a long tensor each, or all of them near its start
+    step = 2**31 if w.rows == 2 else 4 * heads * dim
+    room = torch.empty(step * (w.rows - 1) + 4 * heads * dim, dtype=BF16, device="cuda")
+    at = [room[i * heads * dim:].as_strided((w.rows, h, dim), (step, dim, 1)) for i, h in enumerate((heads, heads, kv_heads, kv_heads))]
+    q, out, k, v = at
+    for x in (q, k, v):
+        x.copy_(w.rand(*x.shape))
+    was = q.clone()
+    cos, sin = ref.rope_tables(900, dim, "cuda")
+    w.cache.append(w.batch, k, v, q=q, q_out=q, cos=cos, sin=sin)
+    near = World(w.lens, kv_heads=kv_heads, dim=dim, page=page)  # the same cache, close at hand
+    q2 = was.clone()
+    near.cache.append(near.batch, k.contiguous(), v.contiguous(), q=q2, q_out=q2, cos=cos, sin=sin)
+    w.batch.check()
+    assert torch.equal(q, q2)
+    for x, y, old in zip((*far, *scales), (near.cache.k, near.cache.v, near.cache.k_scale, near.cache.v_scale), before):
+        assert torch.equal(x[move:].view(torch.uint8), y.view(torch.uint8))
+        assert not torch.equal(y.view(torch.uint8), old.view(torch.uint8))
+    w.cache.attention(w.batch, q, out)
+    _check_attention(w, q, out, scale=dim**-0.5, window=0)
