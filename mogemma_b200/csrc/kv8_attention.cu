@@ -61,6 +61,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLift = 15.0f;  // log2 of a row's largest P: 2^15 is the largest power of two in fp16
+constexpr float kUnlift = 1.0f / 32768.0f;  // 2^-kLift; apart from ex2, which ends at 2^-126: value scales may be as small
 
 // D += A . B, 16 x 8 x 16, fp16 operands, fp32 accumulators.
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -453,7 +454,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                 acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
             }
             // O is in units of 2^(M - kLift), l in units of 2^m; a row that saw nothing has l = 0
-            const float f = ll == 0.f ? 0.f : ex2(bv - b - kLift) / ll;
+            const float f = ll == 0.f ? 0.f : ex2(bv - b) * kUnlift / ll;
             acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
             if (whole) {
                 const int row = it.row0 + r, tok = row / p.a.group, hq = head * p.a.group + row - tok * p.a.group;
@@ -481,18 +482,12 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
 constexpr int kCombThreads = 256;
 constexpr int kCombPerSm = 4;
 
-struct Joined {  // a running join of parts
-    float m = -kInf, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    __device__ __forceinline__ void add(float pm, float pl, float4 v) {
-        const float mn = fmaxf(m, pm), b = mn == -kInf ? 0.f : mn;
-        const float fa = ex2(m - b), fb = pl * ex2(pm - b);
-        acc.x = acc.x * fa + v.x * fb, acc.y = acc.y * fa + v.y * fb;
-        acc.z = acc.z * fa + v.z * fb, acc.w = acc.w * fa + v.w * fb;
-        l = l * fa + fb;
-        m = mn;
-    }
-};
+// A part's share is formed before its answers are added up: times l they could pass fp32's range.
+__device__ __forceinline__ float finite_or_0(float x) { return x == -kInf ? 0.f : x; }
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : __fdividef(1.0f, l); }
+__device__ __forceinline__ void add(float4 &acc, const float4 &v, float share) {
+    acc.x += v.x * share, acc.y += v.y * share, acc.z += v.z * share, acc.w += v.w * share;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArgs p, int hd, int ctas, int few) {
@@ -546,69 +541,92 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
         if (n <= few) {  // 16 lanes hold a row, lane gl dims 64 c + 4 gl ..
             const int r = 16 * sub + grp;
             if (r >= sp.nrows) continue;
-            Joined j[4];
+            // lane i has part i's maximum and sum
+            auto part_at = [&](int i) { return static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r; };
+            const uint32_t half = 0xffffu << (lane & 16);
+            const float2 ml = gl < n ? *reinterpret_cast<const float2 *>(p.part.ml + 2 * part_at(gl)) : make_float2(-kInf, 0.f);
+            float top = ml.x;
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(half, top, o));
+            const float w = ml.y * ex2(ml.x - finite_or_0(top));
+            float l = w;
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) l += __shfl_xor_sync(half, l, o);
+            const float mine = w * inverse(l);
+            float4 acc[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
             for (int i = 0; i < n; ++i) {
-                const int64_t at = static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r;
-                const float2 ml = *reinterpret_cast<const float2 *>(p.part.ml + 2 * at);
-                float4 v[4];
+                const float share = __shfl_sync(half, mine, (lane & 16) + i);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    if (c < chunks) v[c] = *reinterpret_cast<const float4 *>(p.part.o + at * hd + 64 * c + 4 * gl);
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (c < chunks) j[c].add(ml.x, ml.y, v[c]);
+                    if (c < chunks) add(acc[c], *reinterpret_cast<const float4 *>(p.part.o + part_at(i) * hd + 64 * c + 4 * gl), share);
             }
             T *dst = out_at(sp, r) + 4 * gl;
-            const float f = j[0].l == 0.f ? 0.f : 1.0f / j[0].l;
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                if (c < chunks) store_out4(dst + 64 * c, j[c].acc.x * f, j[c].acc.y * f, j[c].acc.z * f, j[c].acc.w * f);
+                if (c < chunks) store_out4(dst + 64 * c, acc[c].x, acc[c].y, acc[c].z, acc[c].w);
             continue;
         }
         // 4 lanes hold 16 dims of the row, every 64th part per 4 lanes
         const int r = sub / fine, d = 16 * (sub % fine) + 4 * (tid & 3);
-        Joined j;
-#pragma unroll 4
-        for (int i = tid >> 2; i < n; i += kCombThreads / 4) {
-            const int64_t at = static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r;
-            const float2 ml = *reinterpret_cast<const float2 *>(p.part.ml + 2 * at);
-            j.add(ml.x, ml.y, *reinterpret_cast<const float4 *>(p.part.o + at * hd + d));
+        float m = -kInf, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kAt = 4;  // parts at a time
+        for (int i0 = tid >> 2; i0 < n; i0 += kAt * (kCombThreads / 4)) {
+            float2 ml[kAt];
+            float4 v[kAt];
+#pragma unroll
+            for (int k = 0; k < kAt; ++k) {
+                const int i = i0 + k * (kCombThreads / 4);
+                const int64_t at = static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r;
+                ml[k] = i < n ? *reinterpret_cast<const float2 *>(p.part.ml + 2 * at) : make_float2(-kInf, 0.f);
+                v[k] = i < n ? *reinterpret_cast<const float4 *>(p.part.o + at * hd + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            const float mn = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)), b = finite_or_0(mn);
+            const float old = l * ex2(m - b);
+            l = old;
+#pragma unroll
+            for (int k = 0; k < kAt; ++k) l += ml[k].y *= ex2(ml[k].x - b);
+            m = mn;
+            const float inv = inverse(l), so = old * inv;
+            acc.x *= so, acc.y *= so, acc.z *= so, acc.w *= so;
+#pragma unroll
+            for (int k = 0; k < kAt; ++k) add(acc, v[k], ml[k].y * inv);
         }
         // join the warp's 8 groups, then the warps
+        float top = m;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float w = l * ex2(m - finite_or_0(top));
+        l = w;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float share = w * inverse(l);
+        acc.x *= share, acc.y *= share, acc.z *= share, acc.w *= share;
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
-            const float om = __shfl_xor_sync(0xffffffffu, j.m, o), ol = __shfl_xor_sync(0xffffffffu, j.l, o);
-            float4 v;
-            v.x = __shfl_xor_sync(0xffffffffu, j.acc.x, o), v.y = __shfl_xor_sync(0xffffffffu, j.acc.y, o);
-            v.z = __shfl_xor_sync(0xffffffffu, j.acc.z, o), v.w = __shfl_xor_sync(0xffffffffu, j.acc.w, o);
-            const float top = fmaxf(j.m, om), b = top == -kInf ? 0.f : top;
-            const float fa = ex2(j.m - b), fb = ex2(om - b);
-            j.acc.x = j.acc.x * fa + v.x * fb, j.acc.y = j.acc.y * fa + v.y * fb;
-            j.acc.z = j.acc.z * fa + v.z * fb, j.acc.w = j.acc.w * fa + v.w * fb;
-            j.l = j.l * fa + ol * fb;
-            j.m = top;
+            acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o), acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+            acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o), acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
         }
         if (lane < 4) {
-            acc_s[warp][lane] = j.acc;
-            if (lane == 0) ml_s[warp] = make_float2(j.m, j.l);
+            acc_s[warp][lane] = acc;
+            if (lane == 0) ml_s[warp] = make_float2(top, l);
         }
         __syncthreads();
         if (tid < 4) {
-            j = Joined();
-            float top = -kInf;
+            constexpr int kW = kCombThreads / 32;
+            float all = -kInf, sum = 0.f, ws[kW];
 #pragma unroll
-            for (int i = 0; i < kCombThreads / 32; ++i) top = fmaxf(top, ml_s[i].x);
-            const float b = top == -kInf ? 0.f : top;
+            for (int i = 0; i < kW; ++i) all = fmaxf(all, ml_s[i].x);
 #pragma unroll
-            for (int i = 0; i < kCombThreads / 32; ++i) {
-                const float f = ex2(ml_s[i].x - b);
-                const float4 v = acc_s[i][tid];
-                j.acc.x += v.x * f, j.acc.y += v.y * f, j.acc.z += v.z * f, j.acc.w += v.w * f;
-                j.l += ml_s[i].y * f;
-            }
-            const float f = j.l == 0.f ? 0.f : 1.0f / j.l;
-            store_out4(out_at(sp, r) + d, j.acc.x * f, j.acc.y * f, j.acc.z * f, j.acc.w * f);
+            for (int i = 0; i < kW; ++i) sum += ws[i] = ml_s[i].y * ex2(ml_s[i].x - finite_or_0(all));
+            const float inv = inverse(sum);
+            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < kW; ++i) add(acc, acc_s[i][tid], ws[i] * inv);
+            store_out4(out_at(sp, r) + d, acc.x, acc.y, acc.z, acc.w);
         }
         __syncthreads();
     }

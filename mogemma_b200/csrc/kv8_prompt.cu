@@ -78,7 +78,7 @@ constexpr float kInf = __builtin_huge_valf();
 // 2^15.9, within fp16.  A higher lift keeps more of the weights far below the row's largest (down to 2^(-24 - kLift)) and
 // rescales more often: lift 0, 6, 8, 13 take 261, 266, 272, 284 us for the 27B prompt below, whose key scales lie 8
 // times apart, and 259 us each where they are alike.
-constexpr float kLift = 8.0f;
+constexpr float kLift = 8.0f, kUnlift = 1.0f / 256.0f;  // 2^-kLift apart from ex2, which ends at 2^-126
 constexpr float kRescale = 15.9f - kLift;
 constexpr int kRing = 4;  // units whose scales are at hand
 
@@ -844,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
             if (any_rows) {
                 const int slot = d->slot;
                 const bool whole = slot < 0;
-                const float f = l == 0.f || !begun ? 0.f : ex2(finite_or_0(mref) - finite_or_0(m) - kLift) / l;
+                const float f = l == 0.f || !begun ? 0.f : ex2(finite_or_0(mref) - finite_or_0(m)) * kUnlift / l;
                 const int row = d->row0 + tg * kM + r, tok = row / p.a.group, hq = d->head * p.a.group + row - tok * p.a.group;
                 T *dst = static_cast<T *>(p.out) + (static_cast<int64_t>(d->q0) + tok) * p.out_row + hq * p.out_head;
                 const int64_t at = static_cast<int64_t>(slot) * C::kRows + tg * kM + r;

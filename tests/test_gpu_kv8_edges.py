@@ -421,3 +421,14 @@ def test_offsets_beyond_32_bits(n) -> None:
         assert not torch.equal(y.view(torch.uint8), old.view(torch.uint8))
     w.cache.attention(w.batch, q, out)
     _check_attention(w, q, out, scale=dim**-0.5, window=0)
+
+
+@pytest.mark.parametrize(("n", "dim"), [(1, 64), (1, 256), (8, 128), (40, 64), (40, 256)])
+@pytest.mark.parametrize("power", [-120, -100, 100, 118])
+def test_value_scales_near_the_ends_of_the_range(n, dim, power) -> None:
+    w = World([(n, 300), (n, 65)], kv_heads=2, dim=dim, page=32)
+    w.cache.v_scale.fill_(2.0**power)
+    q = w.rand(w.rows, 4, dim, dtype=BF16)
+    out = w.cache.attention(w.batch, q)
+    _check_attention(w, q, out, scale=dim**-0.5, window=0)
+    assert bool((out != 0).any())
