@@ -123,6 +123,9 @@ struct Item {
     int lo, hi;          // positions its rows see lie in [lo, hi)
     int unit0, units;    // units unit0 .. unit0 + units - 1
     int cost;            // extra + units; 0: no rows
+    // The pair to go on to: behind a tile without rows its sequence has no more.  (max_q may be far above most lengths:
+    // one visit per tile kept the prompt kernel's roles waiting for the next item, 4 million tiles beyond 20 ms.)
+    int after;
 };
 __device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, int pair, bool report) {
     Item it;
@@ -131,6 +134,7 @@ __device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, in
     it.row0 = t * a.rows;
     it.nrows = min(a.rows, it.seq.nq * a.group - it.row0);
     it.units = it.cost = 0;
+    it.after = it.nrows > 0 ? pair + 1 : (i + 1) * a.tiles;
     if (it.nrows <= 0) return it;
     const int first = it.seq.pos0 + it.row0 / a.group, last = it.seq.pos0 + (it.row0 + it.nrows - 1) / a.group;
     it.lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
@@ -139,12 +143,6 @@ __device__ __forceinline__ Item load_item(const Batch &b, const AttnShape &a, in
     it.units = max(1, (it.hi + a.unit - 1) / a.unit - it.unit0);
     it.cost = it.units + a.extra;
     return it;
-}
-
-// The pair to go on to: behind a tile without rows its sequence has no more.  (max_q may be far above most lengths:
-// one visit per tile kept the prompt kernel's roles waiting for the next item, 4 million tiles beyond 20 ms.)
-__device__ __forceinline__ int pair_after(const AttnShape &a, int pair, const Item &it) {
-    return it.cost > 0 ? pair + 1 : (pair / a.tiles + 1) * a.tiles;
 }
 
 // Where CTA `cta` of `ctas` starts: its range [w0, w1) of the whole cost, and
@@ -168,7 +166,7 @@ __device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, 
     for (int p = p0; p < p1;) {
         const Item it = load_item(b, a, p, cta == 0);
         mine += it.cost;
-        p = pair_after(a, p, it);
+        p = it.after;
     }
     int64_t upto = mine;
 #pragma unroll
@@ -197,7 +195,7 @@ __device__ __forceinline__ Place find_place(const Batch &b, const AttnShape &a, 
         int p = p0;
         for (;;) {
             const Item it = load_item(b, a, p, false);
-            const int next = pair_after(a, p, it);
+            const int next = it.after;
             if (left < it.cost || next >= p1) break;
             left -= it.cost;
             p = next;
@@ -236,7 +234,7 @@ struct Walk {
     __device__ __forceinline__ void step(const Batch &b, const AttnShape &a) {
         w += it.cost > 0 ? it.cost - skip : 0;
         skip = 0;
-        pair = pair_after(a, pair, it);
+        pair = it.after;
         if (pair >= b.batch * a.tiles) pair = 0, ++head;
     }
     __device__ __forceinline__ bool start(const Batch &b, const AttnShape &a, const Place &pl) {
