@@ -543,6 +543,13 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
             if (r >= sp.nrows) continue;
             // lane i has part i's maximum and sum
             auto part_at = [&](int i) { return static_cast<int64_t>(2 * (first + i) + (i == 0 ? 1 : 0)) * p.a.rows + r; };
+            auto load = [&](float4 (&v)[4], int i) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (c < chunks) v[c] = *reinterpret_cast<const float4 *>(p.part.o + part_at(i) * hd + 64 * c + 4 * gl);
+            };
+            float4 v0[4];  // on its way while the shares are formed
+            load(v0, 0);
             const uint32_t half = 0xffffu << (lane & 16);
             const float2 ml = gl < n ? *reinterpret_cast<const float2 *>(p.part.ml + 2 * part_at(gl)) : make_float2(-kInf, 0.f);
             float top = ml.x;
@@ -556,12 +563,16 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
             float4 acc[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-            for (int i = 0; i < n; ++i) {
+            auto take = [&](const float4 (&v)[4], int i) {
                 const float share = __shfl_sync(half, mine, (lane & 16) + i);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    if (c < chunks) add(acc[c], *reinterpret_cast<const float4 *>(p.part.o + part_at(i) * hd + 64 * c + 4 * gl), share);
+                    if (c < chunks) add(acc[c], v[c], share);
+            };
+            for (int i = 0;;) {
+                take(v0, i);
+                if (++i == n) break;
+                load(v0, i);
             }
             T *dst = out_at(sp, r) + 4 * gl;
 #pragma unroll
