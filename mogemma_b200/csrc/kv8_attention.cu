@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
             float up = 1.0f, down = 1.0f;
             if (e >= 255) {
                 down = __int_as_float(0x7fc00000);
-            } else if (e > 0) {
+            } else if (most > 0) {  // bf16 subnormals too: e is 0
                 const int sh = min(142 - e, 126);  // exponent of `up`; |sh| <= 126 keeps both normal
                 up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
                 down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);

@@ -432,3 +432,14 @@ def test_value_scales_near_the_ends_of_the_range(n, dim, power) -> None:
     out = w.cache.attention(w.batch, q)
     _check_attention(w, q, out, scale=dim**-0.5, window=0)
     assert bool((out != 0).any())
+
+
+@pytest.mark.parametrize(("n", "dim"), [(1, 64), (8, 128), (2, 256), (40, 64), (40, 256)])
+def test_query_rows_of_subnormals(n, dim) -> None:
+    """bf16 rows below 2^-126, brought back by the scale; fp16 rows below 2^-14."""
+    w = World([(n, 300), (n, 65)], kv_heads=2, dim=dim, page=32)
+    for dtype, power in ((BF16, 129), (F16, 20)):
+        q = (w.rand(w.rows, 4, dim) * 2.0**-power).to(dtype)
+        scale = 2.0**(power - 3)
+        out = w.cache.attention(w.batch, q, scale=scale)
+        _check_attention(w, q, out, scale=scale, window=0)
