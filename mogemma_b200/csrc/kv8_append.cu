@@ -510,6 +510,10 @@ extern "C" mg_status mg_kv8_append(const mg_kv8_cache *cache, const mg_kv8_batch
         (args->out_dtype != args->dtype || args->out_row_stride != args->q_row_stride ||
          args->out_head_stride != args->q_head_stride))
         return report_error(MG_ERR_INVALID, "mg_kv8_append: q_out may be q only with its dtype and strides");
+    // the one-token form: a group of head_dim / 8 lanes per sequence and kv head
+    if (batch->max_q == 1 &&
+        static_cast<int64_t>(batch->batch) * cache->num_kv_heads > INT32_MAX * static_cast<int64_t>(kTokenThreads / (cache->head_dim / 8)))
+        return report_error(MG_ERR_UNSUPPORTED, "mg_kv8_append: batch * num_kv_heads too large");
     AppendParams p;
     p.c = cache_of(cache);
     p.b = batch_of(batch);

@@ -7,7 +7,7 @@ import subprocess
 import sys
 
 import pytest
-from test_kv8 import INVALID, LIB, P, _append, _attention, _batch, _cache, _refused
+from test_kv8 import INVALID, LIB, P, UNSUPPORTED, _append, _attention, _batch, _cache, _refused
 
 torch = pytest.importorskip("torch")
 
@@ -78,3 +78,10 @@ def test_a_star_import_needs_no_torch() -> None:
     from mogemma_b200 import KV8Batch as by_name
 
     assert by_name is KV8Batch
+
+
+def test_more_single_tokens_than_a_grid_holds_are_refused() -> None:
+    """2^20 sequences of 2^13 kv heads of 256 would be 2^31 CTAs, one beyond the largest grid."""
+    cache = _cache(num_kv_heads=1 << 13, head_dim=256, token_stride=256, head_stride=8192, page_stride=1 << 26)
+    batch = _batch(batch=1 << 20, max_q=1)
+    _refused(LIB.mg_kv8_append, cache, batch, _append(num_heads=0), UNSUPPORTED, "too large")
