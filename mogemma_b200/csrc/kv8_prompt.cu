@@ -321,13 +321,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
         budget_s = p.wait_ns;
         fence_barrier_init();
     }
+    // before the allocation: a predecessor that lets this kernel begin early may still have to allocate TMEM itself, and
+    // would wait for this kernel, which waits for it
+    kernel_begins();
     if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                      "r"(kTmemCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    kernel_begins();
     const Place pl = find_place<kThreads>(p.b, p.a, p.c.heads, cta, gridDim.x);
     tc::tc_fence_before();
     __syncthreads();
