@@ -443,3 +443,34 @@ def test_query_rows_of_subnormals(n, dim) -> None:
         scale = 2.0**(power - 3)
         out = w.cache.attention(w.batch, q, scale=scale)
         _check_attention(w, q, out, scale=scale, window=0)
+
+
+@pytest.mark.parametrize(("n", "dim", "group"), [(600, 64, 1), (600, 128, 2), (300, 256, 2), (1, 128, 4), (5, 256, 2)])
+def test_a_non_finite_token_far_behind(n, dim, group) -> None:
+    """Where whole units are seen: every query from the token on answers NaN, also long after it, and no other."""
+    w = World([(n, 900), (n, 700)], kv_heads=2, dim=dim, page=64)
+    q, bad = w.rand(w.rows, 2 * group, dim, dtype=BF16), 450
+    good = w.cache.attention(w.batch, q)
+    w.cache.k.view(torch.uint8)[w.table[0][bad // 64], 1, bad % 64] = 0x7F  # as the append stores it: K NaN, V 0
+    w.cache.v.view(torch.uint8)[w.table[0][bad // 64], 1, bad % 64] = 0
+    out = w.cache.attention(w.batch, q)
+    windowed = w.cache.attention(w.batch, q, window=100)
+    w.batch.check()
+    first = max(0, bad - (900 - n))  # the first row that sees it
+    assert bool(out[first:n, group:].isnan().all())
+    assert torch.equal(out[:first], good[:first]) and torch.equal(out[n:], good[n:])
+    assert torch.equal(out[:n, :group], good[:n, :group])
+    for i in (first, first + 99, first + 100, n - 1):
+        if i < n:
+            sees = bad <= 900 - n + i < bad + 100
+            assert bool(windowed[i, group:].isnan().all() if sees else windowed[i, group:].isfinite().all())
+    assert bool(windowed[n:].isfinite().all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize(("n", "group"), [(1, 33), (1, 128), (3, 100), (7, 128), (1, 17), (2, 13)])
+def test_many_heads_to_a_kv_head(dim, n, group) -> None:
+    w = World([(n, 500), (n, 31), (n, 129)], kv_heads=1, dim=dim, page=16)
+    q = w.rand(w.rows, group, dim, dtype=F16)
+    out = w.cache.attention(w.batch, q, window=200)
+    _check_attention(w, q, out, scale=dim**-0.5, window=200)
