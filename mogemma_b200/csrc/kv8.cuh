@@ -75,12 +75,7 @@ cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, size_t s
 }
 
 // ---- e4m3 <-> wider.  Codes convert to fp16 exactly (448 and 2^-9 are both in its range).
-__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t two) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
-    return r;
-}
-// Both halves of a word: codes 0, 1 and codes 2, 3.
+// A word's codes 0, 1 and codes 2, 3.
 __device__ __forceinline__ void e4m3x4_to_h2x2(uint32_t four, uint32_t &a, uint32_t &b) {
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
         "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
@@ -101,6 +96,43 @@ __device__ __forceinline__ float ex2(float x) {  // PTX ex2.approx: one MUFU op,
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+constexpr float kInf = __builtin_huge_valf();
+__device__ __forceinline__ float finite_or_0(float x) { return x == -kInf ? 0.f : x; }
+
+// ---- query rows.  Two values of type T in a word, as floats and back.
+template <typename T>
+__device__ __forceinline__ float2 two(uint32_t w);
+template <>
+__device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 two<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ uint32_t pack(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// The power of two that brings a row's largest magnitude (as bits) to [2^15, 2^16), fp16's last binade, and its inverse:
+// fp16 rows then stay as they are, bf16 values exact down to 2^-32 of the largest.  A row with an infinity or NaN gets
+// NaN for the inverse and answers NaN.
+__device__ __forceinline__ void row_scale(uint32_t most, float &up, float &down) {
+    const int e = static_cast<int>(most >> 23);
+    up = down = 1.0f;
+    if (e >= 255) {
+        down = __int_as_float(0x7fc00000);
+    } else if (most > 0) {  // bf16 subnormals too: e is 0
+        const int sh = min(142 - e, 126);  // exponent of `up`; |sh| <= 126 keeps both normal
+        up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
+        down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
+    }
 }
 
 // ---- the attention's schedule

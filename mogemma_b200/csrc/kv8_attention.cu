@@ -59,7 +59,6 @@ constexpr int kRows = 8;       // query rows of an MMA; an item has 8 or 16
 constexpr int kUnit = 64;      // tokens of a unit of the schedule
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr float kInf = __builtin_huge_valf();
 constexpr float kLift = 15.0f;  // log2 of a row's largest P: 2^15 is the largest power of two in fp16
 constexpr float kUnlift = 1.0f / 32768.0f;  // 2^-kLift; apart from ex2, which ends at 2^-126: value scales may be as small
 
@@ -75,28 +74,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-// 2 query values of type T as floats.
-template <typename T>
-__device__ __forceinline__ float2 two(uint32_t w);
-template <>
-__device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t w) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ float2 two<__half>(uint32_t w) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-}
 __device__ __forceinline__ void store_out4(__half *p, float a, float b, float c, float d) {
-    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_h2(a, b), pack_h2(c, d));
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack(a, b, __half()), pack(c, d, __half()));
 }
 __device__ __forceinline__ void store_out4(__nv_bfloat16 *p, float a, float b, float c, float d) {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
-    *reinterpret_cast<uint2 *>(p) =
-        make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+    *reinterpret_cast<uint2 *>(p) = make_uint2(pack(a, b, __nv_bfloat16()), pack(c, d, __nv_bfloat16()));
 }
 __device__ __forceinline__ float max_over_rows(float v) {  // over the 8 lanes that share lane % 4
 #pragma unroll
@@ -241,23 +223,14 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                 }
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-            // a power of two that brings the row's maximum to [2^15, 2^16), fp16's last binade: fp16 values then stay
-            // as they are, bf16 values down to 2^-32 of it.  A row with an infinity or NaN answers NaN.
-            const int e = static_cast<int>(most >> 23);
-            float up = 1.0f, down = 1.0f;
-            if (e >= 255) {
-                down = __int_as_float(0x7fc00000);
-            } else if (most > 0) {  // bf16 subnormals too: e is 0
-                const int sh = min(142 - e, 126);  // exponent of `up`; |sh| <= 126 keeps both normal
-                up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
-                down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
-            }
+            float up, down;
+            row_scale(most, up, down);
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float2 f = two<T>(raw[c][i]);
-                    qf[nt][c][i >> 1][i & 1] = pack_h2(f.x * up, f.y * up);
+                    qf[nt][c][i >> 1][i & 1] = pack(f.x * up, f.y * up, __half());
                 }
             // columns 2 t, 2 t + 1 of the accumulators are rows held by lanes 8 t, 8 t + 4
 #pragma unroll
@@ -341,8 +314,8 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                 for (int c = 0; c < 2; ++c) {
                     const float mn = fmaxf(m[nt][c], max_over_rows(top[c]));
                     const float vn = fmaxf(mv[nt][c], max_over_rows(topv[c]));
-                    base[nt][c] = mn == -kInf ? 0.f : mn;
-                    basev[nt][c] = vn == -kInf ? 0.f : vn;
+                    base[nt][c] = finite_or_0(mn);
+                    basev[nt][c] = finite_or_0(vn);
                     l[nt][c] *= ex2(m[nt][c] - base[nt][c]);
                     moved |= vn != mv[nt][c];
                     top[c] = ex2(mv[nt][c] - basev[nt][c]);  // O's factor
@@ -368,8 +341,8 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
                         l[nt][e & 1] += ex2(s[i][nt][e] - base[nt][e & 1]);
                         pr[e] = ex2(s[i][nt][e] + (lv[i] + kLift) - basev[nt][e & 1]);
                     }
-                    b0[nt] = transpose8x8(pack_h2(pr[0], pr[1]));
-                    b1[nt] = transpose8x8(pack_h2(pr[2], pr[3]));
+                    b0[nt] = transpose8x8(pack(pr[0], pr[1], __half()));
+                    b1[nt] = transpose8x8(pack(pr[2], pr[3], __half()));
                 }
                 // lane's V: tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9, bytes kVB (8 h + g) .. of each
                 const unsigned char *row = vt + (16 * i + 2 * t) * Cfg::kRow + Cfg::kVB * g;
@@ -444,7 +417,7 @@ __global__ void __launch_bounds__(kThreads) kv8_rows_kernel(const AttnArgs p) {
             float mm = -kInf, mmv = -kInf, ll = 0.f;
 #pragma unroll
             for (int i = 0; i < kWarps; ++i) mm = fmaxf(mm, mlm[i][r][0]), mmv = fmaxf(mmv, mlm[i][r][2]);
-            const float b = mm == -kInf ? 0.f : mm, bv = mmv == -kInf ? 0.f : mmv;
+            const float b = finite_or_0(mm), bv = finite_or_0(mmv);
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < kWarps; ++i) {
@@ -483,7 +456,6 @@ constexpr int kCombThreads = 256;
 constexpr int kCombPerSm = 4;
 
 // A part's share is formed before its answers are added up: times l they could pass fp32's range.
-__device__ __forceinline__ float finite_or_0(float x) { return x == -kInf ? 0.f : x; }
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : __fdividef(1.0f, l); }
 __device__ __forceinline__ void add(float4 &acc, const float4 &v, float share) {
     acc.x += v.x * share, acc.y += v.y * share, acc.z += v.z * share, acc.w += v.w * share;

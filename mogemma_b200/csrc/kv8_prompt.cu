@@ -73,7 +73,6 @@ namespace {
 constexpr int kM = 128;   // rows of a tile
 constexpr int kN = 128;   // tokens of a unit
 constexpr int kThreads = 640;
-constexpr float kInf = __builtin_huge_valf();
 // log2 of P at a row's reference M, and how far the maximum may grow past M before O is rescaled: P stays below
 // 2^15.9, within fp16.  A higher lift keeps more of the weights far below the row's largest (down to 2^(-24 - kLift)) and
 // rescales more often: lift 0, 6, 8, 13 take 261, 266, 272, 284 us for the 27B prompt below, whose key scales lie 8
@@ -161,25 +160,6 @@ __device__ __forceinline__ uint4 ldg16(const uint8_t *p) {
                  : "l"(p));
     return v;
 }
-template <typename T>
-__device__ __forceinline__ float2 two(uint32_t w);
-template <>
-__device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t w) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ float2 two<__half>(uint32_t w) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-}
-__device__ __forceinline__ uint32_t pack(float a, float b, __half) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // Bounded wait.  err_dev may hold a bad page's code already, so a stop is announced in shared memory.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t *err,
                                      const volatile uint64_t *budget) {
@@ -228,7 +208,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float finite_or_0(float x) { return x == -kInf ? 0.f : x; }
 
 template <int N>
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[N]) {
@@ -618,15 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prompt_kernel(const AttnArgs 
                         }
                         most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
                         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                        const int e = static_cast<int>(most >> 23);
-                        float up = 1.0f, down = 1.0f;
-                        if (e >= 255) {  // a row with an infinity or NaN answers NaN
-                            down = __int_as_float(0x7fc00000);
-                        } else if (most > 0) {  // bf16 subnormals too: e is 0
-                            const int sh = min(142 - e, 126);
-                            up = __uint_as_float(static_cast<uint32_t>(127 + sh) << 23);
-                            down = __uint_as_float(static_cast<uint32_t>(127 - sh) << 23);
-                        }
+                        float up, down;
+                        row_scale(most, up, down);
                         if (p.scale_log2 < 0.f) up = -up;  // factors of S stay positive
                         if (lr < nrows) {
                             if (sub == 0) q_down[lr] = down;
