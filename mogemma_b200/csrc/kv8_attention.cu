@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
         const int r = sub / fine, d = 16 * (sub % fine) + 4 * (tid & 3);
         float m = -kInf, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr int kAt = 4;  // parts at a time
+        constexpr int kAt = 5;  // parts at a time: all of one item's on 148 SMs (two CTAs each, 64 groups here)
         for (int i0 = tid >> 2; i0 < n; i0 += kAt * (kCombThreads / 4)) {
             float2 ml[kAt];
             float4 v[kAt];
@@ -567,8 +567,10 @@ __global__ void __launch_bounds__(kCombThreads) kv8_combine_kernel(const AttnArg
                 ml[k] = i < n ? *reinterpret_cast<const float2 *>(p.part.ml + 2 * at) : make_float2(-kInf, 0.f);
                 v[k] = i < n ? *reinterpret_cast<const float4 *>(p.part.o + at * hd + d) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            const float mn = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)), b = finite_or_0(mn);
-            const float old = l * ex2(m - b);
+            float mn = m;
+#pragma unroll
+            for (int k = 0; k < kAt; ++k) mn = fmaxf(mn, ml[k].x);
+            const float b = finite_or_0(mn), old = l * ex2(m - b);
             l = old;
 #pragma unroll
             for (int k = 0; k < kAt; ++k) l += ml[k].y *= ex2(ml[k].x - b);
