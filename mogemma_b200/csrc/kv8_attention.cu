@@ -50,7 +50,10 @@ mg_status check_cache_batch(const char *who, const mg_kv8_cache *c, const mg_kv8
 Cache cache_of(const mg_kv8_cache *c);
 Batch batch_of(const mg_kv8_batch *b);
 // kv8_prompt.cu
-constexpr int kPromptUnit = 128, kPromptExtra = 3;
+constexpr int kPromptUnit = 128;
+// What an item's start and end cost, in units: with 0, 3, 6 the 27B prompt takes 322, 270, 282 us, two chunks of 512
+// before 8192 positions (hd 256) 105, 97, 101, ragged prompts of hd 64 41.8, 39.4, 41.4, two prompts of 300 tokens 23.4 each.
+constexpr int kPromptExtra = 3;
 int prompt_rows(int hd);
 cudaError_t launch_prompt(const AttnArgs &p, int hd, bool f16, int ctas, cudaStream_t s);
 
@@ -648,7 +651,7 @@ cudaError_t launch_rows(const AttnArgs &p, int ctas, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_combine(const AttnArgs &p, int hd, int ctas, int sms, cudaStream_t s) {
     // parts up to which an item is joined by rows: more where there are many items to fill the grid with (48 items of 6
-    // to 9 parts: 40 us -> 37 with 16; one item of 10 parts: 2 us slower with 16 than with 8)
+    // to 9 parts: 36.0 us with 8, 31.2 with 16; one item of 10 parts: 9.9 with 8, 11.1 with 16; ten other shapes alike)
     const int few = static_cast<int64_t>(p.b.batch) * p.a.tiles * p.c.heads >= 32 ? 16 : 8;
     return launch_behind(kv8_combine_kernel<T>, dim3(kCombPerSm * sms), kCombThreads,
                          sizeof(int) * static_cast<size_t>(ctas), s, p, hd, ctas, few);
