@@ -290,13 +290,21 @@ mg_status mg_tp_disconnect(mg_model *m);
  * part of wider ones).
  * All of it is read on the device when the kernels run, so a captured call may
  * be replayed with new lengths, tables and rows within those bounds.
+ * max_q chooses the kernels: from more than 32 query rows per kv head (tokens of
+ * a sequence times q heads of the group) on, every sequence runs in the tensor
+ * core form, whose tiles have 128 or 256 rows, so a bound far above the lengths,
+ * or single tokens in one batch with a long chunk, cost several times what a
+ * batch of each kind costs.
  *
  * err_dev is a device word that receives a nonzero code (the first one stays):
  * MG_KV8_ERR_LENGTHS when a length breaks the bounds (the sequence's tokens are
- * not stored and its queries answer 0), MG_KV8_ERR_PAGE when a page id that is
- * needed is outside [0, num_pages) (its tokens are neither stored nor seen);
- * nothing outside the tensors is touched.  MG_KV8_ERR_WAIT: a bounded wait
- * inside a kernel expired and the call's answers are not complete.
+ * not stored and its queries, the first max_q of them that are rows, answer 0),
+ * MG_KV8_ERR_PAGE when a page id that is needed is outside [0, num_pages) (its
+ * tokens are neither stored nor seen); nothing outside the tensors is touched.
+ * Where q_start falls, sequences claim each other's rows: those are written by
+ * any of them, and the error is all that the call promises.
+ * MG_KV8_ERR_WAIT: a bounded wait inside a kernel expired and the call's answers
+ * are not complete.
  * Both calls run on `stream` (a cudaStream_t of the current device; NULL: the
  * legacy default stream) without allocating or synchronising. */
 #define MG_KV8_BLOCK 16
@@ -360,11 +368,18 @@ mg_status mg_kv8_append(const mg_kv8_cache *cache, const mg_kv8_batch *batch, co
  * multiple of num_kv_heads, at most 128 per kv head; rows as above with strides
  * in multiples of 8 elements and 16-byte aligned data.
  * out overlaps no other tensor of the call, q neither.
+ * The weights of the values are fp16 in the products, relative to a row's
+ * largest weight (times value scale): exact to 2^-11 of themselves down to 2^-29
+ * of it (more than 32 query rows per kv head: 2^-22), to 2^-40 (2^-33) of it below,
+ * where a term ends.  Their sum, the scores and the answers' sums are fp32.  bf16
+ * query elements below 2^-32 of their row's largest lose bits.  |scale| at most
+ * 2.35e38.
  * V codes must be finite (the append writes no others); the cache's content
  * behind ctx_len is never used, nor are pages that lie before every window.
  * The workspace (16-byte aligned, mg_kv8_attention_workspace bytes on this
  * device for these cache dimensions and bounds) needs no initial value and
- * keeps nothing between calls: calls that may overlap need one each. */
+ * keeps nothing between calls: calls that may overlap need one each, others (a
+ * model's layers) may share one. */
 typedef struct mg_kv8_attention_args {
     int32_t struct_size; /* sizeof(mg_kv8_attention_args) */
     int32_t dtype, num_heads, window;

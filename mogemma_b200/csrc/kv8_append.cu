@@ -21,9 +21,12 @@
 // Measured (launches in a graph; a plain copy on this GPU reaches 6.46 TB/s):
 // one token of 4 q and 1 kv heads of 256, 3.5 us, bound by the launch (4.8 in
 // the block form); 128 tokens of 32 and 16 heads of 128 in fp16, 3.8 us (12.6
-// in the block form); 7500 fp32 prompt tokens of 8 and 4 heads of 256, 31 us,
+// in the block form); 5451 fp32 prompt tokens of 8 and 4 heads of 256, 31 us,
 // 4.2 TB/s; one prompt of 16384 bf16 tokens of 32 and 16 heads of 128, 96 us,
 // 5.0 TB/s (43 and 133 us while a token's rows were loaded one after another).
+// Call by call, without a graph, 4.0 us for either decode step and 99 to 101 us
+// (4.8 TB/s) for the long prompt.  The block form spills a little at 64 registers
+// (fp32 32 bytes, fp16 8); with room for them an SM holds fewer CTAs.
 #include "kv8.cuh"
 
 #include <cstdio>
@@ -136,7 +139,7 @@ __device__ __forceinline__ uint32_t most_of(const float (&x)[8]) {
     uint32_t most = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
-    if constexpr (HD == 256) {  // a group is a warp: one instruction (7500 fp32 prompt tokens: 32 us -> 31)
+    if constexpr (HD == 256) {  // a group is a warp: one instruction (5451 fp32 prompt tokens: 32 us -> 31)
         return __reduce_max_sync(0xffffffffu, most);
     } else {
 #pragma unroll

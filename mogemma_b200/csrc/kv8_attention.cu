@@ -22,11 +22,12 @@
 // ahead, 64 KB per SM at most were in flight: 4.3 TB/s on 1.37 GB of cache
 // where the ring reaches 5.8.
 //
-// Measured (in a graph, with the combine): 32 tokens over 16384 positions each,
-// 32 / 16 heads of 128, 235 us, 5.8 TB/s; one token over 131072 positions, 4 / 1
-// heads of 256, 24 us, 2.8 TB/s; one over 640 positions, 9.7 us, which is
-// latency alone: two launches, the scan for a CTA's place, the page look-up, two
-// steps and the join.
+// Measured (in a graph, with the combine): 32 tokens over 4096 to 16384 positions
+// each, 10.4 thousand on average, 32 / 16 heads of 128, 226 to 236 us, 5.8 to 6.1
+// TB/s (255 us, 5.4 TB/s, call by call); one token over 131072 positions, 4 / 1
+// heads of 256, 24 us, 2.8 TB/s; one over 640 positions, 10 us, which is latency
+// alone: two launches, the scan for a CTA's place, the page look-up, two steps
+// and the join.
 //
 // With s = scale log2(e) k_scale <q, k> the state per row is m = max s,
 // l = sum 2^(s - m) and the sum of P V with P = 2^(s + log2 v_scale - M + 15),
@@ -51,8 +52,8 @@ Cache cache_of(const mg_kv8_cache *c);
 Batch batch_of(const mg_kv8_batch *b);
 // kv8_prompt.cu
 constexpr int kPromptUnit = 128;
-// What an item's start and end cost, in units: with 0, 3, 6 the 27B prompt takes 322, 270, 282 us, two chunks of 512
-// before 8192 positions (hd 256) 105, 97, 101, ragged prompts of hd 64 41.8, 39.4, 41.4, two prompts of 300 tokens 23.4 each.
+// What an item's start and end cost, in units: with 0, 3, 6 the 27B prompt takes 322, 270, 282 us, chunks of 512 and 365
+// tokens at 8192 and 5844 positions (hd 256) 105, 97, 101, ragged prompts of hd 64 41.8, 39.4, 41.4, two prompts of 300 tokens 23.4 each.
 constexpr int kPromptExtra = 3;
 int prompt_rows(int hd);
 cudaError_t launch_prompt(const AttnArgs &p, int hd, bool f16, int ctas, cudaStream_t s);

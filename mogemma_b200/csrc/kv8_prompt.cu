@@ -49,15 +49,16 @@
 // half the work (48 cycles per MMA against 64 for N = 128), and the waits
 // between roles (200 to 300 cycles each) came twice as often.
 //
-// Measured (in a graph, with the combine): 4096 bf16 tokens of 32 q and 16 kv
-// heads of 128 in one prompt, 262 us, 525 TFLOP/s of the masked products; two
-// chunks of 512 tokens before 8192 positions, 8 / 4 heads of 256, 98 us, 510
-// TFLOP/s; seven prompts of 777 tokens, 12 / 4 heads of 64, 39 us.  What bounds
-// it: a unit of 128 tokens of two row tiles (hd 128) takes 3.4 us, of which the
-// MMAs and the exponentials each need 1.1: without loads and softmax the loop
-// takes 1.4, loads add 0.5, and the softmax the rest, two warps on an SM
+// Measured (in a graph, with the combine; then without loads, without softmax,
+// without either): 4096 bf16 tokens of 32 q and 16 kv heads of 128 in one prompt,
+// 273 us, 504 TFLOP/s of the masked products (252, 151, 134); chunks of 512 and
+// 365 tokens that end at 8192 and 5844 positions, 8 / 4 heads of 256, 102 us, 492
+// TFLOP/s (83, 82, 60); seven prompts of 246 to 777 tokens, 12 / 4 heads of 64,
+// 40 us (40, 28, 27).  What bounds it: at hd 128 the softmax, two warps on an SM
 // sub-partition not hiding each other's latencies (TMEM loads, the row's serial
-// maximum, the exponentials, the store of P).
+// maximum, the exponentials, the store of P); at hd 256, with one row tile and
+// one stage of K and V, the hand-offs between MMAs, loads and softmax in equal
+// parts; short prompts, the launches, Q, the first K and the join.
 //
 // Every wait is bounded; on expiry the kernel records kErrWait, every role
 // leaves its loop, TMEM is freed and the kernel returns.

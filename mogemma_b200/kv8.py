@@ -16,9 +16,14 @@ stream of the cache's device; the caller orders its own tensors between streams,
 the call its workspace and error word), so a decode loop that keeps its buffers pays for
 the checks once.  A bound call reads the tensors' contents anew every time: new
 rows, lengths and tables are written into the same tensors.  It may be captured
-into a CUDA graph; the call object then has to live as long as the graph.  An
-attention call has a workspace of its own unless one is given; calls that may
-run at the same time must not share one.
+into a CUDA graph; the call object then has to live as long as the graph.
+
+An attention call has a workspace of its own unless one is given: up to 39 MB
+(prompts).  Calls that may run at the same time must not share
+one; calls that follow each other may, as a model's layers should:
+
+    ws = torch.empty(cache.workspace_bytes(batch, heads), dtype=torch.uint8, device="cuda")
+    calls = [c.attention_call(batch, q, out, workspace=ws) for c in caches]
 """
 
 from __future__ import annotations

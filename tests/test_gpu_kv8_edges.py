@@ -474,3 +474,27 @@ def test_many_heads_to_a_kv_head(dim, n, group) -> None:
     q = w.rand(w.rows, group, dim, dtype=F16)
     out = w.cache.attention(w.batch, q, window=200)
     _check_attention(w, q, out, scale=dim**-0.5, window=200)
+
+
+def test_layers_share_one_workspace() -> None:
+    """Calls that follow each other, of both kernels and several head dims, over one workspace, eager and in a graph."""
+    worlds = [World([(n, 700), (n, 3001)], kv_heads=2, dim=dim, page=32, seed=i)
+              for i, (n, dim) in enumerate([(1, 128), (40, 64), (1, 256), (50, 256), (7, 128)])]
+    qs = [w.rand(w.rows, 8, w.cache.head_dim, dtype=BF16) for w in worlds]
+    want = [w.cache.attention(w.batch, q) for w, q in zip(worlds, qs)]
+    size = max(w.cache.workspace_bytes(w.batch, 8) for w in worlds)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    outs = [torch.zeros_like(q) for q in qs]
+    calls = [w.cache.attention_call(w.batch, q, o, workspace=ws) for w, q, o in zip(worlds, qs, outs)]
+    for call in calls:
+        call()
+    assert all(torch.equal(o, x) for o, x in zip(outs, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in calls:
+            call()
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        assert all(torch.equal(o, x) for o, x in zip(outs, want))
