@@ -224,7 +224,8 @@ mg_status mg_set_debug(mg_model *m, uint64_t wait_budget_ns, int32_t stall_phase
  * 3 keys done, 4 values, 5 values done, 6 queries, 7 scores, 8 weights,
  * 9 answers, 10 scales, 11 the halves of a row (head dim 256), 12 the end).  The
  * waits on it run out, the call's err_dev receives MG_KV8_ERR_WAIT, and the
- * kernel ends; calls after the hook is cleared run as before. */
+ * kernel ends; calls after the hook is cleared run as before (a graph captured under
+ * it keeps it). */
 mg_status mg_kv8_set_debug(uint64_t wait_budget_ns, int32_t stall);
 
 /* ---- inspection (tests) ---- */

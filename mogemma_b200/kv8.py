@@ -282,7 +282,8 @@ class KV8Cache:
 
     def attention_call(self, batch: KV8Batch, q: torch.Tensor, out: torch.Tensor, *, scale: float | None = None,
                        window: int = 0, workspace: torch.Tensor | None = None) -> KV8Call:
-        """Binds ``mg_kv8_attention``: q and out [rows, heads, head dim]; scale defaults to head_dim ** -0.5; window 0:
+        """Binds ``mg_kv8_attention``: q and out [rows, heads, head dim], bfloat16 or float16 (which an append of float32
+        rows may write as its q_out); scale defaults to head_dim ** -0.5; window 0:
         every earlier position.  workspace: a uint8 tensor of at least ``workspace_bytes``."""
         d = self.head_dim
         _rows("q", q, self.device, d)
