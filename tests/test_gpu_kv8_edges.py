@@ -498,3 +498,18 @@ def test_layers_share_one_workspace() -> None:
             o.zero_()
         graph.replay()
         assert all(torch.equal(o, x) for o, x in zip(outs, want))
+
+
+@pytest.mark.parametrize("max_q", [1, 7, 40, 4000])
+def test_a_step_without_tokens_touches_nothing(max_q) -> None:
+    """Every sequence idle, though the row tensors have rows (a captured step between two requests)."""
+    w = World([(0, 100), (0, 0), (0, 33)], kv_heads=2, dim=64, page=16, extra_rows=5, max_q=max_q)
+    k, v, more = _append_args(w, 2, F16)
+    before, out = _snapshot(w), w.rand(w.rows, 4, 64, dtype=F16)
+    was = out.clone()
+    w.cache.append(w.batch, k, v, **more)
+    w.cache.attention(w.batch, more["q"], out)
+    w.batch.check()
+    assert torch.equal(out, was) and bool((more["q_out"] == 7.0).all())
+    for x, old in zip(_snapshot(w), before):
+        assert torch.equal(x.view(torch.uint8), old.view(torch.uint8))
