@@ -53,7 +53,8 @@ Batch batch_of(const mg_kv8_batch *b);
 // kv8_prompt.cu
 constexpr int kPromptUnit = 128;
 // What an item's start and end cost, in units: with 0, 3, 6 the 27B prompt takes 322, 270, 282 us, chunks of 512 and 365
-// tokens at 8192 and 5844 positions (hd 256) 105, 97, 101, ragged prompts of hd 64 41.8, 39.4, 41.4, two prompts of 300 tokens 23.4 each.
+// tokens at 8192 and 5844 positions (hd 256) 105, 97, 101, ragged prompts of hd 64 41.8, 39.4, 41.4, two prompts of 300
+// tokens 23.4 each.
 constexpr int kPromptExtra = 3;
 int prompt_rows(int hd);
 cudaError_t launch_prompt(const AttnArgs &p, int hd, bool f16, int ctas, cudaStream_t s);

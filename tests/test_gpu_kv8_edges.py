@@ -62,7 +62,8 @@ def _set_values(w, b, at, row):
 
 
 # P is rounded to fp16 as 2^lift times its ratio to the row's largest so far
-@pytest.mark.parametrize(("n", "dim", "group", "lift"), [(1, 256, 4, 15), (1, 64, 1, 15), (6, 128, 2, 15), (40, 64, 1, 8), (70, 128, 2, 8), (20, 256, 4, 8)])
+@pytest.mark.parametrize(("n", "dim", "group", "lift"), [
+    (1, 256, 4, 15), (1, 64, 1, 15), (6, 128, 2, 15), (40, 64, 1, 8), (70, 128, 2, 8), (20, 256, 4, 8)])
 @pytest.mark.parametrize("depth", [18.0, 25.2, 30.0])
 def test_a_long_tail_of_small_weights_counts(n, dim, group, lift, depth) -> None:
     """One token whose weight is 2^depth of every other's and whose value is 0, before 100000 equal ones; 600 streams over
@@ -93,14 +94,17 @@ def test_a_long_tail_of_small_weights_counts(n, dim, group, lift, depth) -> None
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize(("n", "dim", "group"), [(1, 64, 2), (4, 128, 3), (2, 256, 8), (50, 64, 2), (50, 128, 1), (20, 256, 3)])
+@pytest.mark.parametrize(("n", "dim", "group"), [
+    (1, 64, 2), (4, 128, 3), (2, 256, 8), (50, 64, 2), (50, 128, 1), (20, 256, 3)])
 def test_query_elements_far_below_their_rows_largest(n, dim, group, dtype) -> None:
     """The largest elements meet keys of zero, and the scores come from elements 2^-15 to 2^-31 of them."""
     w = World([(n, 300), (n, 65)], kv_heads=2, dim=dim, page=32, seed=dim)
     w.cache.k.view(torch.uint8)[..., ::4] = 0
     q = w.rand(w.rows, 2 * group, dim)
     bf16 = dtype == BF16
-    low = torch.randint(24, 31, q.shape, device="cuda", generator=w.g) if bf16 else torch.full(q.shape, 15, device="cuda")
+    low = torch.full(q.shape, 15, device="cuda")
+    if bf16:
+        low = torch.randint(24, 31, q.shape, device="cuda", generator=w.g)
     q = (q.clamp(-3.9, 3.9).abs().clamp(min=1.0).copysign(q) * torch.exp2(-low.float()))  # bits down to 2^-38 of 1
     q[..., ::4] = 1.5 if bf16 else 60000.0
     q = q.to(dtype)
@@ -235,10 +239,11 @@ def test_a_call_bound_on_one_stream_and_captured_on_another() -> None:
 
 
 def test_caches_whose_vectors_share_memory_are_refused() -> None:
-    codes, scales = torch.zeros(40_000, dtype=torch.uint8, device="cuda"), [torch.ones(3, 2, 2, device="cuda") for _ in range(2)]
+    codes = torch.zeros(40_000, dtype=torch.uint8, device="cuda")
+    scales = [torch.ones(3, 2, 2, device="cuda") for _ in range(2)]
     shape = (3, 2, 32, 64)
-    k, v = (codes[i:].as_strided(shape, (6144, 3072, 96, 1)) for i in (0, 18_448))
-    for strides in ((4096, 2048, 64), (4096, 64, 128), (2048, 6144, 64), (6144, 3072, 96)):
+    k, v = (codes[i:].as_strided(shape, (5120, 2560, 80, 1)) for i in (0, 18_448))
+    for strides in ((4096, 2048, 64), (4096, 64, 128), (2048, 6144, 64), (5120, 2560, 80)):
         KV8Cache.wrap(*(x.as_strided(shape, (*strides, 1), x.storage_offset()) for x in (k, v)), *scales)
     for strides in ((64, 2048, 64), (4096, 2048, 48), (4096, 64, 64), (4096, 1024, 64), (4096, 0, 64), (0, 2048, 64)):
         with pytest.raises(ValueError, match="must not overlap"):
@@ -379,7 +384,8 @@ def test_starts_out_of_bounds_hide_their_own_sequence(start, max_q) -> None:
 
 # ---------------------------------------------------------------- far apart
 @pytest.mark.parametrize(("n", "dim", "group", "window"), [
-    (1, 64, 1, 0), (1, 256, 4, 0), (3, 128, 3, 0), (40, 64, 2, 0), (20, 256, 2, 0), (1, 128, 2, 70_001), (33, 128, 1, 70_001)])
+    (1, 64, 1, 0), (1, 256, 4, 0), (3, 128, 3, 0), (40, 64, 2, 0), (20, 256, 2, 0),
+    (1, 128, 2, 70_001), (33, 128, 1, 70_001)])
 def test_attention_over_300000_positions(n, dim, group, window) -> None:
     w = World([(n, 300_001), (n, 131_072)], kv_heads=1, dim=dim, page=128, seed=2)
     q = w.rand(w.rows, group, dim, dtype=BF16)
@@ -392,7 +398,8 @@ def test_offsets_beyond_32_bits(n) -> None:
     """Pages behind 2^32 bytes of codes, and rows 2^31 elements apart."""
     dim, kv_heads, heads, page, pages = 256, 4, 8, 256, 20_000
     w = World([(n, 700), (n, 900)], kv_heads=kv_heads, dim=dim, page=page)
-    far = [torch.empty(pages, kv_heads, page, dim, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)]
+    far = [torch.empty(pages, kv_heads, page, dim, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+           for _ in range(2)]
     scales = [torch.empty(pages, kv_heads, page // 16, device="cuda") for _ in range(2)]
     move = pages - w.cache.num_pages
     for new, old in zip((*far, *scales), (w.cache.k, w.cache.v, w.cache.k_scale, w.cache.v_scale)):
@@ -404,7 +411,8 @@ def test_offsets_beyond_32_bits(n) -> None:
     # two rows at the ends of a long tensor each, or all of them near its start
     step = 2**31 if w.rows == 2 else 4 * heads * dim
     room = torch.empty(step * (w.rows - 1) + 4 * heads * dim, dtype=BF16, device="cuda")
-    at = [room[i * heads * dim:].as_strided((w.rows, h, dim), (step, dim, 1)) for i, h in enumerate((heads, heads, kv_heads, kv_heads))]
+    at = [room[i * heads * dim:].as_strided((w.rows, h, dim), (step, dim, 1))
+          for i, h in enumerate((heads, heads, kv_heads, kv_heads))]
     q, out, k, v = at
     for x in (q, k, v):
         x.copy_(w.rand(*x.shape))
